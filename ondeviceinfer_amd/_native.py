@@ -1,5 +1,5 @@
-"""ctypes binding of ``libondeviceinfer_wq.so`` (the C ABI in ``include/ondeviceinfer_wq.h``
-and ``include/ondeviceinfer_decode.h``).
+"""ctypes binding of ``libondeviceinfer_wq.so`` (the C ABI in ``include/ondeviceinfer_wq.h``,
+``include/ondeviceinfer_decode.h`` and ``include/ondeviceinfer_paged.h``).
 
 torch is imported first so its bundled HIP runtime (``libamdhip64.so.7``) is
 the one the library binds to: the kernels then run in torch's context and on
@@ -93,6 +93,12 @@ _SIGNATURES = {
     'wq_host_device_pointer': [_P, ctypes.POINTER(ctypes.c_void_p)],
     'wq_embed_rows': [_P, _I64, _I64, _P, _I64, _P, _P, _P],
     'wq_lm_head_rmsnorm': [_P, _I64, _P, _P, _I64, ctypes.c_float, _P, _I64, _P, _P, _P, ctypes.c_size_t, _P],
+    # include/ondeviceinfer_paged.h
+    'wq_paged_append': [_P, _I64, _I64, _I64, _I64, _P, _P, ctypes.c_float, _P, _P, _I64, _P, _P, _I64, _P, _P, _I64,
+                        _P, _I64, _P, _I64, _I64, _I64, _P, _P],
+    'wq_paged_attention_workspace_size': [_I64, _I64, _I64, _I64, _I64, _I64, _I64, _SIZE_P],
+    'wq_paged_attention': [_P, _I64, _I64, _I64, _I64, _P, _I64, _P, _I64, _I64, _I64, _P, _I64, _P, _P, _I64, _P,
+                           ctypes.c_float, _P, _P, ctypes.c_size_t, _P],
 }
 EXPORTED_SYMBOLS = ('wq_last_error', *_SIGNATURES)
 
@@ -148,6 +154,15 @@ def _call(name: str, *args) -> None:
 def _stream(device: torch.device) -> int:
     # The raw handle, without building a torch Stream object (0.1 against 1.9 us per call).
     return torch._C._cuda_getCurrentRawStream(device.index)
+
+
+def _call_on(device: torch.device, name: str, *args) -> None:
+    """``_call`` with ``device`` as the current one: operands may live on another device than the caller's."""
+    if torch._C._cuda_getDevice() == device.index:
+        _call(name, *args)
+    else:
+        with torch.cuda.device(device):
+            _call(name, *args)
 
 
 def _ptr(t: torch.Tensor | None) -> int | None:
@@ -948,6 +963,118 @@ def argmax_f16(x: torch.Tensor, *, out: torch.Tensor | None = None,
         workspace = shared_workspace(device, argmax_f16_workspace_size(n), ('argmax_f16', n))
     _call('wq_argmax_f16', _ptr(_aligned(x)), n, _ptr(out), workspace.data_ptr(),
           workspace.numel() * workspace.element_size(), _stream(device))
+    return out
+
+
+# ----------------------------------------------------------------------------- paged cache
+
+def _page_stride(t: torch.Tensor, name: str) -> int:
+    """The distance of two pages in elements; a page itself is contiguous."""
+    _, heads, rows, dim = t.shape
+    if t.dtype != torch.float16:
+        raise TypeError(f'{name}: expected {torch.float16}, got {t.dtype}')
+    stride = t.stride()
+    if stride[1:] != (rows * dim, dim, 1) and not t[:1].is_contiguous():
+        raise ValueError(f'{name}: a page [{heads}, {rows}, {dim}] must be contiguous')
+    return stride[0] if t.shape[0] > 1 else heads * rows * dim
+
+
+def _check_batch(page_table: torch.Tensor, query_starts: torch.Tensor, seq_lens: torch.Tensor) -> tuple[int, int]:
+    """(sequences, table width) of a batch's device tensors."""
+    if page_table.dim() != 2:
+        raise ValueError(f'page_table must be [sequences, pages], got {tuple(page_table.shape)}')
+    sequences, width = page_table.shape
+    _check(page_table, torch.int32, (sequences, width), 'page_table')
+    _check(query_starts, torch.int32, (sequences + 1,), 'query_starts')
+    _check(seq_lens, torch.int32, (sequences,), 'seq_lens')
+    return sequences, width
+
+
+def _check_pages(key_pages: torch.Tensor, value_pages: torch.Tensor) -> tuple[int, int, int, int]:
+    """(pages, kv_heads, page_size, head_dim) of a pool."""
+    if key_pages.dim() != 4 or key_pages.shape != value_pages.shape:
+        raise ValueError('key_pages and value_pages must both be [pages, kv_heads, page_size, head_dim], got '
+                         f'{tuple(key_pages.shape)} and {tuple(value_pages.shape)}')
+    return tuple(key_pages.shape)
+
+
+def paged_append(qkv: torch.Tensor, q_heads: int, q_norm: torch.Tensor | None, k_norm: torch.Tensor | None, eps: float,
+                 cos_table: torch.Tensor, sin_table: torch.Tensor, key_pages: torch.Tensor, value_pages: torch.Tensor,
+                 page_table: torch.Tensor, query_starts: torch.Tensor, seq_lens: torch.Tensor,
+                 positions: torch.Tensor | None = None, q_out: torch.Tensor | None = None) -> torch.Tensor:
+    """q/k RMSNorm + rotation of the new tokens' fused QKV rows; k and v go to
+    their sequences' pages, q comes back as ``[tokens, q_heads, head_dim]``
+    (``wq_paged_append``)."""
+    device = _require_gpu(qkv, q_norm, k_norm, cos_table, sin_table, key_pages, value_pages, page_table, query_starts,
+                          seq_lens, positions, q_out)
+    pages, kv_heads, page_size, head_dim = _check_pages(key_pages, value_pages)
+    k_stride, v_stride = _page_stride(key_pages, 'key_pages'), _page_stride(value_pages, 'value_pages')
+    sequences, width = _check_batch(page_table, query_starts, seq_lens)
+    if qkv.dim() != 2:
+        raise ValueError(f'qkv must be [tokens, (q_heads + 2 kv_heads) * head_dim], got {tuple(qkv.shape)}')
+    tokens = qkv.shape[0]
+    _check(qkv, torch.float16, (tokens, (q_heads + 2 * kv_heads) * head_dim), 'qkv')
+    for t, name in ((q_norm, 'q_norm'), (k_norm, 'k_norm')):
+        if t is not None:
+            _check(t, torch.float16, (head_dim,), name)
+    if cos_table.dim() != 2:
+        raise ValueError(f'cos_table must be [positions, {head_dim}], got {tuple(cos_table.shape)}')
+    for t, name in ((cos_table, 'cos_table'), (sin_table, 'sin_table')):
+        _check(t, torch.float16, (cos_table.shape[0], head_dim), name)
+    if positions is not None:
+        _check(positions, torch.int32, (tokens,), 'positions')
+    if q_out is None:
+        q_out = torch.empty(tokens, q_heads, head_dim, dtype=torch.float16, device=device)
+    else:
+        _check(q_out, torch.float16, (tokens, q_heads, head_dim), 'q_out')
+    _call_on(device, 'wq_paged_append', _ptr(qkv), tokens, q_heads, kv_heads, head_dim, _ptr(q_norm), _ptr(k_norm),
+             float(eps), _ptr(cos_table), _ptr(sin_table), cos_table.shape[0], _ptr(positions), _ptr(page_table), width,
+             _ptr(query_starts), _ptr(seq_lens), sequences, _ptr(key_pages), k_stride, _ptr(value_pages), v_stride,
+             pages, page_size, _ptr(q_out), _stream(device))
+    return q_out
+
+
+@functools.lru_cache(maxsize=1024)   # a pure function of the shape, asked for on every call
+def paged_attention_workspace_size(tokens: int, sequences: int, q_heads: int, kv_heads: int, head_dim: int,
+                                   table_width: int, page_size: int) -> int:
+    b = ctypes.c_size_t()
+    _call('wq_paged_attention_workspace_size', tokens, sequences, q_heads, kv_heads, head_dim, table_width, page_size,
+          ctypes.byref(b))
+    return b.value
+
+
+def paged_attention(query: torch.Tensor, key_pages: torch.Tensor, value_pages: torch.Tensor, page_table: torch.Tensor,
+                    query_starts: torch.Tensor, seq_lens: torch.Tensor, scale: float,
+                    tree_mask: torch.Tensor | None = None, out: torch.Tensor | None = None,
+                    workspace: torch.Tensor | None = None) -> torch.Tensor:
+    """Attention of the new tokens ``[tokens, q_heads, head_dim]`` over their
+    sequences' pages, causal or (``tree_mask`` int64 ``[tokens]``) a tree of
+    drafted tokens (``wq_paged_attention``)."""
+    device = _require_gpu(query, key_pages, value_pages, page_table, query_starts, seq_lens, tree_mask, out, workspace)
+    pages, kv_heads, page_size, head_dim = _check_pages(key_pages, value_pages)
+    k_stride, v_stride = _page_stride(key_pages, 'key_pages'), _page_stride(value_pages, 'value_pages')
+    sequences, width = _check_batch(page_table, query_starts, seq_lens)
+    if query.dim() != 3 or query.shape[2] != head_dim:
+        raise ValueError(f'query must be [tokens, q_heads, {head_dim}], got {tuple(query.shape)}')
+    tokens, q_heads, _ = query.shape
+    _check(query, torch.float16, (tokens, q_heads, head_dim), 'query')
+    if tree_mask is not None:
+        _check(tree_mask, torch.int64, (tokens,), 'tree_mask')
+    if out is None:
+        out = torch.empty_like(query)
+    else:
+        _check(out, torch.float16, (tokens, q_heads, head_dim), 'out')
+    ws_ptr, ws_bytes = None, 0
+    if workspace is None:
+        ws_bytes = paged_attention_workspace_size(tokens, sequences, q_heads, kv_heads, head_dim, width, page_size)
+        if ws_bytes:   # split partials only (no counters): any scratch of this call's own
+            workspace = query.new_empty(ws_bytes, dtype=torch.uint8)
+            ws_ptr = workspace.data_ptr()
+    else:
+        ws_ptr, ws_bytes = workspace.data_ptr(), workspace.numel() * workspace.element_size()
+    _call_on(device, 'wq_paged_attention', _ptr(query), tokens, q_heads, kv_heads, head_dim, _ptr(key_pages), k_stride,
+             _ptr(value_pages), v_stride, pages, page_size, _ptr(page_table), width, _ptr(query_starts),
+             _ptr(seq_lens), sequences, _ptr(tree_mask), float(scale), _ptr(out), ws_ptr, ws_bytes, _stream(device))
     return out
 
 

@@ -1,0 +1,526 @@
+// Grouped-query attention over the paged key/value cache: ragged new tokens,
+// causal or a tree of drafted ones.
+//
+// The new tokens of a sequence times the query heads of one kv head are the
+// rows that share its keys; row r of a sequence is token r / G, head r % G.
+// Rows are taken in tiles of 16, the keys of a tile are cut into chunks when
+// there are too few tiles to fill the machine, and every (sequence, tile,
+// chunk, kv head) is one workgroup.
+#include "ondeviceinfer_paged.h"
+#include "wq_paged.h"
+#include "wq_status.h"
+
+#include <math.h>
+
+namespace wq {
+namespace {
+
+constexpr int kKeys = 32;          // keys per step of a wave
+constexpr int kWaves = 4;          // waves per workgroup
+constexpr int kMaxPagedGroup = 16; // q heads per kv head
+
+struct PagedArgs {
+  const half_t *q, *kp, *vp;
+  const int32_t *table, *starts, *lens;
+  const int64_t* mask;          // nullptr: causal
+  half_t* out;
+  float* part_o;                // [slots][KV][R][128] unnormalized outputs of split tiles
+  float2_t* part_ml;            // [slots][KV][R] (max in log2 units, sum)
+  int64_t k_stride, v_stride;   // elements from page to page
+  float scale_log2;
+  int sequences, tokens, H, KV, G, width, page_size, num_pages;
+  int slots;                    // (tile, chunk) places the grid has per kv head
+  int spare;                    // of those, beyond the largest possible number of tiles (0: nothing is split)
+  int min_blocks;               // smallest chunk, in steps of kKeys keys
+};
+
+// One sequence's share of the call, from the device's starts and lengths.
+struct Seq {
+  int start, count, base;   // first token, tokens, positions before them (may be negative: refused by the rows)
+  int keys;                 // positions that may be attended; past the table one more, which has no page
+  int tiles, blocks;
+};
+
+template <int R>
+__device__ __forceinline__ Seq read_seq(const PagedArgs& a, int b) {
+  Seq s{};
+  if (b >= a.sequences) return s;
+  const int s0 = a.starts[b], s1 = a.starts[b + 1], len = a.lens[b];
+  if (s0 < 0 || s1 > a.tokens || s1 <= s0) return s;
+  s.start = s0;
+  s.count = s1 - s0;
+  s.base = (int)max((int64_t)len - s.count, -((int64_t)1 << 30));
+  s.keys = min(max(len, 0), a.width * a.page_size + 1);
+  s.tiles = (s.count * a.G + R - 1) / R;
+  s.blocks = (s.keys + kKeys - 1) / kKeys;
+  return s;
+}
+
+// Where flat place `place` of the call lies: a (tile, chunk) slot, or with
+// BY_TILE a tile.  Every wave computes it for itself: two reductions and a
+// scan over the sequences, 64 at a time.
+//   chunk length C = max(min_blocks, ceil(sum_b tiles_b blocks_b / spare)), so
+//   that sum_b tiles_b ceil(blocks_b / C) <= tiles + spare <= slots.
+struct Place {
+  Seq s;
+  int b, tile, chunk, chunks;
+  int64_t slot0;   // slot of the sequence's tile 0, chunk 0
+  bool found;
+};
+
+template <int R, bool BY_TILE>
+__device__ __forceinline__ Place find_place(const PagedArgs& a, int place, int lane) {
+  int chunk_blocks = 0x7fffffff;
+  if (a.spare > 0) {
+    int64_t work = 0;
+    for (int b0 = 0; b0 < a.sequences; b0 += 64) {
+      const Seq s = read_seq<R>(a, b0 + lane);
+      work += (int64_t)s.tiles * s.blocks;
+    }
+    work = wave_sum_i64(work);
+    const int64_t c = (work + a.spare - 1) / a.spare;
+    chunk_blocks = (int)max(min(c, (int64_t)0x7fffffff), (int64_t)a.min_blocks);
+  }
+  Place p{};
+  // Starts that do not follow one another could name more tiles than the grid has: 64-bit sums, and such places
+  // are never found or merged.
+  int64_t slots_before = 0, before = 0;
+  for (int b0 = 0; b0 < a.sequences; b0 += 64) {
+    const Seq s = read_seq<R>(a, b0 + lane);
+    const int chunks = s.blocks > chunk_blocks ? (s.blocks + chunk_blocks - 1) / chunk_blocks : 1;
+    const int slots = s.tiles * chunks;
+    int upto = slots, tiles_upto = s.tiles;   // inclusive scans over the lanes
+#pragma unroll
+    for (int o = 1; o < 64; o <<= 1) {
+      const int u = __shfl_up(upto, o), v = __shfl_up(tiles_upto, o);
+      if (lane >= o) {
+        upto += u;
+        tiles_upto += v;
+      }
+    }
+    const int mine = BY_TILE ? s.tiles : slots;
+    const int end = BY_TILE ? tiles_upto : upto;
+    const int64_t want = place - before;
+    const uint64_t hit = __builtin_amdgcn_ballot_w64(want >= end - mine && want < end);
+    if (hit) {
+      const int l = __builtin_ctzll(hit);
+      p.found = true;
+      p.b = b0 + l;
+      p.s.start = __builtin_amdgcn_readlane(s.start, l);
+      p.s.count = __builtin_amdgcn_readlane(s.count, l);
+      p.s.base = __builtin_amdgcn_readlane(s.base, l);
+      p.s.keys = __builtin_amdgcn_readlane(s.keys, l);
+      p.s.tiles = __builtin_amdgcn_readlane(s.tiles, l);
+      p.s.blocks = __builtin_amdgcn_readlane(s.blocks, l);
+      p.chunks = __builtin_amdgcn_readlane(chunks, l);
+      p.slot0 = slots_before + __builtin_amdgcn_readlane(upto - slots, l);
+      const int rest = (int)want - __builtin_amdgcn_readlane(end - mine, l);
+      p.tile = rest % p.s.tiles;
+      p.chunk = rest / p.s.tiles;
+      return p;
+    }
+    slots_before += __builtin_amdgcn_readlane(upto, 63);
+    before += __builtin_amdgcn_readlane(BY_TILE ? tiles_upto : upto, 63);
+  }
+  return p;
+}
+
+// The wave's 16-key groups of pages, one per lane: page number (-1: none) and
+// first row of the group in its page.
+struct Groups {
+  int page, row;
+  uint64_t bad;   // lanes whose group has no page
+};
+
+__device__ __forceinline__ Groups load_groups(const PagedArgs& a, int b, int first, int last, int lane) {
+  Groups g;
+  const unsigned key = 16u * (unsigned)min(first + lane, last);   // groups past the chunk's keys reread its last one
+  const unsigned entry = key / (unsigned)a.page_size;
+  g.row = (int)(key - entry * a.page_size);
+  g.page = entry < (unsigned)a.width ? a.table[(size_t)b * a.width + entry] : -1;
+  const bool ok = g.page >= 0 && g.page < a.num_pages;
+  g.bad = __builtin_amdgcn_ballot_w64(!ok);
+  if (!ok) {
+    g.page = 0;
+    g.row = 0;
+  }
+  return g;
+}
+
+// grid = slots * KV workgroups of four waves (flat id f: kv head f % KV, place
+// f / KV; with 8 kv heads the workgroups of one head share an XCD's L2).  Wave
+// w takes the w-th quarter of the chunk's 32-key steps and runs its own online
+// softmax over them for the tile's 16 rows, without barriers and without LDS:
+//   scores  S^T = K . Q^T on the matrix cores (16x16x32): A = 16 keys (lane
+//           (i, kb) = (l % 16, l / 16) holds key i, d = 32 ks + 8 kb ..), B =
+//           Q^T; lane (i, kb) receives keys 4 kb .. 4 kb + 3 of row i;
+//   values  lane (i, kb) loads d = 8 i .. 8 i + 7 of the keys 4 kb + e and
+//           16 + 4 kb + e: eight keys by eight d, transposed in registers (32
+//           byte permutes), which makes them the A operand of O^T = V^T . P^T
+//           whose m index i of tile t is d = 8 i + t and whose k slots are the
+//           keys that the same lane's scores hold.  P^T needs no exchange
+//           either: the lane's eight probabilities are its B operand;
+//   output  lane (i, kb) holds row i, d = 8 (4 kb + v) + t in acc[t][v].
+// The next step's keys are requested as soon as the scores have consumed the
+// present ones, the values likewise, so that both are in flight during the
+// softmax of the other.
+__global__ __launch_bounds__(256, 2) void paged_attention_rows_kernel(PagedArgs a) {
+  constexpr int R = 16, D = kPagedDim;
+  __shared__ __attribute__((aligned(16))) float red[kWaves][R][D];
+  __shared__ float2_t mlw[kWaves][R];
+  const int tid = threadIdx.x, lane = tid & 63;
+  const int wave = __builtin_amdgcn_readfirstlane(tid >> 6);
+  const int i = lane & 15, kb = lane >> 4;
+  const int kvh = blockIdx.x % a.KV, slot = blockIdx.x / a.KV;
+  const Place p = find_place<R, false>(a, slot, lane);
+  if (!p.found) return;
+
+  // The row of this lane, its token and what it may attend.
+  const int rows = p.s.count * a.G;
+  const int r = p.tile * R + i;
+  const int tok = min(r, rows - 1) / a.G;
+  const int head = kvh * a.G + min(r, rows - 1) - tok * a.G;
+  const int first_tok = (p.tile * R) / a.G;
+  const int last_tok = (min(p.tile * R + R, rows) - 1) / a.G;
+  const bool tree = a.mask != nullptr;
+  const bool refused = tree && p.s.count > kMaxTreeTokens;
+  const int64_t bits = tree ? a.mask[p.s.start + tok] : 0;
+  const int limit = p.s.base + tok;                 // causal: the last position attended
+  // Keys of the tile, and the first key that not all of its rows attend.
+  const int keys = refused ? 0 : tree ? p.s.keys : max(0, min(p.s.keys, p.s.base + last_tok + 1));
+  const int ragged = tree ? p.s.base : p.s.base + first_tok + 1;
+  const int per = p.s.blocks / p.chunks, extra = p.s.blocks % p.chunks;
+  const int c0 = p.chunk * per + min(p.chunk, extra), c1 = c0 + per + (p.chunk < extra ? 1 : 0);
+  const int nblk = min(c1, (keys + kKeys - 1) / kKeys) - c0;   // steps of this workgroup (may be negative)
+  const int w0 = nblk > 0 ? c0 + nblk * wave / kWaves : 0;
+  const int w1 = nblk > 0 ? c0 + nblk * (wave + 1) / kWaves : 0;
+
+  const half_t* qp = a.q + ((size_t)(p.s.start + tok) * a.H + head) * D + 8 * kb;
+  half8_t qf[4];
+#pragma unroll
+  for (int ks = 0; ks < 4; ++ks) qf[ks] = ld_h8(qp + 32 * ks);
+
+  float4_t acc[8];
+#pragma unroll
+  for (int t = 0; t < 8; ++t) acc[t] = float4_t{0.f, 0.f, 0.f, 0.f};
+  float m_run = -INFINITY, l_run = 0.f;   // of row i; l_run this lane's keys only
+
+  if (w0 < w1) {
+    const size_t head_off = (size_t)kvh * a.page_size * D;
+    const half_t* kbase = a.kp + head_off + (size_t)i * D + 8 * kb;
+    const half_t* vbase = a.vp + head_off + (size_t)(4 * kb) * D + 8 * i;
+    const int last_group = (keys - 1) >> 4;
+    int g0 = 2 * w0;
+    Groups g = load_groups(a, p.b, g0, last_group, lane);
+    uint4_t kr[2][4], vr[8];
+    bool kbad[2];
+    auto load_keys = [&](int blk) {
+#pragma unroll
+      for (int h = 0; h < 2; ++h) {
+        const int l = 2 * blk + h - g0;
+        const half_t* src = kbase + (size_t)__builtin_amdgcn_readlane(g.page, l) * a.k_stride +
+                            (size_t)__builtin_amdgcn_readlane(g.row, l) * D;
+#pragma unroll
+        for (int ks = 0; ks < 4; ++ks) kr[h][ks] = *reinterpret_cast<const uint4_t*>(src + 32 * ks);
+        kbad[h] = (g.bad >> l) & 1;
+      }
+    };
+    auto load_values = [&](int blk) {
+#pragma unroll
+      for (int h = 0; h < 2; ++h) {
+        const int l = 2 * blk + h - g0;
+        const half_t* src = vbase + (size_t)__builtin_amdgcn_readlane(g.page, l) * a.v_stride +
+                            (size_t)__builtin_amdgcn_readlane(g.row, l) * D;
+#pragma unroll
+        for (int e = 0; e < 4; ++e) vr[4 * h + e] = *reinterpret_cast<const uint4_t*>(src + (size_t)e * D);
+      }
+    };
+    load_keys(w0);
+    load_values(w0);
+    for (int blk = w0; blk < w1; ++blk) {
+      const int k0 = blk * kKeys;
+      float4_t sc[2];
+#pragma unroll
+      for (int h = 0; h < 2; ++h) {
+        sc[h] = float4_t{0.f, 0.f, 0.f, 0.f};
+#pragma unroll
+        for (int ks = 0; ks < 4; ++ks) sc[h] = mfma16(__builtin_bit_cast(half8_t, kr[h][ks]), qf[ks], sc[h]);
+        if (kbad[h]) sc[h] = float4_t{NAN, NAN, NAN, NAN};
+      }
+      // A wave's groups run out after 32 steps; the values of this step are on their way already.
+      const bool more = blk + 1 < w1;
+      if (more && 2 * (blk + 1) - g0 >= 64) {
+        g0 = 2 * (blk + 1);
+        g = load_groups(a, p.b, g0, last_group, lane);
+      }
+      if (more) load_keys(blk + 1);
+      if (k0 + kKeys > ragged || k0 + kKeys > keys) {
+#pragma unroll
+        for (int h = 0; h < 2; ++h)
+#pragma unroll
+          for (int v = 0; v < 4; ++v) {
+            const int key = k0 + 16 * h + 4 * kb + v;
+            const int j = key - p.s.base;
+            const bool seen = key < keys && (tree ? j < 0 || ((bits >> (j & 63)) & 1) : key <= limit);
+            if (!seen) sc[h][v] = -INFINITY;
+          }
+      }
+      float mb = -INFINITY;
+#pragma unroll
+      for (int h = 0; h < 2; ++h)
+#pragma unroll
+        for (int v = 0; v < 4; ++v) mb = fmaxf(mb, sc[h][v]);
+      mb = fmaxf(mb, __shfl_xor(mb, 16));
+      mb = fmaxf(mb, __shfl_xor(mb, 32));
+      const float m_new = fmaxf(m_run, mb * a.scale_log2);   // scale > 0
+      const float m_use = m_new == -INFINITY ? 0.f : m_new;
+      const float alpha = exp2_hw(m_run - m_use);
+      m_run = m_new;
+      half8_t pb;
+      float ls = 0.f;
+#pragma unroll
+      for (int h = 0; h < 2; ++h)
+#pragma unroll
+        for (int v = 0; v < 4; ++v) {
+          const float pv = exp2_hw(__builtin_fmaf(sc[h][v], a.scale_log2, -m_use));
+          ls += pv;
+          pb[4 * h + v] = (half_t)pv;
+        }
+      l_run = l_run * alpha + ls;
+      if (__builtin_amdgcn_ballot_w64(alpha != 1.f) != 0) {
+#pragma unroll
+        for (int t = 0; t < 8; ++t)
+#pragma unroll
+          for (int v = 0; v < 4; ++v) acc[t][v] *= alpha;
+      }
+      if (k0 + kKeys > keys) {   // what lies behind the last key is not the sequence's: 0 * NaN would poison the sums
+#pragma unroll
+        for (int e = 0; e < 8; ++e)
+          if (k0 + 16 * (e >> 2) + 4 * kb + (e & 3) >= keys) vr[e] = uint4_t{0u, 0u, 0u, 0u};
+      }
+#pragma unroll
+      for (int t = 0; t < 8; ++t) {
+        uint4_t vt;
+#pragma unroll
+        for (int w = 0; w < 4; ++w) {
+          const uint32_t lo = vr[2 * w][t >> 1], hi = vr[2 * w + 1][t >> 1];
+          vt[w] = __builtin_amdgcn_perm(hi, lo, t & 1 ? 0x07060302u : 0x05040100u);
+        }
+        acc[t] = mfma16(__builtin_bit_cast(half8_t, vt), pb, acc[t]);
+      }
+      if (more) load_values(blk + 1);
+    }
+    l_run += __shfl_xor(l_run, 16);
+    l_run += __shfl_xor(l_run, 32);
+  }
+
+  // Combine the four waves.
+#pragma unroll
+  for (int v = 0; v < 4; ++v) {
+    float* dst = &red[wave][i][8 * (4 * kb + v)];
+    *reinterpret_cast<float4_t*>(dst) = float4_t{acc[0][v], acc[1][v], acc[2][v], acc[3][v]};
+    *reinterpret_cast<float4_t*>(dst + 4) = float4_t{acc[4][v], acc[5][v], acc[6][v], acc[7][v]};
+  }
+  if (kb == 0) mlw[wave][i] = float2_t{m_run, l_run};
+  __syncthreads();
+  // Thread (row, d8): row = tid / 16, d = 8 (tid % 16) ..
+  const int row = tid >> 4, d = 8 * (tid & 15);
+  if (p.tile * R + row >= rows) return;
+  float M = -INFINITY;
+#pragma unroll
+  for (int w = 0; w < kWaves; ++w) M = fmaxf(M, mlw[w][row].x);
+  const float Mu = M == -INFINITY ? 0.f : M;
+  float num[8];
+#pragma unroll
+  for (int e = 0; e < 8; ++e) num[e] = 0.f;
+  float den = 0.f;
+#pragma unroll
+  for (int w = 0; w < kWaves; ++w) {
+    const float wt = exp2_hw(mlw[w][row].x - Mu);
+    den += wt * mlw[w][row].y;
+#pragma unroll
+    for (int e = 0; e < 8; ++e) num[e] += wt * red[w][row][d + e];
+  }
+  if (p.chunks > 1) {
+    const size_t at = ((size_t)slot * a.KV + kvh) * R + row;
+    *reinterpret_cast<float4_t*>(a.part_o + at * D + d) = float4_t{num[0], num[1], num[2], num[3]};
+    *reinterpret_cast<float4_t*>(a.part_o + at * D + d + 4) = float4_t{num[4], num[5], num[6], num[7]};
+    if (d == 0) a.part_ml[at] = float2_t{M, den};
+    return;
+  }
+  const int rr = p.tile * R + row, t = rr / a.G;
+  half8_t o;
+#pragma unroll
+  for (int e = 0; e < 8; ++e) o[e] = refused ? (half_t)NAN : den == 0.f ? (half_t)0.f : (half_t)(num[e] / den);
+  *reinterpret_cast<half8_t*>(a.out + ((size_t)(p.s.start + t) * a.H + kvh * a.G + rr - t * a.G) * D + d) = o;
+}
+
+// The chunks of split tiles joined: grid = (tiles the call can have * KV, R /
+// 4), a wave per row, two elements of d per lane.  The weights 2^(m_c - M) of
+// up to 64 chunks are held one per lane and read out as each chunk is added,
+// in chunk order.
+template <int R>
+__global__ __launch_bounds__(256) void paged_attention_merge_kernel(PagedArgs a) {
+  constexpr int D = kPagedDim;
+  const int lane = threadIdx.x & 63;
+  const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
+  const int kvh = blockIdx.x % a.KV;
+  const Place p = find_place<R, true>(a, blockIdx.x / a.KV, lane);
+  if (!p.found || p.chunks == 1 || p.slot0 + (int64_t)p.s.tiles * p.chunks > a.slots) return;
+  const int row = 4 * blockIdx.y + wave;
+  const int rr = p.tile * R + row;
+  if (rr >= p.s.count * a.G) return;
+  auto at = [&](int chunk) {
+    return ((size_t)(p.slot0 + chunk * p.s.tiles + p.tile) * a.KV + kvh) * R + row;
+  };
+  float M = -INFINITY;
+  for (int c0 = 0; c0 < p.chunks; c0 += 64)
+    if (c0 + lane < p.chunks) M = fmaxf(M, a.part_ml[at(c0 + lane)].x);
+  M = wave_max_rl(M);
+  const float Mu = M == -INFINITY ? 0.f : M;
+  float den = 0.f;
+  float2_t num = {0.f, 0.f};
+  for (int c0 = 0; c0 < p.chunks; c0 += 64) {
+    const int n = min(64, p.chunks - c0);
+    const float2_t ml = lane < n ? a.part_ml[at(c0 + lane)] : float2_t{-INFINITY, 0.f};
+    const float w = exp2_hw(ml.x - Mu);
+    den += wave_sum_rl(w * ml.y);
+    for (int c = 0; c < n; c += 8) {
+      float2_t o[8];
+#pragma unroll
+      for (int u = 0; u < 8; ++u)
+        o[u] = *reinterpret_cast<const float2_t*>(a.part_o + at(c0 + min(c + u, n - 1)) * D + 2 * lane);
+#pragma unroll
+      for (int u = 0; u < 8; ++u) {
+        const float wc = c + u < n ? lane_f(w, min(c + u, 63)) : 0.f;
+        if (c + u < n) num += wc * o[u];
+      }
+    }
+  }
+  const bool refused = a.mask != nullptr && p.s.count > kMaxTreeTokens;
+  const int t = rr / a.G;
+  half2_t h;
+#pragma unroll
+  for (int e = 0; e < 2; ++e) {
+    const float n = num[e];
+    h[e] = refused ? (half_t)NAN : den == 0.f ? (half_t)0.f : (half_t)(n / den);
+  }
+  half_t* dst = a.out + ((size_t)(p.s.start + t) * a.H + kvh * a.G + rr - t * a.G) * D + 2 * lane;
+  *reinterpret_cast<half2_t*>(dst) = h;
+}
+
+// Places of the grid per kv head: the tiles the call can have at most, and as
+// many more for chunks as bring the workgroups to about four per compute unit.
+struct PagedPlan {
+  int64_t tiles, spare, slots;
+  int min_blocks;
+  size_t bytes;
+};
+
+constexpr int kTargetGroups = 1024;
+constexpr int kMinBlocks = 4;
+
+PagedPlan paged_plan(int64_t tokens, int64_t sequences, int64_t G, int64_t KV, int64_t width, int64_t page_size) {
+  constexpr int R = 16;
+  PagedPlan p{};
+  // sum_b ceil(count_b G / R) <= ceil(tokens G / R) + sequences, and no more tiles than rows.
+  p.tiles = (tokens * G + R - 1) / R + sequences;
+  if (p.tiles > tokens * ((G + R - 1) / R)) p.tiles = tokens * ((G + R - 1) / R);
+  p.min_blocks = kMinBlocks;
+  const int64_t blocks = width * page_size / kKeys + 1;
+  const int64_t spare = (kTargetGroups + KV - 1) / KV;
+  p.spare = blocks > kMinBlocks && p.tiles * KV < 4 * kTargetGroups ? spare : 0;
+  p.slots = p.tiles + p.spare;
+  p.bytes = p.spare ? (size_t)p.slots * KV * R * (kPagedDim + 2) * 4 : 0;
+  return p;
+}
+
+int paged_attention_check(int64_t q_heads, int64_t kv_heads) {
+  WQ_REQUIRE(q_heads > 0 && kv_heads > 0 && q_heads % kv_heads == 0, WQ_ERR_INVALID_ARGUMENT,
+             "q_heads (%lld) must be a positive multiple of kv_heads (%lld)", (long long)q_heads, (long long)kv_heads);
+  WQ_REQUIRE(q_heads / kv_heads <= kMaxPagedGroup, WQ_ERR_UNSUPPORTED, "at most %d query heads per kv head",
+             kMaxPagedGroup);
+  return WQ_OK;
+}
+
+}  // namespace
+}  // namespace wq
+
+using namespace wq;
+
+extern "C" int wq_paged_attention_workspace_size(int64_t tokens, int64_t sequences, int64_t q_heads,
+                                                 int64_t kv_heads, int64_t head_dim, int64_t table_width,
+                                                 int64_t page_size, size_t* bytes) {
+  WQ_REQUIRE(bytes, WQ_ERR_INVALID_ARGUMENT, "null pointer argument");
+  int rc = paged_attention_check(q_heads, kv_heads);
+  if (rc != WQ_OK) return rc;
+  const int64_t page = kv_heads * page_size * head_dim;
+  rc = paged_pool_check(head_dim, kv_heads, page, page, 1, page_size, table_width, sequences, tokens);
+  if (rc != WQ_OK) return rc;
+  *bytes = tokens && sequences
+               ? paged_plan(tokens, sequences, q_heads / kv_heads, kv_heads, table_width, page_size).bytes
+               : 0;
+  return WQ_OK;
+}
+
+extern "C" int wq_paged_attention(const uint16_t* q, int64_t tokens, int64_t q_heads, int64_t kv_heads,
+                                  int64_t head_dim, const uint16_t* key_pages, int64_t key_page_stride,
+                                  const uint16_t* value_pages, int64_t value_page_stride, int64_t num_pages,
+                                  int64_t page_size, const int32_t* page_table, int64_t table_width,
+                                  const int32_t* query_starts, const int32_t* seq_lens, int64_t sequences,
+                                  const int64_t* tree_mask, float scale, uint16_t* out, void* workspace,
+                                  size_t workspace_bytes, void* stream) {
+  int rc = paged_attention_check(q_heads, kv_heads);
+  if (rc != WQ_OK) return rc;
+  rc = paged_pool_check(head_dim, kv_heads, key_page_stride, value_page_stride, num_pages, page_size, table_width,
+                        sequences, tokens);
+  if (rc != WQ_OK) return rc;
+  // The maximum of the raw scores stands for the maximum of the scaled ones.
+  WQ_REQUIRE(scale > 0.f && scale < INFINITY, WQ_ERR_INVALID_ARGUMENT, "scale must be positive and finite (got %g)",
+             (double)scale);
+  if (tokens == 0 || sequences == 0) return WQ_OK;
+  WQ_REQUIRE(q && key_pages && value_pages && page_table && query_starts && seq_lens && out, WQ_ERR_INVALID_ARGUMENT,
+             "null pointer argument");
+  WQ_REQUIRE(((uintptr_t)q | (uintptr_t)key_pages | (uintptr_t)value_pages | (uintptr_t)out) % 16 == 0,
+             WQ_ERR_INVALID_ARGUMENT, "q, the pages and out must be 16-byte aligned");
+  WQ_REQUIRE(((uintptr_t)page_table | (uintptr_t)query_starts | (uintptr_t)seq_lens) % 4 == 0 &&
+                 (uintptr_t)tree_mask % 8 == 0,
+             WQ_ERR_INVALID_ARGUMENT, "integer operands must be aligned to their size");
+  const PagedPlan plan = paged_plan(tokens, sequences, q_heads / kv_heads, kv_heads, table_width, page_size);
+  WQ_REQUIRE(plan.bytes == 0 || (workspace && workspace_bytes >= plan.bytes && (uintptr_t)workspace % 16 == 0),
+             WQ_ERR_WORKSPACE, "paged attention needs a 16-byte aligned workspace of %zu bytes (got %zu)", plan.bytes,
+             workspace_bytes);
+  WQ_REQUIRE(plan.slots * kv_heads <= 0x7fffffff, WQ_ERR_UNSUPPORTED, "too many tokens for one call");
+  PagedArgs a{};
+  a.q = reinterpret_cast<const half_t*>(q);
+  a.kp = reinterpret_cast<const half_t*>(key_pages);
+  a.vp = reinterpret_cast<const half_t*>(value_pages);
+  a.table = page_table;
+  a.starts = query_starts;
+  a.lens = seq_lens;
+  a.mask = tree_mask;
+  a.out = reinterpret_cast<half_t*>(out);
+  a.part_o = reinterpret_cast<float*>(workspace);
+  a.part_ml = reinterpret_cast<float2_t*>(a.part_o + (size_t)plan.slots * kv_heads * 16 * kPagedDim);
+  a.k_stride = key_page_stride;
+  a.v_stride = value_page_stride;
+  a.scale_log2 = scale * kLog2e;
+  a.sequences = (int)sequences;
+  a.tokens = (int)tokens;
+  a.H = (int)q_heads;
+  a.KV = (int)kv_heads;
+  a.G = (int)(q_heads / kv_heads);
+  a.width = (int)table_width;
+  a.page_size = (int)page_size;
+  a.num_pages = (int)num_pages;
+  a.slots = (int)plan.slots;
+  a.spare = (int)plan.spare;
+  a.min_blocks = plan.min_blocks;
+  hipLaunchKernelGGL(paged_attention_rows_kernel, dim3((unsigned)(plan.slots * kv_heads)), dim3(256), 0,
+                     as_stream(stream), a);
+  rc = check_launch("paged_attention");
+  if (rc != WQ_OK || plan.spare == 0) return rc;
+  hipLaunchKernelGGL(paged_attention_merge_kernel<16>, dim3((unsigned)(plan.tiles * kv_heads), 4), dim3(256), 0,
+                     as_stream(stream), a);
+  return check_launch("paged_attention_merge");
+}

@@ -1,0 +1,340 @@
+"""The paged-cache operators (paged.paged_append, paged.paged_attention) against
+their formulas in 64 bits on the CPU: ragged batches, page sizes and head
+groups, trees of drafted tokens, rows that attend nothing, pages that do not
+exist, padding, strided pools, captured replays."""
+import math
+import random
+
+import pytest
+import torch
+
+from ondeviceinfer_amd.layers import RotaryEmbedding
+from ondeviceinfer_amd.paged import PagedBatch, paged_append, paged_attention
+
+pytestmark = pytest.mark.gpu
+D = 128
+HALF_ULP = 2.0 ** -11          # fp16: a rounding's largest relative error
+TINY = 2.0 ** -25              # ... and its largest absolute one among the subnormals
+
+
+class Pool:
+    """Pages in random order; every row that belongs to no sequence holds NaN."""
+
+    def __init__(self, new, past, *, hq, hkv, page, seed, interleaved=False, extra_width=1, pad=0):
+        gen = torch.Generator().manual_seed(seed)
+        self.new, self.past, self.hq, self.hkv, self.page = new, past, hq, hkv, page
+        lens = [n + p for n, p in zip(new, past)]
+        used = [(max(n, 0) + page - 1) // page for n in lens]
+        pages = sum(used) + 2
+        order = torch.randperm(pages, generator=gen).tolist()
+        width = max(used) + extra_width
+        self.table = torch.full((len(new), width), -7, dtype=torch.int32)
+        shape = (pages, 2, hkv, page, D) if interleaved else (2, pages, hkv, page, D)
+        block = torch.full(shape, float('nan'), dtype=torch.float16)
+        self.k, self.v = (block[:, 0], block[:, 1]) if interleaved else (block[0], block[1])
+        at = 0
+        for b, n in enumerate(lens):
+            for e in range(used[b]):
+                self.table[b, e] = order[at]
+                at += 1
+                rows = min(page, n - e * page)
+                for t in (self.k, self.v):
+                    t[order[at - 1], :, :rows] = torch.randn(hkv, rows, D, generator=gen).half()
+        starts = [0]
+        for n in new:
+            starts.append(starts[-1] + n)
+        self.starts, self.tokens, self.pad = starts, starts[-1], pad
+        self.lens = lens
+        self.gen = gen
+        self.block = block
+
+    def rand(self, *shape, scale=1.0):
+        return (scale * torch.randn(*shape, generator=self.gen)).half()
+
+    def to(self, gpu):
+        block = self.block.to(gpu)
+        k, v = (block[:, 0], block[:, 1]) if self.k.stride(0) != self.hkv * self.page * D else (block[0], block[1])
+        return k, v, PagedBatch(self.table.to(gpu), torch.tensor(self.starts, dtype=torch.int32, device=gpu),
+                                torch.tensor(self.lens, dtype=torch.int32, device=gpu))
+
+    def rows(self, b, t):
+        """[length, hkv, D] of sequence b from the pool ``t``."""
+        out = []
+        for i in range(max(self.lens[b], 0)):
+            out.append(t[self.table[b, i // self.page].item(), :, i % self.page])
+        return torch.stack(out) if out else torch.zeros(0, self.hkv, D, dtype=t.dtype)
+
+
+def tree_masks(new, rng):
+    masks = []
+    for count in new:
+        rows = []
+        for i in range(count):
+            rows.append((1 << i) | (rows[rng.randrange(max(0, i - 5), i)] if i else 0))
+        masks += rows
+    return masks
+
+
+def signed(m):
+    return m - (1 << 64) if m >> 63 else m
+
+
+def expected_attention(pool, query, scale, masks=None):
+    """(out, tolerance) in float64.  The probabilities' rounding moves a result
+    by at most 2^-11 sum p|v| (and 2^-25 per key, in units of the row's largest
+    probability, where they are subnormal), the result's own rounding by 2^-11
+    |o|; the 32-bit scores add, to first order, 130 2^-24 scale sum|q||k| to a
+    probability's exponent (128 products and their sum, twice the weight's
+    share: numerator and denominator), below a tenth of the first term here."""
+    out = torch.zeros(pool.tokens + pool.pad, pool.hq, D, dtype=torch.float64)
+    tol = torch.zeros_like(out)
+    group = pool.hq // pool.hkv
+    for b, (n, p) in enumerate(zip(pool.new, pool.past)):
+        if n == 0:
+            continue
+        k, v = pool.rows(b, pool.k).double(), pool.rows(b, pool.v).double()
+        for i in range(n):
+            t = pool.starts[b] + i
+            if masks is None:
+                seen = list(range(max(p + i + 1, 0)))
+            else:
+                seen = list(range(max(p, 0))) + [p + j for j in range(n) if (masks[t] >> j) & 1 and p + j >= 0]
+            if not seen:
+                continue
+            ks, vs = k[seen], v[seen]
+            q = query[t].double().view(pool.hkv, group, D)
+            s = torch.einsum('hgd,khd->hgk', q, ks) * scale
+            w = torch.exp(s - s.amax(-1, keepdim=True))
+            l = w.sum(-1, keepdim=True)
+            o = torch.einsum('hgk,khd->hgd', w / l, vs)
+            a = torch.einsum('hgk,khd->hgd', w / l, vs.abs())
+            size = torch.einsum('hgd,khd->hgk', q.abs(), ks.abs()).amax(-1, keepdim=True) * scale
+            bound = (a * (HALF_ULP + 2 * 130 * 2.0 ** -24 * size) + len(seen) * TINY * vs.abs().amax() / l
+                     + o.abs() * HALF_ULP + TINY)
+            out[t], tol[t] = o.reshape(pool.hq, D), bound.reshape(pool.hq, D)
+    return out, tol
+
+
+def check(got, want, tol):
+    got = got.double().cpu()
+    assert not torch.isnan(got).any()
+    worst = ((got - want).abs() / tol.clamp(min=1e-30)).where(got != want, torch.zeros_like(got)).max().item()
+    print(f'worst error / tolerance: {worst:.3f}', flush=True)
+    assert worst <= 1.0
+
+
+BATCHES = {
+    # name: (new, past, hq, hkv, page)
+    'one-token': ([1], [0], 4, 2, 16),
+    'one-behind-15': ([1], [15], 4, 2, 16),
+    'one-behind-16': ([1], [16], 4, 2, 16),
+    'decode': ([1, 1, 1, 1, 1], [0, 31, 32, 700, 133], 10, 2, 32),
+    'decode-long': ([1, 1], [2500, 3], 16, 2, 16),
+    'decode-page-64': ([1] * 3, [64 * 33, 64 * 16 - 1, 900], 5, 1, 64),
+    'group-16': ([1, 3], [40, 90], 16, 1, 48),
+    'group-1': ([2, 1], [17, 300], 3, 3, 16),
+    'sits-out': ([1, 0, 1, 0], [50, 20, 0, 7], 8, 2, 16),
+    'chunk': ([37, 5], [0, 100], 8, 2, 16),
+    'chunk-wide': ([150, 1, 64], [77, 600, 1], 10, 2, 32),
+    'chunk-page-128': ([90], [200], 4, 1, 128),
+    'seventy': ([1] * 70, [(37 * b) % 200 for b in range(70)], 4, 2, 16),
+}
+
+
+@pytest.mark.parametrize('interleaved', [False, True])
+@pytest.mark.parametrize('name', list(BATCHES))
+def test_causal_attention(gpu, name, interleaved):
+    new, past, hq, hkv, page = BATCHES[name]
+    print(name, interleaved, flush=True)
+    pool = Pool(new, past, hq=hq, hkv=hkv, page=page, seed=len(name), interleaved=interleaved, pad=3)
+    query = pool.rand(pool.tokens + pool.pad, hq, D, scale=1.5)
+    scale = 1.0 / math.sqrt(D)
+    want, tol = expected_attention(pool, query, scale)
+    k, v, batch = pool.to(gpu)
+    out = torch.full((pool.tokens + pool.pad, hq, D), 7.0, dtype=torch.float16, device=gpu)
+    got = paged_attention(query.to(gpu), k, v, batch, scale=scale, out=out)
+    assert got is out
+    torch.cuda.synchronize()
+    assert (out[pool.tokens:] == 7.0).all()          # padding behind the last sequence: left as it was
+    check(out[:pool.tokens], want[:pool.tokens], tol[:pool.tokens])
+
+
+TREES = {
+    'one': ([1], [0], 4, 2, 16),
+    'seven': ([7], [700], 10, 2, 16),
+    'sixty-four': ([64, 1, 33], [100, 45, 0], 8, 2, 32),
+    'long': ([12, 64], [2600, 1500], 5, 1, 16),
+}
+
+
+@pytest.mark.parametrize('name', list(TREES))
+def test_tree_attention(gpu, name):
+    new, past, hq, hkv, page = TREES[name]
+    print(name, flush=True)
+    pool = Pool(new, past, hq=hq, hkv=hkv, page=page, seed=3)
+    masks = tree_masks(new, random.Random(9))
+    query = pool.rand(pool.tokens, hq, D, scale=1.5)
+    scale = 1.0 / math.sqrt(D)
+    want, tol = expected_attention(pool, query, scale, masks)
+    k, v, batch = pool.to(gpu)
+    mask = torch.tensor([signed(m) for m in masks], dtype=torch.int64, device=gpu)
+    got = paged_attention(query.to(gpu), k, v, batch, scale=scale, tree_mask=mask)
+    check(got, want, tol)
+
+
+def test_rows_that_attend_nothing_are_zero(gpu):
+    """An empty mask in front of an empty cache, and lengths shorter than the new tokens."""
+    pool = Pool([3, 2], [0, 40], hq=4, hkv=2, page=16, seed=1)
+    masks = [0b001, 0, 0b101, 0, 0b11]       # token 1: nothing; token 3: only the cached ones
+    query = pool.rand(5, 4, D)
+    want, tol = expected_attention(pool, query, 0.1, masks)
+    k, v, batch = pool.to(gpu)
+    got = paged_attention(query.to(gpu), k, v, batch, scale=0.1,
+                          tree_mask=torch.tensor(masks, dtype=torch.int64, device=gpu))
+    assert (got[1] == 0).all()
+    check(got, want, tol)
+    # Sequence 0 has two positions for its three new tokens: the first token lies before the first position.
+    pool = Pool([3, 2], [-1, 40], hq=4, hkv=2, page=16, seed=2)
+    query = pool.rand(5, 4, D)
+    want, tol = expected_attention(pool, query, 0.1)
+    k, v, batch = pool.to(gpu)
+    got = paged_attention(query.to(gpu), k, v, batch, scale=0.1)
+    assert (got[0] == 0).all()
+    check(got, want, tol)
+
+
+def test_positions_without_a_page_give_nan(gpu):
+    """A page number outside the pool, or a length past the table: NaN for the tokens that attend it and no others."""
+    pool = Pool([1, 1, 1, 2], [40, 100, 300, 30], hq=4, hkv=2, page=16, seed=5, extra_width=0)
+    query = pool.rand(5, 4, D)
+    want, tol = expected_attention(pool, query, 0.1)
+    k, v, batch = pool.to(gpu)
+    pages = k.shape[0]
+    table = batch.page_table.clone()
+    table[0, 1] = pages                     # one past the pool
+    table[1, 6] = -1                        # the last page, position 96 ..
+    table[3, 1] = 1 << 30                   # positions 16 .. 31 of the two-token sequence
+    lens = batch.seq_lens.clone()
+    lens[2] = 2 ** 31 - 1                   # far past the table's width
+    got = paged_attention(query.to(gpu), k, v, PagedBatch(table, batch.query_starts, lens), scale=0.1)
+    for t in (0, 1, 2, 3, 4):
+        assert torch.isnan(got[t]).all(), t
+    # The same entries one position behind what is attended are never read.
+    table = batch.page_table.clone()
+    table = torch.cat((table, torch.full((4, 2), 1 << 30, dtype=torch.int32, device=gpu)), dim=1).contiguous()
+    check(paged_attention(query.to(gpu), k, v, PagedBatch(table, batch.query_starts, batch.seq_lens), scale=0.1), want, tol)
+
+
+def test_starts_out_of_order_touch_only_their_sequence(gpu):
+    pool = Pool([2, 3, 1], [20, 30, 40], hq=4, hkv=2, page=16, seed=6)
+    query = pool.rand(6, 4, D)
+    want, tol = expected_attention(pool, query, 0.1)
+    k, v, batch = pool.to(gpu)
+    out = torch.full((6, 4, D), 7.0, dtype=torch.float16, device=gpu)
+    starts = torch.tensor([0, 2, 500, 500], dtype=torch.int32, device=gpu)     # sequences 1 and 2: past the tokens
+    paged_attention(query.to(gpu), k, v, PagedBatch(batch.page_table, starts, batch.seq_lens), scale=0.1, out=out)
+    assert (out[2:] == 7.0).all()
+    check(out[:2], want[:2], tol[:2])
+
+
+def test_more_than_64_drafted_tokens_give_nan(gpu):
+    pool = Pool([65, 2], [10, 5], hq=4, hkv=2, page=16, seed=8)
+    query = pool.rand(67, 4, D)
+    k, v, batch = pool.to(gpu)
+    mask = torch.full((67,), 3, dtype=torch.int64, device=gpu)
+    got = paged_attention(query.to(gpu), k, v, batch, scale=0.1, tree_mask=mask)
+    assert torch.isnan(got[:65]).all() and not torch.isnan(got[65:]).any()
+
+
+# ----------------------------------------------------------------------------- append
+
+def tables(positions=400):
+    cos, sin = RotaryEmbedding(D).table(positions, 'cpu')
+    return cos, sin
+
+
+def expected_rows(x, weight, cos, sin, eps):
+    """[heads, D] rows of one token in float64 (before the rounding)."""
+    u = x.double()
+    if weight is not None:
+        u = u / torch.sqrt((u * u).mean(-1, keepdim=True) + eps) * weight.double()
+    turned = torch.cat((-u[:, 64:], u[:, :64]), dim=-1)
+    return u * cos.double() + turned * sin.double()
+
+
+@pytest.mark.parametrize('norm', [True, False])
+@pytest.mark.parametrize('name', ['one-token', 'decode', 'sits-out', 'chunk', 'group-1', 'seventy'])
+def test_append(gpu, name, norm):
+    new, past, hq, hkv, page = BATCHES[name]
+    past = [min(p, 300) for p in past]
+    print(name, norm, flush=True)
+    pool = Pool(new, past, hq=hq, hkv=hkv, page=page, seed=11, interleaved=len(name) % 2 == 0, pad=2)
+    cos, sin = tables()
+    qkv = pool.rand(pool.tokens + 2, (hq + 2 * hkv) * D, scale=2.0)
+    qn, kn = (1 + 0.3 * pool.rand(D).float()).half(), (1 + 0.3 * pool.rand(D).float()).half()
+    if not norm:
+        qn = kn = None
+    k, v, batch = pool.to(gpu)
+    k0, v0 = k.clone(), v.clone()
+    out = torch.full((pool.tokens + 2, hq, D), 7.0, dtype=torch.float16, device=gpu)
+    up = lambda t: None if t is None else t.to(gpu)  # noqa: E731
+    paged_append(qkv.to(gpu), k, v, batch, q_heads=hq, q_norm=up(qn), k_norm=up(kn), eps=1e-6, cos_table=up(cos),
+                 sin_table=up(sin), out=out)
+    torch.cuda.synchronize()
+    assert (out[pool.tokens:] == 7.0).all()
+    want_k, want_v = k0.cpu(), v0.cpu()
+    got_k, got_v, got_q = k.cpu(), v.cpu(), out.cpu()
+    for b, (n, p) in enumerate(zip(new, past)):
+        for i in range(n):
+            t, at = pool.starts[b] + i, p + i
+            x = qkv[t].view(hq + 2 * hkv, D)
+            slot = pool.table[b, at // page].item()
+            want_v[slot, :, at % page] = x[hq + hkv:]
+            for got, heads, w in ((got_q[t], x[:hq], qn), (got_k[slot, :, at % page], x[hq:hq + hkv], kn)):
+                want = expected_rows(heads, w, cos[at], sin[at], 1e-6)
+                # One rounding of the result; in 32 bits each of the two products carries the norm's few roundings
+                # (sum of squares, reciprocal root, two products: below 16 half-ulps of 2^-24 together).
+                size = expected_rows(heads.abs(), w, cos[at].abs(), sin[at].abs(), 1e-6).abs() + want.abs()
+                tol = want.abs() * HALF_ULP + TINY + 16 * 2.0 ** -24 * 3 * size
+                big = torch.cat((heads[:, 64:], heads[:, :64]), dim=-1).abs().double() * 3 + heads.abs().double() * 3
+                tol = tol + 16 * 2.0 ** -24 * big
+                assert ((got.double() - want).abs() <= tol).all()
+            want_k[slot, :, at % page] = got_k[slot, :, at % page]
+    # Nothing but the new tokens' rows changed.
+    assert torch.equal(got_k.view(torch.int16), want_k.view(torch.int16))
+    assert torch.equal(got_v.view(torch.int16), want_v.view(torch.int16))
+
+
+def test_append_refuses_tokens_without_a_place(gpu):
+    """No page, a page outside the pool, an index past the table, a position past the tables: NaN queries, no write."""
+    pool = Pool([1, 1, 1, 1, 2], [20, 20, 20, 390, 20], hq=4, hkv=2, page=16, seed=12, extra_width=0)
+    cos, sin = tables(388)
+    qkv = pool.rand(6, 8 * D)
+    k, v, batch = pool.to(gpu)
+    table, lens = batch.page_table.clone(), batch.seq_lens.clone()
+    table[0, 1] = -1
+    table[1, 1] = k.shape[0]
+    lens[2] = 16 * table.shape[1] + 1
+    lens[4] = 1                       # two new tokens, one position: the first has index -1
+    k0, v0 = k.clone(), v.clone()
+    got = paged_append(qkv.to(gpu), k, v, PagedBatch(table, batch.query_starts, lens), q_heads=4, q_norm=None,
+                       k_norm=None, eps=1e-6, cos_table=cos.to(gpu), sin_table=sin.to(gpu))
+    torch.cuda.synchronize()
+    assert torch.isnan(got[:5]).all() and not torch.isnan(got[5]).any()
+    page = table[4, 0].item()
+    k0[page, :, 0], v0[page, :, 0] = k[page, :, 0], v[page, :, 0]
+    assert torch.equal(k.view(torch.int16), k0.view(torch.int16))
+    assert torch.equal(v.view(torch.int16), v0.view(torch.int16))
+
+
+def test_append_takes_given_positions(gpu):
+    pool = Pool([4], [30], hq=2, hkv=1, page=16, seed=13)
+    cos, sin = tables()
+    qkv = pool.rand(4, 4 * D)
+    k, v, batch = pool.to(gpu)
+    positions = torch.tensor([30, 31, 31, 32], dtype=torch.int32, device=gpu)
+    got = paged_append(qkv.to(gpu), k, v, batch, q_heads=2, q_norm=None, k_norm=None, eps=1e-6,
+                       cos_table=cos.to(gpu), sin_table=sin.to(gpu), positions=positions).cpu()
+    for t, at in enumerate((30, 31, 31, 32)):
+        want = expected_rows(qkv[t].view(4, D)[:2], None, cos[at], sin[at], 1e-6)
+        assert (got[t].double() - want).abs().max() <= want.abs().max() * HALF_ULP + 1e-5

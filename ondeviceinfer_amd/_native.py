@@ -1,5 +1,6 @@
 """ctypes binding of ``libondeviceinfer_wq.so`` (the C ABI in ``include/ondeviceinfer_wq.h``,
-``include/ondeviceinfer_decode.h`` and ``include/ondeviceinfer_paged.h``).
+``include/ondeviceinfer_decode.h``, ``include/ondeviceinfer_paged.h`` and
+``include/ondeviceinfer_sample.h``).
 
 torch is imported first so its bundled HIP runtime (``libamdhip64.so.7``) is
 the one the library binds to: the kernels then run in torch's context and on
@@ -99,6 +100,10 @@ _SIGNATURES = {
     'wq_paged_attention_workspace_size': [_I64, _I64, _I64, _I64, _I64, _I64, _I64, _SIZE_P],
     'wq_paged_attention': [_P, _I64, _I64, _I64, _I64, _P, _I64, _P, _I64, _I64, _I64, _P, _I64, _P, _P, _I64, _P,
                            ctypes.c_float, _P, _P, ctypes.c_size_t, _P],
+    # include/ondeviceinfer_sample.h
+    'wq_sample_workspace_size': [_I64, _I64, _SIZE_P],
+    'wq_sample': [_P, ctypes.c_int32, _I64, _I64, _I64, _P, _P, ctypes.c_float, _P, ctypes.c_int32, _P, ctypes.c_float,
+                  _P, ctypes.c_float, _P, _P, ctypes.c_size_t, _P],
 }
 EXPORTED_SYMBOLS = ('wq_last_error', *_SIGNATURES)
 
@@ -1075,6 +1080,65 @@ def paged_attention(query: torch.Tensor, key_pages: torch.Tensor, value_pages: t
     _call_on(device, 'wq_paged_attention', _ptr(query), tokens, q_heads, kv_heads, head_dim, _ptr(key_pages), k_stride,
              _ptr(value_pages), v_stride, pages, page_size, _ptr(page_table), width, _ptr(query_starts),
              _ptr(seq_lens), sequences, _ptr(tree_mask), float(scale), _ptr(out), ws_ptr, ws_bytes, _stream(device))
+    return out
+
+
+# ----------------------------------------------------------------------------- sampling
+
+_LOGITS = {torch.float16: 0, torch.float32: 1}
+
+
+@functools.lru_cache(maxsize=1024)   # a pure function of the shape, asked for on every call
+def sample_workspace_size(rows: int, vocab: int) -> int:
+    b = ctypes.c_size_t()
+    _call('wq_sample_workspace_size', rows, vocab, ctypes.byref(b))
+    return b.value
+
+
+def _setting(value, dtype: torch.dtype, rows: int, name: str) -> tuple[int | None, float | int]:
+    """(device pointer, scalar) of a per-row setting."""
+    if isinstance(value, torch.Tensor):
+        _check(value, dtype, (rows,), name)
+        return value.data_ptr(), 0
+    return None, value
+
+
+def sample(logits: torch.Tensor, uniform: torch.Tensor, temperature=1.0, top_k=0, top_p=1.0, min_p=0.0,
+           out: torch.Tensor | None = None, workspace: torch.Tensor | None = None) -> torch.Tensor:
+    """One token per row of ``logits`` [rows, vocab] (fp16 or fp32) drawn with
+    ``uniform`` [rows] after temperature, top-k, top-p and min-p, each a number
+    or a per-row device tensor (``wq_sample``)."""
+    tensors = [t for t in (temperature, top_k, top_p, min_p) if isinstance(t, torch.Tensor)]
+    device = _require_gpu(logits, uniform, out, workspace, *tensors)
+    kind = _LOGITS.get(logits.dtype)
+    if kind is None:
+        raise TypeError(f'logits: expected float16 or float32, got {logits.dtype}')
+    if logits.dim() != 2:
+        raise ValueError(f'logits must be [rows, vocab], got {tuple(logits.shape)}')
+    rows, vocab = logits.shape
+    stride, inner = logits.stride()
+    if (inner != 1 and vocab > 1) or (rows > 1 and stride < vocab):
+        raise ValueError(f'logits: a row must be contiguous and rows must not overlap, got strides {logits.stride()}')
+    _check(uniform, torch.float32, (rows,), 'uniform')
+    t_ptr, t_all = _setting(temperature, torch.float32, rows, 'temperature')
+    k_ptr, k_all = _setting(top_k, torch.int32, rows, 'top_k')
+    p_ptr, p_all = _setting(top_p, torch.float32, rows, 'top_p')
+    m_ptr, m_all = _setting(min_p, torch.float32, rows, 'min_p')
+    if t_ptr is None and not 0.0 <= t_all < float('inf'):
+        raise ValueError(f'temperature must be finite and not negative, got {t_all}')
+    if (p_ptr is None and p_all != p_all) or (m_ptr is None and m_all != m_all):
+        raise ValueError('top_p and min_p must be numbers')
+    if k_ptr is None:
+        k_all = int(min(max(k_all, 0), 0x7fffffff))
+    if out is None:
+        out = torch.empty(rows, dtype=torch.int64, device=device)
+    else:
+        _check(out, torch.int64, (rows,), 'out')
+    if workspace is None:   # sums of the row's parts (no counters): any scratch of this call's own
+        workspace = uniform.new_empty(sample_workspace_size(rows, vocab), dtype=torch.uint8)
+    _call_on(device, 'wq_sample', _ptr(logits), kind, rows, vocab, max(stride, vocab), _ptr(uniform), t_ptr,
+             float(t_all), k_ptr, k_all, p_ptr, float(p_all), m_ptr, float(m_all), _ptr(out), _ptr(workspace),
+             workspace.numel() * workspace.element_size(), _stream(device))
     return out
 
 

@@ -1,0 +1,231 @@
+"""sampling.sample_tokens against its definition in 64 bits on the CPU, token
+for token: types, odd vocabularies and strides, ties, every filter alone and
+together, infinities, rows without a distribution, scalars and per-row
+settings, captured replays."""
+import math
+
+import numpy as np
+import pytest
+import torch
+
+from ondeviceinfer_amd.sampling import sample_tokens
+
+pytestmark = pytest.mark.gpu
+
+
+def definition(row, u, temperature, top_k, top_p, min_p):
+    """The token of one row, from the definition (numpy float64)."""
+    values = row.astype(np.float64) + 0.0
+    if np.isnan(values).any() or not (values > -np.inf).any():
+        return -1
+    order = np.lexsort((np.arange(values.size), -values))
+    if temperature == 0.0:
+        return int(order[0])
+    top = values[order[0]]
+    with np.errstate(invalid='ignore'):
+        z = np.where(values == top, 0.0, (values - top) / float(np.float32(temperature)))[order]
+    if top_k > 0:
+        order, z = order[:top_k], z[:top_k]
+    w = np.exp(z)
+    if top_p < 1.0:
+        goal = float(np.float32(top_p)) * w.sum()
+        n = max(1, int((np.cumsum(w) - w < goal).sum()))
+        order, z, w = order[:n], z[:n], w[:n]
+    if min_p > 0.0:
+        keep = z >= math.log(np.float32(min_p))
+        keep[0] = True
+        order, w = order[keep], w[keep]
+    by_index = np.argsort(order)
+    order, w = order[by_index], w[by_index]
+    run = np.cumsum(w)
+    hit = (run > float(np.float32(u)) * run[-1]) & (w > 0)
+    return int(order[np.argmax(hit)] if hit.any() else order[np.nonzero(w)[0][-1]])
+
+
+def settings(rows, kind, rng):
+    out = []
+    for _ in range(rows):
+        m = rng.choice(['both', 'top_k', 'top_p', 'min_p', 'none', 'greedy', 'all']) if kind == 'mixed' else kind
+        out.append((0.0 if m == 'greedy' else round(rng.uniform(0.3, 1.6), 3),
+                    int(rng.integers(1, 200)) if m in ('both', 'top_k', 'all') else 0,
+                    round(rng.uniform(0.1, 0.99), 3) if m in ('both', 'top_p', 'all') else 1.0,
+                    round(rng.uniform(0.001, 0.3), 4) if m in ('min_p', 'all') else 0.0))
+    return out
+
+
+def run(gpu, logits, u, asks, **kw):
+    t, k, p, m = zip(*asks)
+    f = lambda x: torch.tensor(x, dtype=torch.float32, device=gpu)  # noqa: E731
+    return sample_tokens(logits, u.to(gpu), temperature=f(t), top_k=torch.tensor(k, dtype=torch.int32, device=gpu),
+                         top_p=f(p), min_p=f(m), **kw)
+
+
+def compare(got, logits, u, asks):
+    got = got.cpu().tolist()
+    rows = logits.cpu().float().numpy()
+    want = [definition(rows[r], u[r].item(), *asks[r]) for r in range(len(asks))]
+    assert got == want, [(r, g, w, asks[r]) for r, (g, w) in enumerate(zip(got, want)) if g != w]
+
+
+@pytest.mark.parametrize('kind', ['none', 'top_k', 'top_p', 'min_p', 'both', 'mixed'])
+@pytest.mark.parametrize('dtype', [torch.float16, torch.float32])
+@pytest.mark.parametrize('rows,vocab', [(3, 1), (5, 7), (4, 1000), (9, 4097), (40, 12289), (2, 151936)])
+def test_tokens_follow_the_definition(gpu, rows, vocab, dtype, kind):
+    print(rows, vocab, dtype, kind, flush=True)
+    gen = torch.Generator().manual_seed(vocab + rows)
+    rng = np.random.default_rng(vocab)
+    logits = torch.randn(rows, vocab, generator=gen) * 2.5
+    logits[:, torch.randint(vocab, (20,), generator=gen)] += 9.0
+    logits = logits.to(dtype)
+    u = torch.rand(rows, generator=gen)
+    asks = settings(rows, kind, rng)
+    compare(run(gpu, logits.to(gpu), u, asks), logits, u, asks)
+
+
+@pytest.mark.parametrize('step', [0.25, 2.0, 1000.0])
+def test_ties_go_to_the_lowest_index(gpu, step):
+    """Few distinct values, so that every cut ends among equal ones; step 1000: all equal."""
+    gen = torch.Generator().manual_seed(1)
+    rng = np.random.default_rng(2)
+    logits = (torch.round(torch.randn(30, 9000, generator=gen) / step) * step).half()
+    u = torch.rand(30, generator=gen)
+    for kind in ('top_k', 'top_p', 'both', 'all'):
+        asks = settings(30, kind, rng)
+        compare(run(gpu, logits.to(gpu), u, asks), logits, u, asks)
+
+
+def test_equal_values_are_cut_exactly(gpu):
+    """4096 equal weights, half of the mass: the first 2048 tokens and no others."""
+    logits = torch.zeros(4, 4096)
+    logits[:, 1::2] = -0.0                     # equal to +0
+    u = torch.tensor([0.0, 0.5, 1.0 - 2.0 ** -24, 1023 / 2048])
+    got = sample_tokens(logits.to(gpu), u.to(gpu), top_p=0.5)
+    assert got.tolist() == [0, 1024, 2047, 1023]
+    got = sample_tokens(logits.to(gpu), u.to(gpu), top_k=8)
+    assert got.tolist() == [0, 4, 7, 3]
+
+
+def test_flat_and_peaked_rows(gpu):
+    """Large and small temperatures: nearly all tokens in one octave of weights, or one token with all of it."""
+    gen = torch.Generator().manual_seed(4)
+    logits = torch.randn(12, 30000, generator=gen)
+    u = torch.rand(12, generator=gen)
+    for temperature in (1e-6, 0.01, 50.0, 1e6):
+        for top_k, top_p, min_p in ((0, 1.0, 0.0), (500, 1.0, 0.0), (0, 0.6, 0.0), (700, 0.3, 0.5), (0, 0.95, 0.99)):
+            asks = [(temperature, top_k, top_p, min_p)] * 12
+            compare(run(gpu, logits.to(gpu), u, asks), logits, u, asks)
+            half = logits.half()
+            compare(run(gpu, half.to(gpu), u, asks), half, u, asks)
+
+
+def test_masked_and_infinite_logits(gpu):
+    inf = float('inf')
+    logits = torch.randn(8, 5000, generator=torch.Generator().manual_seed(5))
+    logits[0, :4990] = -inf                    # a grammar that allows ten tokens
+    logits[1] = -inf
+    logits[2, 17] = float('nan')
+    logits[3, [5, 4000]] = inf                 # they share the whole weight
+    logits[4] = torch.finfo(torch.float32).min
+    logits[4, 77] = 1.0
+    logits[5] = torch.finfo(torch.float32).min     # all at the type's lowest value: equal
+    logits[6, 1:] = -inf
+    u = torch.tensor([0.3, 0.3, 0.3, 0.7, 0.5, 0.25, 0.99, 0.1])
+    for asks in ([(1.0, 0, 1.0, 0.0)] * 8, [(0.7, 20, 0.9, 0.0)] * 8, [(0.0, 0, 1.0, 0.0)] * 8, [(1.0, 0, 0.5, 0.2)] * 8):
+        got = run(gpu, logits.to(gpu), u, asks)
+        compare(got, logits, u, asks)
+        assert got[1] == -1 and got[2] == -1 and got[4] == 77 and got[6] == 0
+
+
+def test_settings_without_a_meaning_give_minus_one(gpu):
+    nan, inf = float('nan'), float('inf')
+    logits = torch.randn(8, 300, generator=torch.Generator().manual_seed(6)).to(gpu)
+    u = torch.tensor([0.5] * 7 + [nan], device=gpu)
+    f = lambda *x: torch.tensor(x, dtype=torch.float32, device=gpu)  # noqa: E731
+    got = sample_tokens(logits, u, temperature=f(-1.0, nan, inf, 1, 1, 1, 1, 1), top_p=f(1, 1, 1, nan, 1, 0.0, -3.0, 1),
+                        min_p=f(0, 0, 0, 0, nan, 0, 0, 0)).tolist()
+    assert got[:5] == [-1] * 5 and got[7] == -1
+    assert got[5:7] == logits.argmax(dim=1).tolist()[5:7]       # top_p of nothing: the first always stays
+    got = sample_tokens(logits, u, top_k=-4, min_p=2.0).tolist()
+    assert got[:7] == logits.argmax(dim=1).tolist()[:7] and got[7] == -1
+
+
+def test_greedy_is_the_argmax(gpu):
+    logits = torch.randn(6, 151936, generator=torch.Generator().manual_seed(7)).half().to(gpu)
+    logits[:, [40, 90000]] = 30.0
+    assert sample_tokens(logits, torch.rand(6, device=gpu), temperature=0.0).tolist() == [40] * 6
+
+
+@pytest.mark.parametrize('dtype', [torch.float16, torch.float32])
+def test_strided_and_misaligned_rows(gpu, dtype):
+    gen = torch.Generator().manual_seed(8)
+    rng = np.random.default_rng(9)
+    block = torch.randn(6, 3, 5003, generator=gen).to(dtype)
+    u = torch.rand(6, generator=gen)
+    for offset in (0, 1, 3):
+        rows = block.to(gpu)[:, -1, offset:]
+        asks = settings(6, 'mixed', rng)
+        compare(run(gpu, rows, u, asks), block[:, -1, offset:], u, asks)
+
+
+def test_many_rows_and_an_output_of_ones_own(gpu):
+    gen = torch.Generator().manual_seed(10)
+    rng = np.random.default_rng(11)
+    logits = (torch.randn(1500, 700, generator=gen) * 3).half()
+    u = torch.rand(1500, generator=gen)
+    asks = settings(1500, 'mixed', rng)
+    out = torch.full((1500,), -5, dtype=torch.int64, device=gpu)
+    got = run(gpu, logits.to(gpu), u, asks, out=out)
+    assert got is out
+    compare(got, logits, u, asks)
+    assert sample_tokens(logits[:0].to(gpu), u[:0].to(gpu)).shape == (0,)
+
+
+def test_captured_replays_follow_their_inputs(gpu):
+    gen = torch.Generator().manual_seed(12)
+    rng = np.random.default_rng(13)
+    logits = torch.zeros(16, 20000, dtype=torch.float16, device=gpu)
+    u = torch.zeros(16, device=gpu)
+    asks = settings(16, 'mixed', rng)
+    run(gpu, logits, u, asks)
+    t, k, p, m = zip(*asks)
+    f = lambda x: torch.tensor(x, dtype=torch.float32, device=gpu)  # noqa: E731
+    args = dict(temperature=f(t), top_k=torch.tensor(k, dtype=torch.int32, device=gpu), top_p=f(p), min_p=f(m))
+    graph = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(graph):
+        got = sample_tokens(logits, u, **args)
+    for _ in range(4):
+        new = (torch.randn(16, 20000, generator=gen) * 3).half()
+        numbers = torch.rand(16, generator=gen)
+        logits.copy_(new)
+        u.copy_(numbers)
+        graph.replay()
+        torch.cuda.synchronize()
+        compare(got, new, numbers, asks)
+
+
+def test_refusals(gpu):
+    logits, u = torch.zeros(4, 10, device=gpu), torch.zeros(4, device=gpu)
+    with pytest.raises(TypeError):
+        sample_tokens(logits.double(), u)
+    with pytest.raises(TypeError):
+        sample_tokens(logits.bfloat16(), u)
+    with pytest.raises(ValueError):
+        sample_tokens(logits[0], u)
+    with pytest.raises(ValueError):
+        sample_tokens(logits.t().contiguous().t(), u)
+    with pytest.raises(ValueError):
+        sample_tokens(logits[:1].expand(4, 10), u)
+    with pytest.raises(ValueError):
+        sample_tokens(logits, u[:3])
+    with pytest.raises(TypeError):
+        sample_tokens(logits, u.double())
+    with pytest.raises(TypeError):
+        sample_tokens(logits, u, top_k=torch.zeros(4, dtype=torch.int64, device=gpu))
+    with pytest.raises(ValueError):
+        sample_tokens(logits, u, temperature=-1.0)
+    with pytest.raises(ValueError):
+        sample_tokens(logits, u, top_p=float('nan'))
+    with pytest.raises(ValueError):
+        sample_tokens(logits, u.cpu())
+    with pytest.raises(ValueError):
+        sample_tokens(logits, u, workspace=torch.empty(8, dtype=torch.uint8, device=gpu))

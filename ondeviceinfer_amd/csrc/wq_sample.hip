@@ -1,13 +1,16 @@
 // Sampling one token per row of logits: temperature, top-k, top-p, min-p and
 // the draw from a given uniform number.
 //
-// Three launches.  A row is cut into parts of whole 16-byte chunks:
-//   peak    the largest logit of every part and its first index;
-//   tally   with the row's largest logit m known, every token's weight
-//           w = 2^z, z = (l - m) log2(e) / T <= 0, added to one of 16 bins of
-//           its part, bin = min(floor(-z), 15): mass and count;
-//   pick    one workgroup per row finds the bins in which top-k and top-p end,
-//           the value inside them at which they do, and draws.
+// With y = logit log2(e) / T a token weighs 2^y.  Three launches, the row cut
+// into parts of whole 16-byte chunks:
+//   tally   counts every part's tokens and adds their weights in 16 bins of
+//           octaves of weight, from the part's largest down;
+//   gather  from the row's bins follow the ones in which top-k, top-p and
+//           min-p end; their tokens, a few dozen of a peaked row and some
+//           thousands of a flat one, go to a list;
+//   pick    one workgroup per row finds the value at which the cut ends in the
+//           list and draws: a part from the parts' remaining weights, then the
+//           token in it.
 // Which tokens stay comes down to one value: all above it and the first
 // `ties` that equal it, by index.  Everything that decides is exact or in 64
 // bits and summed in a fixed order: with 32-bit sums over 151936 tokens one
@@ -24,21 +27,26 @@ namespace {
 
 constexpr int kBins = 16;
 constexpr int kMaxParts = 64;
+constexpr int kTallyThreads = 256;
 constexpr int kPickThreads = 1024;
+constexpr int kSub = 256;              // steps of a bin, or of a byte of the key
+constexpr int kMostSorted = 512;       // tokens of one step put in order at once
 
 struct SampleArgs {
   const void* logits;
   int64_t row_stride;
   int rows, vocab, parts;
   int mass_bits;      // fraction bits of a mass as a whole number: vocab of them stay below 2^63
+  int list_cap;       // entries of a row's list
   const float *uniform, *temperature, *top_p, *min_p;
   const int32_t* top_k;
   float temperature_all, top_p_all, min_p_all;
   int32_t top_k_all;
   int64_t* tokens;
   float2_t* peak;     // [rows][parts] (largest logit, bits of its first index); NaN: the part holds one
-  double* mass;       // [rows][parts][kBins]
+  double* mass;       // [rows][parts][kBins], in units of 2^base of the part
   uint32_t* count;    // [rows][parts][kBins]
+  float2_t* list;     // [rows][list_cap] (logit, bits of its index)
 };
 
 // One row of logits in 16-byte chunks on 16-byte boundaries: a row that starts
@@ -94,11 +102,11 @@ struct Row {
   }
 };
 
-// What a row asks for, and what there is to say about it before its weights.
+// What a row asks for, and whether there is anything to weigh.
 struct Ask {
   double to_octaves;   // log2(e) / temperature
   double top_p;        // 1: off
-  double floor;        // smallest z (octaves) that min-p keeps; -inf: off
+  double min_p;        // log2 of it; -inf: off
   int top_k;           // vocab: off
   bool greedy, none;
 };
@@ -114,18 +122,42 @@ __device__ __forceinline__ Ask read_ask(const SampleArgs& a, int row) {
   q.greedy = t == 0.f || k == 1 || p <= 0.f || mp > 1.f;
   q.to_octaves = 1.4426950408889634074 / (double)t;
   q.top_p = p < 1.f ? (double)p : 1.0;
-  q.floor = mp > 0.f ? log2((double)mp) : -INFINITY;
+  q.min_p = mp > 0.f ? log2((double)mp) : -INFINITY;
   q.top_k = k > 0 && k < a.vocab ? k : a.vocab;
   return q;
 }
 
-__device__ __forceinline__ double octaves(float v, float top, double to_octaves) {
-  return v == top ? 0.0 : ((double)v - (double)top) * to_octaves;
-}
+// Weights against a base, the octave of the largest rounded up to one of
+// 4 n + 3: the bins of a part and of the row then start whole multiples of
+// four octaves apart.  Infinite logits: where the largest is +inf only its
+// equals weigh anything, and a part that holds nothing above -inf weighs
+// nothing.
+struct Scale {
+  double to_octaves, base;
+  float top;
 
-// 2^z for z <= 0: z = n / 32 + r with |r| <= 1 / 64, 2^(n/32) from a table of
-// 32 and an exponent, 2^r = e^(r ln 2) by its series to the fifth power (the
-// next term is below 3e-15 of the sum).
+  __device__ __forceinline__ Scale(double per_logit, float largest) : to_octaves(per_logit), top(largest) {
+    base = isinf(largest) ? 3.0 : 4.0 * floor(0.25 * floor((double)largest * per_logit)) + 3.0;
+  }
+  __device__ __forceinline__ double y(float v) const {
+    if (isinf(top)) return v == top && top > 0.f ? 0.0 : -INFINITY;
+    return (double)v * to_octaves;
+  }
+  __device__ __forceinline__ double below(double y) const { return base - floor(y); }   // whole octaves
+};
+
+// Bins of octaves below the base: eight of one octave, seven of four, and all
+// that lies 36 or more below (of 2^18 tokens less than 2^-15 of the weight:
+// only top-k goes there).
+__device__ __forceinline__ int bin_of(double below) {
+  const int d = (int)fmin(below, 64.0);
+  return d < 8 ? d : min(8 + ((d - 8) >> 2), kBins - 1);
+}
+__device__ __forceinline__ int bin_depth(int bin) { return bin < 8 ? bin : 8 + 4 * (bin - 8); }   // its first octave
+
+// 2^z: z = n / 32 + r with |r| <= 1 / 64, 2^(n/32) from a table of 32 and an
+// exponent, 2^r = e^(r ln 2) by its series to the fifth power (the next term
+// is below 3e-15 of the sum).
 struct Exp2Table {
   double v[32];
 };
@@ -147,45 +179,48 @@ __device__ __forceinline__ double exp2_64(double z, const Exp2Table& t) {
   return z < -1080.0 ? 0.0 : ldexp(s * t.v[k & 31], k >> 5);
 }
 
-__device__ __forceinline__ int bin_of(double z) { return (int)fmin(-z, (double)(kBins - 1)); }
-
-// The row's largest logit over its parts: NaN if a part holds one.  `index`
-// (its first index) is valid in every lane.
-__device__ __forceinline__ float row_peak(const SampleArgs& a, int row, int lane, int& index) {
-  float best = -INFINITY;
-  int at = INT_MAX;
-  if (lane < a.parts) {
-    const float2_t e = a.peak[(size_t)row * a.parts + lane];
-    best = e.x;
-    const float y = e.y;
-    at = __builtin_bit_cast(int, y);
+// (best, at) the better of two of a row's largest: NaN first, then the larger, then the lower index.
+__device__ __forceinline__ void keep_peak(float& best, int& at, float ov, int oi) {
+  if (best == best && (ov != ov || ov > best || (ov == best && oi < at))) {
+    best = ov;
+    at = oi;
   }
+}
+
+__device__ __forceinline__ void wave_peak(float& best, int& at) {
 #pragma unroll
   for (int o = 32; o > 0; o >>= 1) {
     const float ov = __shfl_xor(best, o);
     const int oi = __shfl_xor(at, o);
-    if (best == best && (ov != ov || ov > best || (ov == best && oi < at))) {
-      best = ov;
-      at = oi;
-    }
+    keep_peak(best, at, ov, oi);
   }
-  index = at;
-  return best;
 }
 
-// grid = (parts, rows), 256 threads.
+// grid = (parts, rows), 256 threads.  Every thread keeps its own column of the
+// bins in LDS, so the additions need no atomics, meet no bank conflicts
+// between lanes and happen in a fixed order.
 template <typename T>
-__global__ __launch_bounds__(256) void sample_peak_kernel(SampleArgs a) {
+__global__ __launch_bounds__(kTallyThreads) void sample_tally_kernel(SampleArgs a) {
   constexpr int E = Row<T>::E;
+  __shared__ double mass[kBins][kTallyThreads];
+  __shared__ uint32_t count[kBins][kTallyThreads];
+  __shared__ Exp2Table table;
   __shared__ float sv[4];
   __shared__ int si[4];
   const int row = blockIdx.y, part = blockIdx.x, tid = threadIdx.x;
+  const Ask q = read_ask(a, row);
   const Row<T> r(a, row);
-  const int c1 = min((part + 1) * r.per_part, r.chunks);
+  const int c0 = part * r.per_part, c1 = min(c0 + r.per_part, r.chunks);
+  fill_exp2(table, tid);
+#pragma unroll
+  for (int b = 0; b < kBins; ++b) {
+    mass[b][tid] = 0.0;
+    count[b][tid] = 0;
+  }
   float best = -INFINITY;
   int at = INT_MAX;
   bool nan = false;
-  for (int c = part * r.per_part + tid; c < c1; c += 256) {
+  for (int c = c0 + tid; c < c1; c += kTallyThreads) {
     float v[E];
     r.load(c, v);
 #pragma unroll
@@ -198,62 +233,27 @@ __global__ __launch_bounds__(256) void sample_peak_kernel(SampleArgs a) {
     }
   }
   if (nan) best = NAN;
-#pragma unroll
-  for (int o = 32; o > 0; o >>= 1) {
-    const float ov = __shfl_xor(best, o);
-    const int oi = __shfl_xor(at, o);
-    if (best == best && (ov != ov || ov > best || (ov == best && oi < at))) {
-      best = ov;
-      at = oi;
-    }
-  }
+  wave_peak(best, at);
   if ((tid & 63) == 0) {
     sv[tid >> 6] = best;
     si[tid >> 6] = at;
   }
   __syncthreads();
-  if (tid == 0) {
-    for (int w = 1; w < 4; ++w)
-      if (best == best && (sv[w] != sv[w] || sv[w] > best || (sv[w] == best && si[w] < at))) {
-        best = sv[w];
-        at = si[w];
-      }
-    a.peak[(size_t)row * a.parts + part] = float2_t{best, __builtin_bit_cast(float, at)};
-  }
-}
-
-// grid = (parts, rows), 256 threads.  Every thread keeps its own column of the
-// bins in LDS, so the additions need no atomics, meet no bank conflicts
-// between lanes and happen in a fixed order.
-template <typename T>
-__global__ __launch_bounds__(256) void sample_tally_kernel(SampleArgs a) {
-  constexpr int E = Row<T>::E;
-  __shared__ double mass[kBins][256];
-  __shared__ uint32_t count[kBins][256];
-  __shared__ Exp2Table table;
-  const int row = blockIdx.y, part = blockIdx.x, tid = threadIdx.x;
-  const Ask q = read_ask(a, row);
-  int at;
-  const float top = row_peak(a, row, tid & 63, at);
-  if (q.none || q.greedy || !(top > -INFINITY)) return;   // the pick needs no weights
-  fill_exp2(table, tid);
-#pragma unroll
-  for (int b = 0; b < kBins; ++b) {
-    mass[b][tid] = 0.0;
-    count[b][tid] = 0;
-  }
-  __syncthreads();
-  const Row<T> r(a, row);
-  const int c1 = min((part + 1) * r.per_part, r.chunks);
-  for (int c = part * r.per_part + tid; c < c1; c += 256) {
+  best = sv[0];
+  at = si[0];
+  for (int w = 1; w < 4; ++w) keep_peak(best, at, sv[w], si[w]);
+  if (tid == 0) a.peak[(size_t)row * a.parts + part] = float2_t{best, __builtin_bit_cast(float, at)};
+  if (q.none || q.greedy || best != best) return;   // the pick needs no weights
+  const Scale s(q.to_octaves, best);
+  for (int c = c0 + tid; c < c1; c += kTallyThreads) {
     float v[E];
     const uint32_t in = r.load(c, v);
 #pragma unroll
     for (int e = 0; e < E; ++e) {
       if (!((in >> e) & 1)) continue;
-      const double z = octaves(v[e], top, q.to_octaves);
-      const int b = bin_of(z);
-      mass[b][tid] += exp2_64(z, table);
+      const double y = s.y(v[e]);
+      const int b = bin_of(s.below(y));
+      mass[b][tid] += exp2_64(y - s.base, table);
       ++count[b][tid];
     }
   }
@@ -262,7 +262,7 @@ __global__ __launch_bounds__(256) void sample_tally_kernel(SampleArgs a) {
   const int b = tid >> 4, j = tid & 15;
   double m = 0.0;
   uint32_t n = 0;
-  for (int k = j; k < 256; k += 16) {
+  for (int k = j; k < kTallyThreads; k += 16) {
     m += mass[b][k];
     n += count[b][k];
   }
@@ -272,9 +272,190 @@ __global__ __launch_bounds__(256) void sample_tally_kernel(SampleArgs a) {
     n += __shfl_xor(n, o);
   }
   if (j == 0) {
-    const size_t at2 = ((size_t)row * a.parts + part) * kBins + b;
-    a.mass[at2] = m;
-    a.count[at2] = n;
+    const size_t to = ((size_t)row * a.parts + part) * kBins + b;
+    a.mass[to] = m;
+    a.count[to] = n;
+  }
+}
+
+// The row's largest logit, in every lane of every wave.
+__device__ __forceinline__ float row_peak(const SampleArgs& a, int row, int lane, int& at) {
+  float best = -INFINITY;
+  at = INT_MAX;
+  if (lane < a.parts) {
+    const float2_t e = a.peak[(size_t)row * a.parts + lane];
+    best = e.x;
+    const float y = e.y;
+    at = __builtin_bit_cast(int, y);
+  }
+  wave_peak(best, at);
+  return best;
+}
+
+// A row's tallies against the row's own base, of each part and altogether.
+struct RowTally {
+  double mass[kBins];
+  uint32_t count[kBins];
+  double part_mass[kMaxParts][kBins];
+  uint32_t part_count[kMaxParts][kBins];
+  double raw_mass[kMaxParts][kBins];        // against the part's base
+  uint32_t raw_count[kMaxParts][kBins];
+  int shift[kMaxParts];       // octaves from the row's base down to the part's (64: as many or more)
+  double scale[kMaxParts];    // 2^-octaves
+};
+
+// By THREADS >= 256 threads, with barriers; the sums in a fixed order.
+template <int THREADS>
+__device__ __forceinline__ void read_tally(const SampleArgs& a, const Scale& s, int row, int tid, RowTally& t) {
+  const size_t from = (size_t)row * a.parts;
+  if (tid < a.parts) {
+    const float top = a.peak[from + tid].x;
+    // Base against base: a part of -inf, or a finite one below +inf, is out of sight.
+    const double down = isinf(s.top) || isinf(top) ? (top == s.top ? 0.0 : INFINITY)
+                                                   : s.base - Scale(s.to_octaves, top).base;
+    t.shift[tid] = (int)fmin(down, 64.0);
+    t.scale[tid] = down < 1074.0 ? ldexp(1.0, -(int)down) : 0.0;
+  }
+  for (int e = tid; e < a.parts * kBins; e += THREADS) {
+    (&t.raw_mass[0][0])[e] = a.mass[from * kBins + e];
+    (&t.raw_count[0][0])[e] = a.count[from * kBins + e];
+  }
+  __syncthreads();
+  for (int e = tid; e < a.parts * kBins; e += THREADS) {
+    const int p = e / kBins, b = e % kBins;
+    double m = 0.0;
+    uint32_t n = 0;
+    for (int i = 0; i <= b; ++i)
+      if ((i == kBins - 1 ? i : bin_of((double)(bin_depth(i) + t.shift[p]))) == b) {
+        m += t.raw_mass[p][i];
+        n += t.raw_count[p][i];
+      }
+    t.part_mass[p][b] = m * t.scale[p];
+    t.part_count[p][b] = n;
+  }
+  __syncthreads();
+  if (tid < 256) {
+    const int b = tid >> 4;
+    double m = 0.0;
+    uint32_t n = 0;
+    for (int p = tid & 15; p < a.parts; p += 16) {
+      m += t.part_mass[p][b];
+      n += t.part_count[p][b];
+    }
+#pragma unroll
+    for (int o = 8; o > 0; o >>= 1) {
+      m += __shfl_xor(m, o);
+      n += __shfl_xor(n, o);
+    }
+    if ((tid & 15) == 0) {
+      t.mass[b] = m;
+      t.count[b] = n;
+    }
+  }
+  __syncthreads();
+}
+
+// The bins whose tokens decide: top-k ends in bin `by_k`, top-p (where
+// top-k is off; under top-k it follows from what that leaves) in `by_p`,
+// min-p in `floor`; kBins where one is off.  The list takes the bins lo ..
+// hi, none if hi < lo.
+struct Range {
+  int by_k, by_p, floor, lo, hi;
+  uint32_t want;       // tokens that top-k leaves of bin by_k
+  double before;       // mass in front of bin by_k
+  double whole;        // mass of all bins
+  double min_y;        // the smallest y that min-p leaves
+};
+
+__device__ __forceinline__ int mass_bin(const RowTally& t, int last, double goal, double& before) {
+  int b = 0;
+  before = 0.0;
+  for (; b < last && before + t.mass[b] < goal; ++b) before += t.mass[b];
+  return b;
+}
+
+__device__ __forceinline__ Range find_range(const SampleArgs& a, const Ask& q, const Scale& s, const RowTally& t) {
+  Range g{kBins, kBins, kBins, 0, -1, 0, 0.0, 0.0, -INFINITY};
+  for (int b = 0; b < kBins; ++b) g.whole += t.mass[b];
+  if (q.min_p > -INFINITY) {
+    g.min_y = s.y(s.top) + q.min_p;
+    g.floor = bin_of(s.below(g.min_y));
+  }
+  if (q.top_k < a.vocab) {
+    g.want = (uint32_t)q.top_k;
+    for (g.by_k = 0; g.by_k < kBins - 1 && t.count[g.by_k] < g.want; ++g.by_k) {
+      g.want -= t.count[g.by_k];
+      g.before += t.mass[g.by_k];
+    }
+    g.lo = 0;
+    g.hi = g.by_k;
+  } else if (q.top_p < 1.0) {
+    double before;
+    g.by_p = mass_bin(t, kBins - 1, q.top_p * g.whole, before);
+    g.lo = min(g.by_p, g.floor);
+    g.hi = g.by_p;
+  } else if (g.floor < kBins) {
+    g.lo = g.hi = g.floor;
+  }
+  return g;
+}
+
+// Tokens of the list; more than it can hold: the pick goes over the row instead.
+__device__ __forceinline__ uint32_t list_length(const RowTally& t, const Range& g) {
+  uint32_t n = 0;
+  for (int b = g.lo; b <= g.hi; ++b) n += t.count[b];
+  return n;
+}
+
+// grid = (parts, rows), 256 threads: the part's tokens of the bins lo .. hi
+// go to its place in the row's list (their order there does not matter).
+template <typename T>
+__global__ __launch_bounds__(256) void sample_gather_kernel(SampleArgs a) {
+  constexpr int E = Row<T>::E;
+  __shared__ RowTally tally;
+  __shared__ int offset, end;
+  const int row = blockIdx.y, part = blockIdx.x, tid = threadIdx.x, lane = tid & 63;
+  const Ask q = read_ask(a, row);
+  int first;
+  const float top = row_peak(a, row, lane, first);
+  if (q.none || q.greedy || !(top > -INFINITY)) return;
+  const Scale s(q.to_octaves, top);
+  read_tally<256>(a, s, row, tid, tally);
+  const Range g = find_range(a, q, s, tally);
+  if (g.hi < g.lo || list_length(tally, g) > (uint32_t)a.list_cap) return;
+  if (tid < 64) {   // the part's place: the tokens of the parts in front of it
+    uint32_t n = 0;
+    if (lane < a.parts)
+      for (int b = g.lo; b <= g.hi; ++b) n += tally.part_count[lane][b];
+    uint32_t upto = n;
+#pragma unroll
+    for (int o = 1; o < 64; o <<= 1) {
+      const uint32_t u = __shfl_up(upto, o);
+      if (lane >= o) upto += u;
+    }
+    if (lane == part) {
+      offset = (int)(upto - n);
+      end = (int)upto;
+    }
+  }
+  __syncthreads();
+  if (offset == end) return;
+  const Row<T> r(a, row);
+  const int c1 = min((part + 1) * r.per_part, r.chunks);
+  float2_t* list = a.list + (size_t)row * a.list_cap;
+  const int limit = end;
+  __syncthreads();
+  for (int c = part * r.per_part + tid; c < c1; c += 256) {
+    float v[E];
+    const uint32_t in = r.load(c, v);
+#pragma unroll
+    for (int e = 0; e < E; ++e) {
+      const int b = bin_of(s.below(s.y(v[e])));
+      if (((in >> e) & 1) && b >= g.lo && b <= g.hi) {
+        const int to = atomicAdd(&offset, 1);
+        if (to < limit) list[to] = float2_t{v[e], __builtin_bit_cast(float, r.index(c) + e)};
+      }
+    }
   }
 }
 
@@ -307,118 +488,265 @@ struct Key<float> {
   }
 };
 
-struct PickShared {
-  Exp2Table table;
-  double mass[kBins];
-  uint32_t count[kBins];
-  double part_mass[kMaxParts];
-  uint32_t part_ties[kMaxParts];
-  uint32_t digit_count[256];
-  unsigned long long digit_mass[256];
-  double wave_d[16];
-  uint32_t wave_n[16];
-  int wave_i[16];
-  // broadcasts
-  uint32_t prefix, ties, ties_before;
-  double above, target;
-  int part;
-};
-
 // The value at which a cut ends, among the row's tokens of one bin.
 struct Cut {
-  int bin;          // tokens of lower bins all stay, of higher ones none
+  int bin;          // tokens of lower bins all stay, of higher ones none (kBins: all stay)
   uint32_t key;     // of this bin: all above it stay, and the first `ties` that equal it
   uint32_t ties;
   double kept;      // mass of this bin's tokens that stay
 };
 
-// Finds the key of bin `bin` at which `want` is reached counting down from the
-// largest: `want` tokens (by_mass false), or the mass `goal`, of which
-// `before` lies in front of the bin.  One byte of the key at a time: a pass
-// over the row adds the tokens of the bin that share the bytes found so far to
-// 256 counters; masses are whole numbers of 2^-mass_bits of the bin's largest
-// weight (2^-45 for a vocabulary of 2^17 to 2^18), so that their sum does not
-// depend on the order.
+struct PickShared {
+  Exp2Table table;
+  RowTally tally;
+  uint32_t step_count[kSub];
+  unsigned long long step_mass[kSub];
+  uint64_t order[kMostSorted];    // (order of the value, index), the first of the order smallest
+  double weight[kMostSorted];
+  double part_mass[kMaxParts];
+  unsigned long long part_edge[kMaxParts];
+  uint32_t part_ties[kMaxParts];
+  double wave_d[16];
+  uint32_t wave_n[16];
+  int wave_i[16];
+  // what one thread found for all
+  int step, n;
+  uint32_t left, ties;
+  double above, target;
+  int part;
+  bool part_has_ties;
+};
+
 template <typename T>
-__device__ Cut find_cut(const SampleArgs& a, const Row<T>& r, const Ask& q, float top, int bin, bool by_mass,
-                        uint32_t want, double before, double goal, PickShared& s) {
-  constexpr int E = Row<T>::E;
-  const int tid = threadIdx.x;
-  const double unit = ldexp(1.0, a.mass_bits + bin), per_unit = ldexp(1.0, -a.mass_bits - bin);
-  if (tid == 0) {
-    s.prefix = 0;
-    s.ties = want;
-    s.above = 0.0;     // mass of the bin above the bytes found so far
-  }
-  for (int byte = Key<T>::kBytes - 1; byte >= 0; --byte) {
-    for (int i = tid; i < 256; i += kPickThreads) {
-      s.digit_count[i] = 0;
-      s.digit_mass[i] = 0;
-    }
-    __syncthreads();
-    const uint32_t prefix = s.prefix;
-    for (int c = tid; c < r.chunks; c += kPickThreads) {
-      float v[E];
-      const uint32_t in = r.load(c, v);
+struct Picker {
+  static constexpr int E = Row<T>::E;
+  const SampleArgs& a;
+  const Row<T>& r;
+  const Scale& s;
+  PickShared& sh;
+  const float2_t* list;   // nullptr: the tokens come from the row
+  int listed;
+  int tid;
+
+  // f(value, index) over the listed tokens, or all of the row's.
+  template <typename F>
+  __device__ __forceinline__ void each(F f) const {
+    if (list != nullptr) {
+      for (int i = tid; i < listed; i += kPickThreads) {
+        const float2_t e = list[i];
+        const float y = e.y;
+        f(e.x, __builtin_bit_cast(int, y));
+      }
+    } else {
+      for (int c = tid; c < r.chunks; c += kPickThreads) {
+        float v[E];
+        const uint32_t in = r.load(c, v);
 #pragma unroll
-      for (int e = 0; e < E; ++e) {
-        if (!((in >> e) & 1)) continue;
-        const double z = octaves(v[e], top, q.to_octaves);
-        if (bin_of(z) != bin) continue;
-        const uint32_t k = Key<T>::of(v[e]);
-        if (byte + 1 < Key<T>::kBytes && (k >> (8 * byte + 8)) != prefix) continue;
-        const int d = (k >> (8 * byte)) & 255;
-        atomicAdd(&s.digit_count[d], 1u);
-        atomicAdd(&s.digit_mass[d], (unsigned long long)rint(exp2_64(z, s.table) * unit));
+        for (int e = 0; e < E; ++e)
+          if ((in >> e) & 1) f(v[e], r.index(c) + e);
+      }
+    }
+  }
+
+  __device__ __forceinline__ uint64_t order_of(float v, int index) const {
+    return ((uint64_t)(~Key<T>::of(v)) << 32) | (uint32_t)index;
+  }
+
+  // One step of 256 down a bin (`byte` = kBytes), or down the values of its
+  // step `sub` that share the leading bytes of the key: which step holds the
+  // end, what lies above it.  The last bin, which has no end, goes in eighths
+  // of an octave.  Masses are whole numbers of 2^-mass_bits of the power of two
+  // next above the bin's weights, so that their sum does not depend on the
+  // order.
+  __device__ __forceinline__ int sub_of(int bin, double y) const {
+    const double per = bin < 8 ? kSub : bin < kBins - 1 ? kSub / 4 : 8;
+    return (int)fmin((s.base + 1.0 - bin_depth(bin) - y) * per, (double)(kSub - 1));
+  }
+  __device__ __forceinline__ void walk(int bin, bool by_mass, double before, double goal, int byte, int sub,
+                                       uint32_t prefix) {
+    const int bits = a.mass_bits + bin_depth(bin) - 1;
+    const double unit = ldexp(1.0, bits), per_unit = ldexp(1.0, -bits);
+    for (int i = tid; i < kSub; i += kPickThreads) {
+      sh.step_count[i] = 0;
+      sh.step_mass[i] = 0;
+    }
+    __syncthreads();
+    each([&](float v, int) {
+      const double y = s.y(v);
+      if (bin_of(s.below(y)) != bin) return;
+      int d = sub_of(bin, y);
+      if (byte < Key<T>::kBytes) {
+        const uint32_t k = Key<T>::of(v);
+        if (d != sub || (byte + 1 < Key<T>::kBytes && (k >> (8 * byte + 8)) != prefix)) return;
+        d = 255 - (int)((k >> (8 * byte)) & 255);
+      }
+      atomicAdd(&sh.step_count[d], 1u);
+      atomicAdd(&sh.step_mass[d], (unsigned long long)rint(exp2_64(y - s.base, sh.table) * unit));
+    });
+    __syncthreads();
+    if (tid < 64) {   // four steps per lane
+      uint32_t n[4], sum_n = 0;
+      unsigned long long m[4], sum_m = 0;
+#pragma unroll
+      for (int i = 0; i < 4; ++i) {
+        n[i] = sh.step_count[4 * tid + i];
+        m[i] = sh.step_mass[4 * tid + i];
+        sum_n += n[i];
+        sum_m += m[i];
+      }
+      uint32_t run_n = sum_n;
+      unsigned long long run_m = sum_m;
+#pragma unroll
+      for (int o = 1; o < 64; o <<= 1) {
+        const uint32_t un = __shfl_up(run_n, o);
+        const unsigned long long um = __shfl_up(run_m, o);
+        if (tid >= o) {
+          run_n += un;
+          run_m += um;
+        }
+      }
+      run_n -= sum_n;
+      run_m -= sum_m;
+      // The first step that reaches the end; roundings can leave a mass a hair out of reach: the last with tokens then.
+      const uint32_t left = sh.left;
+      const double above = sh.above;
+      int hit = kSub, last = -1;
+      uint32_t hit_n = 0, last_n = 0;
+      unsigned long long hit_m = 0, last_m = 0;
+#pragma unroll
+      for (int i = 0; i < 4; ++i) {
+        if (n[i] != 0) {
+          const bool ends = by_mass ? before + above + (double)(run_m + m[i]) * per_unit >= goal : run_n + n[i] >= left;
+          if (ends && hit == kSub) {
+            hit = 4 * tid + i;
+            hit_n = run_n;
+            hit_m = run_m;
+          }
+          last = 4 * tid + i;
+          last_n = run_n;
+          last_m = run_m;
+        }
+        run_n += n[i];
+        run_m += m[i];
+      }
+      const uint64_t hits = __builtin_amdgcn_ballot_w64(hit < kSub);
+      const uint64_t lasts = __builtin_amdgcn_ballot_w64(last >= 0);
+      const bool mine = hits ? tid == __builtin_ctzll(hits) : lasts ? tid == 63 - __builtin_clzll(lasts) : tid == 0;
+      if (mine) {
+        const int d = hits ? hit : max(last, 0);
+        sh.step = d;
+        sh.n = (int)sh.step_count[d];
+        if (!by_mass) sh.left = left - (hits ? hit_n : last_n);
+        sh.above = above + (double)(hits ? hit_m : last_m) * per_unit;
       }
     }
     __syncthreads();
+  }
+
+  // Where the count `want`, or the mass `goal` of which `before` lies in front
+  // of the bin, is reached among the tokens of bin `bin`.
+  __device__ __forceinline__ Cut find_cut(int bin, bool by_mass, uint32_t want, double before, double goal) {
     if (tid == 0) {
-      uint32_t left = s.ties;
-      double above = s.above;
-      int d = 255, last = -1;
-      uint32_t last_left = 0;
-      double last_above = 0.0;
-      for (; d >= 0; --d) {
-        const uint32_t n = s.digit_count[d];
-        if (n == 0) continue;
-        const double m = (double)s.digit_mass[d] * per_unit;
-        last = d;
-        last_left = left;
-        last_above = above;
-        if (by_mass ? before + above + m >= goal : n >= left) break;
-        left -= n;
-        above += m;
-      }
-      // Rounding may leave the goal a hair out of reach: the smallest value then.
-      s.prefix = (prefix << 8) | (uint32_t)max(last, 0);
-      s.ties = last_left;
-      s.above = last_above;
-      s.wave_n[0] = last >= 0 ? s.digit_count[last] : 0;
+      sh.left = want;
+      sh.above = 0.0;     // mass of the bin in front of the steps found so far
+      sh.ties = 0;
     }
+    // The step of the bin; where many of tokens share it, most of them equal, the bytes of the key.
+    int sub = 0;
+    uint32_t prefix = 0;
+    bool few = false;
+    for (int byte = Key<T>::kBytes; byte >= 0; --byte) {
+      walk(bin, by_mass, before, goal, byte, sub, prefix);
+      if (byte == Key<T>::kBytes) {
+        sub = sh.step;
+        few = sh.n <= kMostSorted;
+        if (few) break;
+      } else {
+        prefix = (prefix << 8) | (uint32_t)(255 - sh.step);
+      }
+      __syncthreads();
+    }
+    Cut cut{bin, 0, 0, 0.0};
+    if (few) {
+      const int n = sh.n;
+      __syncthreads();
+      if (tid == 0) sh.n = 0;
+      __syncthreads();
+      each([&](float v, int index) {
+        const double y = s.y(v);
+        if (bin_of(s.below(y)) != bin || sub_of(bin, y) != sub) return;
+        const int to = atomicAdd(&sh.n, 1);
+        if (to < kMostSorted) sh.order[to] = order_of(v, index);
+      });
+      __syncthreads();
+      uint64_t mine = ~0ull;
+      int rank = 0;
+      if (tid < n) {
+        mine = sh.order[tid];
+        for (int j = 0; j < n; ++j) rank += sh.order[j] < mine;
+      }
+      __syncthreads();
+      if (tid < n) {
+        sh.order[rank] = mine;
+        sh.weight[rank] = exp2_64(s.y(Key<T>::value(~(uint32_t)(mine >> 32))) - s.base, sh.table);
+      }
+      __syncthreads();
+      if (tid < 64) {   // how many stay, 64 at a time, and the ones among them that equal the last
+        double run = sh.above;
+        int stay = 0;
+        for (int j0 = 0; j0 < n; j0 += 64) {
+          const double w = j0 + tid < n ? sh.weight[j0 + tid] : 0.0;
+          double upto = w;
+#pragma unroll
+          for (int o = 1; o < 64; o <<= 1) {
+            const double u = __shfl_up(upto, o);
+            if (tid >= o) upto += u;
+          }
+          const int j = j0 + tid;
+          const bool in = j < n && (j == 0 || (by_mass ? before + run + (upto - w) < goal : j < (int)sh.left));
+          const int k = __popcll(__builtin_amdgcn_ballot_w64(in));   // the lanes 0 .. k - 1
+          if (k == 0) break;
+          stay += k;
+          run += __shfl(upto, k - 1);
+          if (k < 64) break;
+        }
+        stay = max(stay, 1);
+        const uint32_t end = (uint32_t)(sh.order[stay - 1] >> 32);
+        int ties = 0;
+        for (int j0 = 0; j0 < stay; j0 += 64)
+          ties += __popcll(__builtin_amdgcn_ballot_w64(j0 + tid < stay && (uint32_t)(sh.order[min(j0 + tid, stay - 1)] >> 32) == end));
+        if (tid == 0) {
+          sh.left = ~end;
+          sh.ties = (uint32_t)ties;
+          sh.above = run;
+        }
+      }
+      __syncthreads();
+      cut.key = sh.left;
+      cut.ties = sh.ties;
+      cut.kept = sh.above;
+      __syncthreads();
+      return cut;
+    }
+    cut.key = prefix;
+    const double w = exp2_64(s.y(Key<T>::value(prefix)) - s.base, sh.table);
+    if (by_mass) {
+      const double need = ceil((goal - before - sh.above) / w);
+      cut.ties = need >= (double)sh.n ? (uint32_t)sh.n : (uint32_t)fmax(need, 1.0);
+    } else {
+      cut.ties = min(sh.left, (uint32_t)sh.n);
+    }
+    cut.kept = sh.above + cut.ties * w;
     __syncthreads();
+    return cut;
   }
-  Cut cut;
-  cut.bin = bin;
-  cut.key = s.prefix;
-  const double w = exp2_64(octaves(Key<T>::value(cut.key), top, q.to_octaves), s.table);
-  const uint32_t n = s.wave_n[0];
-  if (by_mass) {
-    const double need = ceil((goal - before - s.above) / w);
-    cut.ties = need >= (double)n ? n : (uint32_t)fmax(need, 1.0);
-  } else {
-    cut.ties = min(s.ties, n);
-  }
-  cut.kept = s.above + cut.ties * w;
-  __syncthreads();
-  return cut;
-}
+};
 
 // grid = rows, 1024 threads.
 template <typename T>
 __global__ __launch_bounds__(kPickThreads) void sample_pick_kernel(SampleArgs a) {
   constexpr int E = Row<T>::E;
-  __shared__ PickShared s;
+  __shared__ PickShared sh;
   const int row = blockIdx.x, tid = threadIdx.x, lane = tid & 63;
   const int wave = __builtin_amdgcn_readfirstlane(tid >> 6);
   const Ask q = read_ask(a, row);
@@ -429,151 +757,125 @@ __global__ __launch_bounds__(kPickThreads) void sample_pick_kernel(SampleArgs a)
     return;
   }
   const Row<T> r(a, row);
-  fill_exp2(s.table, tid);
-  const double* mass = a.mass + (size_t)row * a.parts * kBins;
-  const uint32_t* count = a.count + (size_t)row * a.parts * kBins;
-  if (tid < kBins) {
-    double m = 0.0;
-    uint32_t n = 0;
-    for (int p = 0; p < a.parts; ++p) {
-      m += mass[p * kBins + tid];
-      n += count[p * kBins + tid];
-    }
-    s.mass[tid] = m;
-    s.count[tid] = n;
-  }
-  __syncthreads();
+  const Scale s(q.to_octaves, top);
+  fill_exp2(sh.table, tid);
+  read_tally<kPickThreads>(a, s, row, tid, sh.tally);
+  const Range g = find_range(a, q, s, sh.tally);
+  const uint32_t listed = list_length(sh.tally, g);
+  Picker<T> pick{a, r, s, sh, listed <= (uint32_t)a.list_cap ? a.list + (size_t)row * a.list_cap : nullptr,
+                 (int)listed, tid};
 
-  // Where top-k ends, then top-p of what it leaves (every thread the same).
+  // Where top-k ends, then top-p of what it leaves.
   Cut cut{kBins, 0, 0, 0.0};
-  double whole = 0.0;
-  for (int b = 0; b < kBins; ++b) whole += s.mass[b];
-  if (q.top_k < a.vocab) {
-    uint32_t left = (uint32_t)q.top_k;
-    double before = 0.0;
-    int b = 0;
-    for (; b < kBins - 1 && s.count[b] < left; ++b) {
-      left -= s.count[b];
-      before += s.mass[b];
-    }
-    cut = find_cut(a, r, q, top, b, false, left, 0.0, 0.0, s);
-    whole = before + cut.kept;
-  }
-  if (q.top_p < 1.0) {
+  double whole = g.whole;
+  for (int stage = 0; stage < 2; ++stage) {
+    const bool by_mass = stage == 1;
+    if (by_mass ? q.top_p == 1.0 : g.by_k == kBins) continue;
     const double goal = q.top_p * whole;
-    double before = 0.0;
-    int b = 0;
-    const int last = min(cut.bin, kBins - 1);
-    for (; b < last && before + s.mass[b] < goal; ++b) before += s.mass[b];
-    const Cut by_p = find_cut(a, r, q, top, b, true, 0, before, goal, s);
-    // Both end at the same value: the fewer ties.  Otherwise top-p's is the higher one, but for roundings.
-    if (by_p.bin < cut.bin || by_p.key > cut.key) cut = by_p;
-    else if (by_p.key == cut.key) cut.ties = min(cut.ties, by_p.ties);
+    double before = g.before;
+    int bin = g.by_k;
+    if (by_mass) bin = mass_bin(sh.tally, min(cut.bin, kBins - 1), goal, before);
+    const Cut end = pick.find_cut(bin, by_mass, g.want, before, goal);
+    if (!by_mass) whole = before + end.kept;
+    // Both may end at one value: the fewer ties.  Otherwise top-p's is the higher one, but for roundings.
+    if (end.bin < cut.bin || end.key > cut.key) cut = end;
+    else if (end.key == cut.key) cut.ties = min(cut.ties, end.ties);
   }
-  const int floor_bin = q.floor == -INFINITY ? kBins : bin_of(q.floor);
-  const int edge = min(cut.bin, floor_bin);   // the only bin of which some tokens stay and some go
+  const int edge = min(cut.bin, g.floor);   // the only bin of which some tokens stay and some go
   // 1: stays, 2: stays while there are ties left.
-  auto stays = [&](float v, double z) -> int {
-    const int b = bin_of(z);
-    if (b > edge) return 0;
-    if (b < edge) return 1;
-    if (z < q.floor) return 0;
+  auto stays = [&](float v, double y) -> int {
+    const int b = bin_of(s.below(y));
+    if (b != edge) return b < edge;
+    if (y < g.min_y) return 0;
     if (b < cut.bin) return 1;
     const uint32_t k = Key<T>::of(v);
     return k > cut.key ? 1 : k == cut.key ? 2 : 0;
   };
-  const double tie_weight =
-      cut.bin < kBins ? exp2_64(octaves(Key<T>::value(cut.key), top, q.to_octaves), s.table) : 0.0;
+  auto weight = [&](double y) { return exp2_64(y - s.base, sh.table); };
 
-  // What stays of every part: the bins in front of the edge, and its own tokens of the edge, a wave per part.
-  for (int p = wave; p < a.parts; p += 16) {
-    double m = 0.0;
-    uint32_t ties = 0;
-    if (edge < kBins && count[p * kBins + edge] != 0) {
-      const int c1 = min((p + 1) * r.per_part, r.chunks);
-      for (int c = p * r.per_part + lane; c < c1; c += 64) {
-        float v[E];
-        const uint32_t in = r.load(c, v);
-#pragma unroll
-        for (int e = 0; e < E; ++e) {
-          if (!((in >> e) & 1)) continue;
-          const double z = octaves(v[e], top, q.to_octaves);
-          if (bin_of(z) != edge) continue;
-          const int st = stays(v[e], z);
-          if (st == 1) m += exp2_64(z, s.table);
-          ties += st == 2;
-        }
-      }
-#pragma unroll
-      for (int o = 32; o > 0; o >>= 1) {
-        m += __shfl_xor(m, o);
-        ties += __shfl_xor(ties, o);
-      }
-    }
-    for (int b = 0; b < min(edge, kBins); ++b) m += mass[p * kBins + b];
-    if (lane == 0) {
-      s.part_mass[p] = m;
-      s.part_ties[p] = ties;
-    }
+  // What stays of every part: the bins in front of the edge, and its own tokens of the edge.
+  const int bits = a.mass_bits + bin_depth(edge) - 1;
+  const double unit = ldexp(1.0, bits), per_unit = ldexp(1.0, -bits);
+  if (tid < kMaxParts) {
+    sh.part_edge[tid] = 0;
+    sh.part_ties[tid] = 0;
   }
   __syncthreads();
-  if (tid == 0) {
-    uint32_t ties = 0;
-    double all = 0.0;
-    for (int p = 0; p < a.parts; ++p) {
-      const uint32_t n = s.part_ties[p];
-      const uint32_t kept = ties < cut.ties ? min(n, cut.ties - ties) : 0;
-      s.part_ties[p] = ties;
-      s.part_mass[p] += kept * tie_weight;
-      ties += n;
-      all += s.part_mass[p];
+  if (edge < kBins)
+    pick.each([&](float v, int index) {
+      const double y = s.y(v);
+      if (bin_of(s.below(y)) != edge) return;
+      const int st = stays(v, y);
+      const int p = (index + r.lead) / E / r.per_part;
+      if (st == 1) atomicAdd(&sh.part_edge[p], (unsigned long long)rint(weight(y) * unit));
+      if (st == 2) atomicAdd(&sh.part_ties[p], 1u);
+    });
+  __syncthreads();
+  if (wave == 0) {   // a part per lane
+    double m = 0.0;
+    uint32_t n = 0;
+    if (lane < a.parts) {
+      for (int b = 0; b < edge; ++b) m += sh.tally.part_mass[lane][b];
+      m += (double)sh.part_edge[lane] * per_unit;
+      n = sh.part_ties[lane];
     }
-    const double target = (double)a.uniform[row] * all;
-    int part = 0;
-    double run = 0.0, before = 0.0;
-    for (int p = 0; p < a.parts; ++p) {
-      if (!(s.part_mass[p] > 0.0)) continue;
-      part = p;
-      before = run;
-      run += s.part_mass[p];
-      if (run > target) break;
+    uint32_t ties = n;
+#pragma unroll
+    for (int o = 1; o < 64; o <<= 1) {
+      const uint32_t u = __shfl_up(ties, o);
+      if (lane >= o) ties += u;
     }
-    s.part = part;
-    s.target = target - before;
-    s.ties_before = s.part_ties[part];
+    ties -= n;   // in front of the part
+    // Signed on purpose: of the unsigned form, ties < cut.ties ? min(n, cut.ties - ties) : 0, hipcc 7.2 keeps a plain
+    // subtraction and drops the comparison.
+    const int kept = max(min((int)n, (int)cut.ties - (int)ties), 0);
+    if (kept > 0) m += kept * weight(s.y(Key<T>::value(cut.key)));
+    double upto = m;
+#pragma unroll
+    for (int o = 1; o < 64; o <<= 1) {
+      const double u = __shfl_up(upto, o);
+      if (lane >= o) upto += u;
+    }
+    const double target = (double)a.uniform[row] * __shfl(upto, 63);
+    const uint64_t some = __builtin_amdgcn_ballot_w64(m > 0.0);   // never none: the largest weighs at least 1
+    const uint64_t past = __builtin_amdgcn_ballot_w64(m > 0.0 && upto > target);
+    const int part = past ? __builtin_ctzll(past) : 63 - __builtin_clzll(some);
+    if (lane == part) {
+      sh.part = part;
+      sh.target = target - (upto - m);
+      sh.ties = ties;
+      sh.part_has_ties = n > 0;
+    }
   }
   __syncthreads();
 
   // The token inside the part: every thread a run of chunks, its mass, the sum of the threads in front of it.
-  const int part = s.part;
-  const double target = s.target;
+  const int part = sh.part;
+  const double target = sh.target;
   const int c0 = part * r.per_part, c1 = min(c0 + r.per_part, r.chunks);
   const int run = (c1 - c0 + kPickThreads - 1) / kPickThreads;
   const int t0 = min(c0 + tid * run, c1), t1 = min(t0 + run, c1);
-  auto scan_n = [&](uint32_t n) {   // exclusive sum over the threads
-    uint32_t x = n;
-#pragma unroll
-    for (int o = 1; o < 64; o <<= 1) {
-      const uint32_t u = __shfl_up(x, o);
-      if (lane >= o) x += u;
-    }
-    __syncthreads();
-    if (lane == 63) s.wave_n[wave] = x;
-    __syncthreads();
-    uint32_t base = 0;
-    for (int w = 0; w < wave; ++w) base += s.wave_n[w];
-    return base + x - n;
-  };
-  uint32_t my_ties = 0;
-  if (cut.bin == edge && edge < kBins)
+  uint32_t ties0 = sh.ties;
+  if (sh.part_has_ties) {
+    uint32_t mine = 0;
     for (int c = t0; c < t1; ++c) {
       float v[E];
       const uint32_t in = r.load(c, v);
 #pragma unroll
       for (int e = 0; e < E; ++e)
-        if ((in >> e) & 1) my_ties += stays(v[e], octaves(v[e], top, q.to_octaves)) == 2;
+        if ((in >> e) & 1) mine += stays(v[e], s.y(v[e])) == 2;
     }
-  const uint32_t ties0 = s.ties_before + scan_n(my_ties);
+    uint32_t x = mine;
+#pragma unroll
+    for (int o = 1; o < 64; o <<= 1) {
+      const uint32_t u = __shfl_up(x, o);
+      if (lane >= o) x += u;
+    }
+    if (lane == 63) sh.wave_n[wave] = x;
+    __syncthreads();
+    for (int w = 0; w < wave; ++w) ties0 += sh.wave_n[w];
+    ties0 += x - mine;
+  }
   double m = 0.0;
   uint32_t ties = ties0;
   for (int c = t0; c < t1; ++c) {
@@ -582,9 +884,9 @@ __global__ __launch_bounds__(kPickThreads) void sample_pick_kernel(SampleArgs a)
 #pragma unroll
     for (int e = 0; e < E; ++e) {
       if (!((in >> e) & 1)) continue;
-      const double z = octaves(v[e], top, q.to_octaves);
-      const int st = stays(v[e], z);
-      if (st == 1 || (st == 2 && ties++ < cut.ties)) m += exp2_64(z, s.table);
+      const double y = s.y(v[e]);
+      const int st = stays(v[e], y);
+      if (st == 1 || (st == 2 && ties++ < cut.ties)) m += weight(y);
     }
   }
   double x = m;
@@ -593,12 +895,12 @@ __global__ __launch_bounds__(kPickThreads) void sample_pick_kernel(SampleArgs a)
     const double u = __shfl_up(x, o);
     if (lane >= o) x += u;
   }
-  if (lane == 63) s.wave_d[wave] = x;
+  if (lane == 63) sh.wave_d[wave] = x;
   __syncthreads();
-  double base = 0.0;
-  for (int w = 0; w < wave; ++w) base += s.wave_d[w];
+  double sum = 0.0;
+  for (int w = 0; w < wave; ++w) sum += sh.wave_d[w];
+  sum += x - m;
   // The first token at which the running weight exceeds the target; failing that (roundings) the last that stays.
-  double sum = base + (x - m);
   int hit = INT_MAX, last = -1;
   ties = ties0;
   for (int c = t0; c < t1; ++c) {
@@ -607,10 +909,10 @@ __global__ __launch_bounds__(kPickThreads) void sample_pick_kernel(SampleArgs a)
 #pragma unroll
     for (int e = 0; e < E; ++e) {
       if (!((in >> e) & 1)) continue;
-      const double z = octaves(v[e], top, q.to_octaves);
-      const int st = stays(v[e], z);
+      const double y = s.y(v[e]);
+      const int st = stays(v[e], y);
       if (st == 1 || (st == 2 && ties++ < cut.ties)) {
-        const double w = exp2_64(z, s.table);
+        const double w = weight(y);
         sum += w;
         if (w > 0.0) {
           last = r.index(c) + e;
@@ -624,16 +926,15 @@ __global__ __launch_bounds__(kPickThreads) void sample_pick_kernel(SampleArgs a)
     hit = min(hit, __shfl_xor(hit, o));
     last = max(last, __shfl_xor(last, o));
   }
-  __syncthreads();
   if (lane == 0) {
-    s.wave_i[wave] = hit;
-    s.wave_n[wave] = (uint32_t)last;
+    sh.wave_i[wave] = hit;
+    sh.wave_n[wave] = (uint32_t)last;
   }
   __syncthreads();
   if (tid == 0) {
     for (int w = 1; w < 16; ++w) {
-      hit = min(hit, s.wave_i[w]);
-      last = max(last, (int)s.wave_n[w]);
+      hit = min(hit, sh.wave_i[w]);
+      last = max(last, (int)sh.wave_n[w]);
     }
     a.tokens[row] = hit != INT_MAX ? hit : last;
   }
@@ -651,6 +952,17 @@ int sample_parts(int64_t rows, int64_t vocab) {
 
 constexpr size_t kPartBytes = sizeof(float2_t) + kBins * (sizeof(double) + sizeof(uint32_t));
 
+// Entries of a row's list: all of the vocabulary, or what 64 MiB of lists leave for a row.
+int sample_list_cap(int64_t rows, int64_t vocab) {
+  int64_t cap = (64 << 20) / (int64_t)sizeof(float2_t) / rows;
+  if (cap < 4096) cap = 4096;
+  return (int)(cap < vocab ? cap : vocab);
+}
+
+size_t sample_bytes(int64_t rows, int64_t vocab) {
+  return (size_t)rows * (sample_parts(rows, vocab) * kPartBytes + sample_list_cap(rows, vocab) * sizeof(float2_t));
+}
+
 int sample_check(int64_t rows, int64_t vocab) {
   WQ_REQUIRE(rows >= 0 && rows <= 65535, WQ_ERR_INVALID_ARGUMENT, "rows must be in [0, 65535] (got %lld)",
              (long long)rows);
@@ -662,11 +974,11 @@ int sample_check(int64_t rows, int64_t vocab) {
 template <typename T>
 int launch_sample(const SampleArgs& a, hipStream_t s) {
   const dim3 grid((unsigned)a.parts, (unsigned)a.rows);
-  hipLaunchKernelGGL(sample_peak_kernel<T>, grid, dim3(256), 0, s, a);
-  int rc = check_launch("sample_peak");
+  hipLaunchKernelGGL(sample_tally_kernel<T>, grid, dim3(kTallyThreads), 0, s, a);
+  int rc = check_launch("sample_tally");
   if (rc != WQ_OK) return rc;
-  hipLaunchKernelGGL(sample_tally_kernel<T>, grid, dim3(256), 0, s, a);
-  rc = check_launch("sample_tally");
+  hipLaunchKernelGGL(sample_gather_kernel<T>, grid, dim3(256), 0, s, a);
+  rc = check_launch("sample_gather");
   if (rc != WQ_OK) return rc;
   hipLaunchKernelGGL(sample_pick_kernel<T>, dim3((unsigned)a.rows), dim3(kPickThreads), 0, s, a);
   return check_launch("sample_pick");
@@ -681,7 +993,7 @@ extern "C" int wq_sample_workspace_size(int64_t rows, int64_t vocab, size_t* byt
   WQ_REQUIRE(bytes, WQ_ERR_INVALID_ARGUMENT, "null pointer argument");
   const int rc = sample_check(rows, vocab);
   if (rc != WQ_OK) return rc;
-  *bytes = rows ? (size_t)rows * sample_parts(rows, vocab) * kPartBytes : 0;
+  *bytes = rows ? sample_bytes(rows, vocab) : 0;
   return WQ_OK;
 }
 
@@ -705,9 +1017,10 @@ extern "C" int wq_sample(const void* logits, int32_t logits_type, int64_t rows, 
              WQ_ERR_INVALID_ARGUMENT, "operands must be aligned to their size");
   SampleArgs a{};
   a.parts = sample_parts(rows, vocab);
-  const size_t places = (size_t)rows * a.parts;
-  WQ_REQUIRE(workspace && workspace_bytes >= places * kPartBytes && (uintptr_t)workspace % 8 == 0, WQ_ERR_WORKSPACE,
-             "sampling needs an 8-byte aligned workspace of %zu bytes (got %zu)", places * kPartBytes, workspace_bytes);
+  const size_t places = (size_t)rows * a.parts, need = sample_bytes(rows, vocab);
+  WQ_REQUIRE(workspace && workspace_bytes >= need && (uintptr_t)workspace % 8 == 0, WQ_ERR_WORKSPACE,
+             "sampling needs an 8-byte aligned workspace of %zu bytes (got %zu)", need, workspace_bytes);
+  a.list_cap = sample_list_cap(rows, vocab);
   a.logits = logits;
   a.row_stride = row_stride;
   a.mass_bits = 63;
@@ -727,7 +1040,8 @@ extern "C" int wq_sample(const void* logits, int32_t logits_type, int64_t rows, 
   a.tokens = tokens;
   a.peak = reinterpret_cast<float2_t*>(workspace);
   a.mass = reinterpret_cast<double*>(a.peak + places);
-  a.count = reinterpret_cast<uint32_t*>(a.mass + places * kBins);
+  a.list = reinterpret_cast<float2_t*>(a.mass + places * kBins);
+  a.count = reinterpret_cast<uint32_t*>(a.list + (size_t)rows * a.list_cap);
   return logits_type == WQ_LOGITS_F16 ? launch_sample<half_t>(a, as_stream(stream))
                                       : launch_sample<float>(a, as_stream(stream));
 }

@@ -3,9 +3,9 @@
 //
 // The new tokens of a sequence times the query heads of one kv head are the
 // rows that share its keys; row r of a sequence is token r / G, head r % G.
-// Rows are taken in tiles of 16, the keys of a tile are cut into chunks when
-// there are too few tiles to fill the machine, and every (sequence, tile,
-// chunk, kv head) is one workgroup.
+// Rows are taken in tiles of 16 (few tokens per sequence) or 128, the keys of a
+// tile are cut into chunks when there are too few tiles to fill the machine,
+// and every (sequence, tile, chunk, kv head) is one workgroup.
 #include "ondeviceinfer_paged.h"
 #include "wq_paged.h"
 #include "wq_status.h"
@@ -64,9 +64,14 @@ __device__ __forceinline__ Seq read_seq(const PagedArgs& a, int b) {
 struct Place {
   Seq s;
   int b, tile, chunk, chunks;
-  int64_t slot0;   // slot of the sequence's tile 0, chunk 0
+  int64_t slot0;   // the sequence's first slot
   bool found;
 };
+
+// The last tiles, which see the most keys, come first.
+__device__ __forceinline__ int64_t slot_of(const Place& p, int tile, int chunk) {
+  return p.slot0 + chunk * p.s.tiles + (p.s.tiles - 1 - tile);
+}
 
 template <int R, bool BY_TILE>
 __device__ __forceinline__ Place find_place(const PagedArgs& a, int place, int lane) {
@@ -115,7 +120,7 @@ __device__ __forceinline__ Place find_place(const PagedArgs& a, int place, int l
       p.chunks = __builtin_amdgcn_readlane(chunks, l);
       p.slot0 = slots_before + __builtin_amdgcn_readlane(upto - slots, l);
       const int rest = (int)want - __builtin_amdgcn_readlane(end - mine, l);
-      p.tile = rest % p.s.tiles;
+      p.tile = p.s.tiles - 1 - rest % p.s.tiles;
       p.chunk = rest / p.s.tiles;
       return p;
     }
@@ -145,6 +150,25 @@ __device__ __forceinline__ Groups load_groups(const PagedArgs& a, int b, int fir
     g.row = 0;
   }
   return g;
+}
+
+// What a row may attend of its sequence's positions.  Bit operations only, no
+// branches: of the short-circuit form (key < keys && (tree ? ... : ...)) inside
+// the unrolled score loops hipcc 7.2 loses the assignment of the hidden lanes.
+struct Sight {
+  int last;         // the last position attended
+  int base;         // where the new tokens start
+  uint64_t unseen;  // drafted ones among them that are not attended
+
+  __device__ __forceinline__ int operator()(int key) const {
+    const int j = key - base;
+    return (int)(key > last) | ((int)(j >= 0) & (int)((unseen >> (j & 63)) & 1));
+  }
+};
+
+__device__ __forceinline__ Sight row_sight(const PagedArgs& a, const Seq& s, int tok, int keys) {
+  if (a.mask != nullptr) return Sight{keys - 1, s.base, ~(uint64_t)a.mask[s.start + tok]};
+  return Sight{min(s.base + tok, keys - 1), s.base, 0};
 }
 
 // grid = slots * KV workgroups of four waves (flat id f: kv head f % KV, place
@@ -184,11 +208,10 @@ __global__ __launch_bounds__(256, 2) void paged_attention_rows_kernel(PagedArgs 
   const int last_tok = (min(p.tile * R + R, rows) - 1) / a.G;
   const bool tree = a.mask != nullptr;
   const bool refused = tree && p.s.count > kMaxTreeTokens;
-  const int64_t bits = tree ? a.mask[p.s.start + tok] : 0;
-  const int limit = p.s.base + tok;                 // causal: the last position attended
   // Keys of the tile, and the first key that not all of its rows attend.
   const int keys = refused ? 0 : tree ? p.s.keys : max(0, min(p.s.keys, p.s.base + last_tok + 1));
   const int ragged = tree ? p.s.base : p.s.base + first_tok + 1;
+  const Sight hidden = row_sight(a, p.s, tok, keys);
   const int per = p.s.blocks / p.chunks, extra = p.s.blocks % p.chunks;
   const int c0 = p.chunk * per + min(p.chunk, extra), c1 = c0 + per + (p.chunk < extra ? 1 : 0);
   const int nblk = min(c1, (keys + kKeys - 1) / kKeys) - c0;   // steps of this workgroup (may be negative)
@@ -259,10 +282,7 @@ __global__ __launch_bounds__(256, 2) void paged_attention_rows_kernel(PagedArgs 
         for (int h = 0; h < 2; ++h)
 #pragma unroll
           for (int v = 0; v < 4; ++v) {
-            const int key = k0 + 16 * h + 4 * kb + v;
-            const int j = key - p.s.base;
-            const bool seen = key < keys && (tree ? j < 0 || ((bits >> (j & 63)) & 1) : key <= limit);
-            if (!seen) sc[h][v] = -INFINITY;
+            sc[h][v] = hidden(k0 + 16 * h + 4 * kb + v) ? -INFINITY : sc[h][v];
           }
       }
       float mb = -INFINITY;
@@ -355,10 +375,256 @@ __global__ __launch_bounds__(256, 2) void paged_attention_rows_kernel(PagedArgs 
   *reinterpret_cast<half8_t*>(a.out + ((size_t)(p.s.start + t) * a.H + kvh * a.G + rr - t * a.G) * D + d) = o;
 }
 
-// The chunks of split tiles joined: grid = (tiles the call can have * KV, R /
-// 4), a wave per row, two elements of d per lane.  The weights 2^(m_c - M) of
-// up to 64 chunks are held one per lane and read out as each chunk is added,
-// in chunk order.
+// Chunks of prompts and trees of many tokens: tiles of 128 rows, grid and
+// places as above.  Wave w owns the rows 32 w .. 32 w + 31 of the tile; all
+// four share the keys and values, 64 at a time through two stages of LDS:
+//   K [key][d], 16-byte chunk c of row r at slot c ^ (r & 15);
+//   V^T [d][key slot], chunk c of row d at slot c ^ ((d >> 1) & 7), so that the
+//   lanes of a fragment read hit distinct banks.
+// Scores are computed transposed on 32x32x16 (A = 32 keys, B = 32 rows): lane
+// (l % 32, l / 32) = (ql, hh) holds in register r key 8 (r / 4) + 4 hh + r % 4
+// of row ql, and the probabilities, rounded to fp16, are the B operand of O^T
+// = V^T . P^T once V^T's key slots follow the same order: slot 8 h + 4 j + e
+// of a 16-key step holds key 8 j + 4 h + e.
+constexpr int kTileRows = 128;
+constexpr int kTileKeys = 64;
+constexpr int kTileKBytes = kTileKeys * kPagedDim * 2;
+constexpr int kTileStage = 2 * kTileKBytes;   // K block, then V^T block
+
+typedef float float16_t __attribute__((ext_vector_type(16)));
+
+__device__ __forceinline__ int vt_offset(int d, int pos) {
+  return kTileKBytes + d * (kTileKeys * 2) + ((((pos >> 3) ^ ((d >> 1) & 7))) << 4) + (pos & 7) * 2;
+}
+
+__global__ __launch_bounds__(256, 2) void paged_attention_tile_kernel(PagedArgs a) {
+  constexpr int R = kTileRows, D = kPagedDim;
+  extern __shared__ __attribute__((aligned(16))) uint8_t smem[];
+  const int tid = threadIdx.x, lane = tid & 63;
+  const int wave = __builtin_amdgcn_readfirstlane(tid >> 6);
+  const int ql = lane & 31, hh = lane >> 5;
+  const int kvh = blockIdx.x % a.KV, slot = blockIdx.x / a.KV;
+  const Place p = find_place<R, false>(a, slot, lane);
+  if (!p.found) return;
+
+  const int rows = p.s.count * a.G;
+  const int r0 = p.tile * R + 32 * wave;                    // this wave's first row
+  const int r = r0 + ql;
+  const int tok = min(r, rows - 1) / a.G;
+  const int head = kvh * a.G + min(r, rows - 1) - tok * a.G;
+  const bool tree = a.mask != nullptr;
+  const bool refused = tree && p.s.count > kMaxTreeTokens;
+  auto keys_of = [&](int last_row) {   // positions that rows up to last_row attend
+    if (refused) return 0;
+    return tree ? p.s.keys : max(0, min(p.s.keys, p.s.base + min(last_row, rows - 1) / a.G + 1));
+  };
+  const int keys = keys_of(p.tile * R + R - 1);
+  const int wave_keys = r0 < rows ? keys_of(r0 + 31) : 0;
+  const int ragged = tree ? p.s.base : p.s.base + min(r0, rows - 1) / a.G + 1;   // first key that not all its rows attend
+  const Sight hidden = row_sight(a, p.s, tok, keys);
+  // Chunks are cut in steps of kKeys; here a step is two of those.
+  const int blocks = (p.s.blocks + 1) >> 1;
+  const int per = blocks / p.chunks, extra = blocks % p.chunks;
+  const int c0 = p.chunk * per + min(p.chunk, extra);
+  const int c1 = min(c0 + per + (p.chunk < extra ? 1 : 0), (keys + kTileKeys - 1) / kTileKeys);
+
+  half8_t qf[8];
+  {
+    const half_t* qp = a.q + ((size_t)(p.s.start + tok) * a.H + head) * D + 8 * hh;
+#pragma unroll
+    for (int ks = 0; ks < 8; ++ks) qf[ks] = ld_h8(qp + 16 * ks);
+  }
+  float16_t acc[4];
+#pragma unroll
+  for (int dt = 0; dt < 4; ++dt)
+#pragma unroll
+    for (int e = 0; e < 16; ++e) acc[dt][e] = 0.f;
+  float m_run = -INFINITY, l_run = 0.f;
+
+  if (c0 < c1) {
+    const size_t head_off = (size_t)kvh * a.page_size * D;
+    // Block loads: K rows 16 u + tid / 16, 16-byte chunk tid % 16; V keys 4 (tid
+    // % 16) .., d chunk tid / 16 (the 16 lanes of a transposed write then cover
+    // one whole 128-byte row).
+    const half_t* kbase = a.kp + head_off + (size_t)(tid >> 4) * D + 8 * (tid & 15);
+    const half_t* vbase = a.vp + head_off + (size_t)(4 * (tid & 3)) * D + 8 * (tid >> 4);
+    const int vgroup = (tid & 15) >> 2;
+    const int last_group = (keys - 1) >> 4;
+    int g0 = 4 * c0;
+    Groups g = load_groups(a, p.b, g0, last_group, lane);
+    uint4_t kr[4], vr[4];
+    uint32_t bad_next = 0, bad = 0;   // of the block in registers, and in the stage being read: groups without a page
+    auto load_block = [&](int kb) {
+      if (4 * kb - g0 >= 64) {
+        g0 = 4 * kb;
+        g = load_groups(a, p.b, g0, last_group, lane);
+      }
+      const int l = 4 * kb - g0;
+      const half_t* vsrc = vbase;
+      int64_t voff = 0;
+#pragma unroll
+      for (int u = 0; u < 4; ++u) {
+        const int64_t page = __builtin_amdgcn_readlane(g.page, l + u), row = __builtin_amdgcn_readlane(g.row, l + u);
+        kr[u] = *reinterpret_cast<const uint4_t*>(kbase + page * a.k_stride + row * D);
+        const int64_t off = page * a.v_stride + row * D;
+        voff = vgroup == u ? off : voff;
+      }
+      vsrc += voff;
+#pragma unroll
+      for (int e = 0; e < 4; ++e) vr[e] = *reinterpret_cast<const uint4_t*>(vsrc + e * D);
+      bad_next = (uint32_t)(g.bad >> l) & 15;
+    };
+    auto store_block = [&](int st, int kb) {
+      if (kb * kTileKeys + kTileKeys > keys) {   // what lies behind the last key is not the sequence's
+#pragma unroll
+        for (int e = 0; e < 4; ++e)
+          if (kb * kTileKeys + 4 * (tid & 15) + e >= keys) vr[e] = uint4_t{0u, 0u, 0u, 0u};
+      }
+      uint8_t* base = smem + st * kTileStage;
+#pragma unroll
+      for (int u = 0; u < 4; ++u) {
+        const int row = 16 * u + (tid >> 4), c = tid & 15;
+        *reinterpret_cast<uint4_t*>(base + row * 256 + ((c ^ (row & 15)) << 4)) = kr[u];
+      }
+      // Keys 4 g .. 4 g + 3 (g = tid % 16) land in the slots pos .. pos + 3.
+      const int gq = tid & 15, kk = (4 * gq) & 15;
+      const int pos = 16 * (gq >> 2) + 8 * ((kk & 7) >> 2) + 4 * (kk >> 3);
+      const int d0 = 8 * (tid >> 4);
+#pragma unroll
+      for (int dd = 0; dd < 8; ++dd) {
+        const uint32_t sel = dd & 1 ? 0x07060302u : 0x05040100u;
+        uint2_t w;
+        w.x = __builtin_amdgcn_perm(vr[1][dd >> 1], vr[0][dd >> 1], sel);
+        w.y = __builtin_amdgcn_perm(vr[3][dd >> 1], vr[2][dd >> 1], sel);
+        *reinterpret_cast<uint2_t*>(base + vt_offset(d0 + dd, pos)) = w;
+      }
+    };
+    auto step = [&](const uint8_t* base, int k0, bool masked) {
+      float16_t sc[2];
+#pragma unroll
+      for (int kt = 0; kt < 2; ++kt) {
+#pragma unroll
+        for (int e = 0; e < 16; ++e) sc[kt][e] = 0.f;
+        const int row = 32 * kt + ql;
+#pragma unroll
+        for (int ks = 0; ks < 8; ++ks) {
+          const int c = 2 * ks + hh;
+          const half8_t ka = *reinterpret_cast<const half8_t*>(base + row * 256 + ((c ^ (row & 15)) << 4));
+          sc[kt] = __builtin_amdgcn_mfma_f32_32x32x16_f16(ka, qf[ks], sc[kt], 0, 0, 0);
+        }
+      }
+      if (bad) {
+#pragma unroll
+        for (int kt = 0; kt < 2; ++kt)
+#pragma unroll
+          for (int e = 0; e < 16; ++e)
+            if ((bad >> (2 * kt + (e >> 3))) & 1) sc[kt][e] = NAN;
+      }
+      if (masked) {
+#pragma unroll
+        for (int kt = 0; kt < 2; ++kt)
+#pragma unroll
+          for (int e = 0; e < 16; ++e) {
+            sc[kt][e] = hidden(k0 + 32 * kt + 8 * (e >> 2) + 4 * hh + (e & 3)) ? -INFINITY : sc[kt][e];
+          }
+      }
+      float mb = -INFINITY;
+#pragma unroll
+      for (int kt = 0; kt < 2; ++kt)
+#pragma unroll
+        for (int e = 0; e < 16; ++e) mb = fmaxf(mb, sc[kt][e]);
+      mb = fmaxf(mb, __shfl_xor(mb, 32));
+      const float m_new = fmaxf(m_run, mb * a.scale_log2);   // scale > 0
+      const float m_use = m_new == -INFINITY ? 0.f : m_new;
+      const float alpha = exp2_hw(m_run - m_use);
+      m_run = m_new;
+      half8_t pb[2][2];
+      float ls = 0.f;
+#pragma unroll
+      for (int kt = 0; kt < 2; ++kt)
+#pragma unroll
+        for (int st = 0; st < 2; ++st)
+#pragma unroll
+          for (int e = 0; e < 8; ++e) {
+            const float pv = exp2_hw(__builtin_fmaf(sc[kt][8 * st + e], a.scale_log2, -m_use));
+            ls += pv;
+            pb[kt][st][e] = (half_t)pv;
+          }
+      l_run = l_run * alpha + ls;
+      if (__builtin_amdgcn_ballot_w64(alpha != 1.f) != 0) {
+#pragma unroll
+        for (int dt = 0; dt < 4; ++dt)
+#pragma unroll
+          for (int e = 0; e < 16; ++e) acc[dt][e] *= alpha;
+      }
+#pragma unroll
+      for (int dt = 0; dt < 4; ++dt) {
+        const int d = 32 * dt + ql;
+#pragma unroll
+        for (int kt = 0; kt < 2; ++kt)
+#pragma unroll
+          for (int st = 0; st < 2; ++st) {
+            const int c = 2 * (2 * kt + st) + hh;
+            const half8_t va = *reinterpret_cast<const half8_t*>(base + kTileKBytes + d * (kTileKeys * 2) +
+                                                                 ((c ^ ((d >> 1) & 7)) << 4));
+            acc[dt] = __builtin_amdgcn_mfma_f32_32x32x16_f16(va, pb[kt][st], acc[dt], 0, 0, 0);
+          }
+      }
+    };
+
+    load_block(c0);
+    // The rows' q land here too: left in flight they would be waited for in every turn of the loop.
+#pragma unroll
+    for (int ks = 0; ks < 8; ++ks) asm volatile("" : "+v"(qf[ks]));
+    __builtin_amdgcn_s_waitcnt(0);
+    store_block(0, c0);
+    bad = bad_next;
+    __syncthreads();
+    for (int kb = c0; kb < c1; ++kb) {
+      const int st = (kb - c0) & 1;
+      const bool more = kb + 1 < c1;
+      if (more) load_block(kb + 1);
+      const int k0 = kb * kTileKeys;
+      if (k0 < wave_keys) step(smem + st * kTileStage, k0, k0 + kTileKeys > ragged || k0 + kTileKeys > keys);
+      if (more) store_block(st ^ 1, kb + 1);   // that stage was last read before the previous barrier
+      bad = bad_next;
+      __syncthreads();
+    }
+    l_run += __shfl_xor(l_run, 32);
+  }
+
+  // Lane (ql, hh) holds d = 32 dt + 8 (e / 4) + 4 hh + e % 4 of row ql.
+  if (r >= rows) return;
+  if (p.chunks > 1) {
+    const size_t at = ((size_t)slot * a.KV + kvh) * R + 32 * wave + ql;
+    float* o = a.part_o + at * D + 4 * hh;
+#pragma unroll
+    for (int dt = 0; dt < 4; ++dt)
+#pragma unroll
+      for (int j = 0; j < 4; ++j)
+        *reinterpret_cast<float4_t*>(o + 32 * dt + 8 * j) =
+            float4_t{acc[dt][4 * j], acc[dt][4 * j + 1], acc[dt][4 * j + 2], acc[dt][4 * j + 3]};
+    if (hh == 0) a.part_ml[at] = float2_t{m_run, l_run};
+    return;
+  }
+  const float inv = 1.0f / l_run;
+  half_t* o = a.out + ((size_t)(p.s.start + tok) * a.H + head) * D + 4 * hh;
+#pragma unroll
+  for (int dt = 0; dt < 4; ++dt)
+#pragma unroll
+    for (int j = 0; j < 4; ++j) {
+      half4_t h;
+#pragma unroll
+      for (int e = 0; e < 4; ++e)
+        h[e] = refused ? (half_t)NAN : l_run == 0.f ? (half_t)0.f : (half_t)(acc[dt][4 * j + e] * inv);
+      *reinterpret_cast<half4_t*>(o + 32 * dt + 8 * j) = h;
+    }
+}
+
+// The chunks of split tiles joined: grid = (tiles the call can have * KV,
+// parts of R rows), a wave per row and turn, two elements of d per lane.  The
+// weights 2^(m_c - M) of up to 64 chunks are held one per lane and read out as
+// each chunk is added, in chunk order.
 template <int R>
 __global__ __launch_bounds__(256) void paged_attention_merge_kernel(PagedArgs a) {
   constexpr int D = kPagedDim;
@@ -367,71 +633,67 @@ __global__ __launch_bounds__(256) void paged_attention_merge_kernel(PagedArgs a)
   const int kvh = blockIdx.x % a.KV;
   const Place p = find_place<R, true>(a, blockIdx.x / a.KV, lane);
   if (!p.found || p.chunks == 1 || p.slot0 + (int64_t)p.s.tiles * p.chunks > a.slots) return;
-  const int row = 4 * blockIdx.y + wave;
-  const int rr = p.tile * R + row;
-  if (rr >= p.s.count * a.G) return;
-  auto at = [&](int chunk) {
-    return ((size_t)(p.slot0 + chunk * p.s.tiles + p.tile) * a.KV + kvh) * R + row;
-  };
-  float M = -INFINITY;
-  for (int c0 = 0; c0 < p.chunks; c0 += 64)
-    if (c0 + lane < p.chunks) M = fmaxf(M, a.part_ml[at(c0 + lane)].x);
-  M = wave_max_rl(M);
-  const float Mu = M == -INFINITY ? 0.f : M;
-  float den = 0.f;
-  float2_t num = {0.f, 0.f};
-  for (int c0 = 0; c0 < p.chunks; c0 += 64) {
-    const int n = min(64, p.chunks - c0);
-    const float2_t ml = lane < n ? a.part_ml[at(c0 + lane)] : float2_t{-INFINITY, 0.f};
-    const float w = exp2_hw(ml.x - Mu);
-    den += wave_sum_rl(w * ml.y);
-    for (int c = 0; c < n; c += 8) {
-      float2_t o[8];
+  const int end = min(R, p.s.count * a.G - p.tile * R);
+  const bool refused = a.mask != nullptr && p.s.count > kMaxTreeTokens;
+  for (int row = 4 * blockIdx.y + wave; row < end; row += 4 * gridDim.y) {
+    auto at = [&](int chunk) { return ((size_t)slot_of(p, p.tile, chunk) * a.KV + kvh) * R + row; };
+    float M = -INFINITY;
+    for (int c0 = 0; c0 < p.chunks; c0 += 64)
+      if (c0 + lane < p.chunks) M = fmaxf(M, a.part_ml[at(c0 + lane)].x);
+    M = wave_max_rl(M);
+    const float Mu = M == -INFINITY ? 0.f : M;
+    float den = 0.f;
+    float2_t num = {0.f, 0.f};
+    for (int c0 = 0; c0 < p.chunks; c0 += 64) {
+      const int n = min(64, p.chunks - c0);
+      const float2_t ml = lane < n ? a.part_ml[at(c0 + lane)] : float2_t{-INFINITY, 0.f};
+      const float w = exp2_hw(ml.x - Mu);
+      den += wave_sum_rl(w * ml.y);
+      for (int c = 0; c < n; c += 8) {
+        float2_t o[8];
 #pragma unroll
-      for (int u = 0; u < 8; ++u)
-        o[u] = *reinterpret_cast<const float2_t*>(a.part_o + at(c0 + min(c + u, n - 1)) * D + 2 * lane);
+        for (int u = 0; u < 8; ++u)
+          o[u] = *reinterpret_cast<const float2_t*>(a.part_o + at(c0 + min(c + u, n - 1)) * D + 2 * lane);
 #pragma unroll
-      for (int u = 0; u < 8; ++u) {
-        const float wc = c + u < n ? lane_f(w, min(c + u, 63)) : 0.f;
-        if (c + u < n) num += wc * o[u];
+        for (int u = 0; u < 8; ++u)
+          if (c + u < n) num += lane_f(w, min(c + u, 63)) * o[u];
       }
     }
-  }
-  const bool refused = a.mask != nullptr && p.s.count > kMaxTreeTokens;
-  const int t = rr / a.G;
-  half2_t h;
+    const int rr = p.tile * R + row, t = rr / a.G;
+    half2_t h;
 #pragma unroll
-  for (int e = 0; e < 2; ++e) {
-    const float n = num[e];
-    h[e] = refused ? (half_t)NAN : den == 0.f ? (half_t)0.f : (half_t)(n / den);
+    for (int e = 0; e < 2; ++e) {
+      const float n = num[e];
+      h[e] = refused ? (half_t)NAN : den == 0.f ? (half_t)0.f : (half_t)(n / den);
+    }
+    half_t* dst = a.out + ((size_t)(p.s.start + t) * a.H + kvh * a.G + rr - t * a.G) * D + 2 * lane;
+    *reinterpret_cast<half2_t*>(dst) = h;
   }
-  half_t* dst = a.out + ((size_t)(p.s.start + t) * a.H + kvh * a.G + rr - t * a.G) * D + 2 * lane;
-  *reinterpret_cast<half2_t*>(dst) = h;
 }
 
-// Places of the grid per kv head: the tiles the call can have at most, and as
-// many more for chunks as bring the workgroups to about four per compute unit.
+// Which kernel a call takes, and its places of the grid per kv head: the tiles
+// the call can have at most, and as many more for chunks as bring the
+// workgroups to about four (small tiles) or two (large ones) per compute unit.
 struct PagedPlan {
+  int rows;                 // of a tile
   int64_t tiles, spare, slots;
   int min_blocks;
   size_t bytes;
 };
 
-constexpr int kTargetGroups = 1024;
-constexpr int kMinBlocks = 4;
-
 PagedPlan paged_plan(int64_t tokens, int64_t sequences, int64_t G, int64_t KV, int64_t width, int64_t page_size) {
-  constexpr int R = 16;
   PagedPlan p{};
+  p.rows = tokens * G > 32 * sequences ? kTileRows : 16;
   // sum_b ceil(count_b G / R) <= ceil(tokens G / R) + sequences, and no more tiles than rows.
-  p.tiles = (tokens * G + R - 1) / R + sequences;
-  if (p.tiles > tokens * ((G + R - 1) / R)) p.tiles = tokens * ((G + R - 1) / R);
-  p.min_blocks = kMinBlocks;
+  p.tiles = (tokens * G + p.rows - 1) / p.rows + sequences;
+  const int64_t most = tokens * ((G + p.rows - 1) / p.rows);
+  if (p.tiles > most) p.tiles = most;
+  const int64_t target = p.rows == 16 ? 1024 : 512;
+  p.min_blocks = p.rows == 16 ? 4 : 8;
   const int64_t blocks = width * page_size / kKeys + 1;
-  const int64_t spare = (kTargetGroups + KV - 1) / KV;
-  p.spare = blocks > kMinBlocks && p.tiles * KV < 4 * kTargetGroups ? spare : 0;
+  p.spare = blocks > p.min_blocks && p.tiles * KV < 4 * target ? (target + KV - 1) / KV : 0;
   p.slots = p.tiles + p.spare;
-  p.bytes = p.spare ? (size_t)p.slots * KV * R * (kPagedDim + 2) * 4 : 0;
+  p.bytes = p.spare ? (size_t)p.slots * KV * p.rows * (kPagedDim + 2) * 4 : 0;
   return p;
 }
 
@@ -501,7 +763,7 @@ extern "C" int wq_paged_attention(const uint16_t* q, int64_t tokens, int64_t q_h
   a.mask = tree_mask;
   a.out = reinterpret_cast<half_t*>(out);
   a.part_o = reinterpret_cast<float*>(workspace);
-  a.part_ml = reinterpret_cast<float2_t*>(a.part_o + (size_t)plan.slots * kv_heads * 16 * kPagedDim);
+  a.part_ml = reinterpret_cast<float2_t*>(a.part_o + (size_t)plan.slots * kv_heads * plan.rows * kPagedDim);
   a.k_stride = key_page_stride;
   a.v_stride = value_page_stride;
   a.scale_log2 = scale * kLog2e;
@@ -516,11 +778,17 @@ extern "C" int wq_paged_attention(const uint16_t* q, int64_t tokens, int64_t q_h
   a.slots = (int)plan.slots;
   a.spare = (int)plan.spare;
   a.min_blocks = plan.min_blocks;
-  hipLaunchKernelGGL(paged_attention_rows_kernel, dim3((unsigned)(plan.slots * kv_heads)), dim3(256), 0,
-                     as_stream(stream), a);
+  const dim3 grid((unsigned)(plan.slots * kv_heads));
+  if (plan.rows == 16)
+    hipLaunchKernelGGL(paged_attention_rows_kernel, grid, dim3(256), 0, as_stream(stream), a);
+  else
+    hipLaunchKernelGGL(paged_attention_tile_kernel, grid, dim3(256), 2 * kTileStage, as_stream(stream), a);
   rc = check_launch("paged_attention");
   if (rc != WQ_OK || plan.spare == 0) return rc;
-  hipLaunchKernelGGL(paged_attention_merge_kernel<16>, dim3((unsigned)(plan.tiles * kv_heads), 4), dim3(256), 0,
-                     as_stream(stream), a);
+  const dim3 merge((unsigned)(plan.tiles * kv_heads), 4);
+  if (plan.rows == 16)
+    hipLaunchKernelGGL(paged_attention_merge_kernel<16>, merge, dim3(256), 0, as_stream(stream), a);
+  else
+    hipLaunchKernelGGL(paged_attention_merge_kernel<kTileRows>, merge, dim3(256), 0, as_stream(stream), a);
   return check_launch("paged_attention_merge");
 }

@@ -149,10 +149,10 @@ struct Scale {
 // Bins of octaves below the base: eight of one octave, seven of four, and all
 // that lies 36 or more below (of 2^18 tokens less than 2^-15 of the weight:
 // only top-k goes there).
-__device__ __forceinline__ int bin_of(double below) {
-  const int d = (int)fmin(below, 64.0);
-  return d < 8 ? d : min(8 + ((d - 8) >> 2), kBins - 1);
+__device__ __forceinline__ int bin_at(int depth) {
+  return depth < 8 ? max(depth, 0) : min(8 + ((depth - 8) >> 2), kBins - 1);
 }
+__device__ __forceinline__ int bin_of(double below) { return bin_at((int)fmin(below, 64.0)); }
 __device__ __forceinline__ int bin_depth(int bin) { return bin < 8 ? bin : 8 + 4 * (bin - 8); }   // its first octave
 
 // 2^z: z = n / 32 + r with |r| <= 1 / 64, 2^(n/32) from a table of 32 and an
@@ -196,9 +196,15 @@ __device__ __forceinline__ void wave_peak(float& best, int& at) {
   }
 }
 
-// grid = (parts, rows), 256 threads.  Every thread keeps its own column of the
-// bins in LDS, so the additions need no atomics, meet no bank conflicts
-// between lanes and happen in a fixed order.
+// An addition in LDS that returns nothing, so that no thread waits for it.
+template <typename V>
+__device__ __forceinline__ void add_lds(V* at, V v) {
+  __hip_atomic_fetch_add(at, v, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_WORKGROUP);
+}
+
+// grid = (parts, rows), 256 threads.  Every thread adds to its own column of
+// the bins in LDS: no two lanes meet in a bank for longer than the access
+// takes, and the additions happen in a fixed order.
 template <typename T>
 __global__ __launch_bounds__(kTallyThreads) void sample_tally_kernel(SampleArgs a) {
   constexpr int E = Row<T>::E;
@@ -250,11 +256,12 @@ __global__ __launch_bounds__(kTallyThreads) void sample_tally_kernel(SampleArgs 
     const uint32_t in = r.load(c, v);
 #pragma unroll
     for (int e = 0; e < E; ++e) {
-      if (!((in >> e) & 1)) continue;
       const double y = s.y(v[e]);
       const int b = bin_of(s.below(y));
-      mass[b][tid] += exp2_64(y - s.base, table);
-      ++count[b][tid];
+      if ((in >> e) & 1) {
+        add_lds(&mass[b][tid], exp2_64(y - s.base, table));
+        add_lds(&count[b][tid], 1u);
+      }
     }
   }
   __syncthreads();
@@ -325,11 +332,13 @@ __device__ __forceinline__ void read_tally(const SampleArgs& a, const Scale& s, 
     const int p = e / kBins, b = e % kBins;
     double m = 0.0;
     uint32_t n = 0;
-    for (int i = 0; i <= b; ++i)
-      if ((i == kBins - 1 ? i : bin_of((double)(bin_depth(i) + t.shift[p]))) == b) {
-        m += t.raw_mass[p][i];
-        n += t.raw_count[p][i];
-      }
+    // The part's bins that start within the row's bin b.
+    const int down = t.shift[p];
+    const int i1 = b == kBins - 1 ? b : bin_at(bin_depth(b + 1) - down) - 1;
+    for (int i = bin_at(bin_depth(b) - down); i <= i1; ++i) {
+      m += t.raw_mass[p][i];
+      n += t.raw_count[p][i];
+    }
     t.part_mass[p][b] = m * t.scale[p];
     t.part_count[p][b] = n;
   }
@@ -365,46 +374,70 @@ struct Range {
   double before;       // mass in front of bin by_k
   double whole;        // mass of all bins
   double min_y;        // the smallest y that min-p leaves
+  uint32_t listed;     // tokens of the list; more than it can hold: the pick goes over the row instead
 };
 
-__device__ __forceinline__ int mass_bin(const RowTally& t, int last, double goal, double& before) {
-  int b = 0;
-  before = 0.0;
-  for (; b < last && before + t.mass[b] < goal; ++b) before += t.mass[b];
-  return b;
-}
+// The row's bins one per lane (lanes 16 .. repeat them), with the sums in
+// front of each: the search for a bin costs a few lane moves instead of a
+// chain of LDS reads.
+struct LaneBins {
+  double mass, before;
+  uint32_t count, count_before;
 
-__device__ __forceinline__ Range find_range(const SampleArgs& a, const Ask& q, const Scale& s, const RowTally& t) {
-  Range g{kBins, kBins, kBins, 0, -1, 0, 0.0, 0.0, -INFINITY};
-  for (int b = 0; b < kBins; ++b) g.whole += t.mass[b];
+  __device__ __forceinline__ LaneBins(const RowTally& t, int lane) {
+    const int b = lane & (kBins - 1);
+    mass = t.mass[b];
+    count = t.count[b];
+    double m = mass;
+    uint32_t n = count;
+#pragma unroll
+    for (int o = 1; o < kBins; o <<= 1) {
+      const double um = __shfl_up(m, o, kBins);
+      const uint32_t un = __shfl_up(n, o, kBins);
+      if (b >= o) {
+        m += um;
+        n += un;
+      }
+    }
+    before = m - mass;
+    count_before = n - count;
+  }
+  __device__ __forceinline__ double whole() const { return __shfl(before + mass, kBins - 1); }
+  // The first bin up to `last` at which the mass reaches `goal`, and the mass in front of it.
+  __device__ __forceinline__ int reach(double goal, int last, int lane, double& in_front) const {
+    const uint64_t hit = __builtin_amdgcn_ballot_w64(lane < kBins && (lane >= last || before + mass >= goal));
+    const int b = __builtin_ctzll(hit);
+    in_front = __shfl(before, b);
+    return b;
+  }
+};
+
+__device__ __forceinline__ Range find_range(const SampleArgs& a, const Ask& q, const Scale& s, const LaneBins& bins,
+                                            int lane) {
+  Range g{kBins, kBins, kBins, 0, -1, 0, 0.0, bins.whole(), -INFINITY};
   if (q.min_p > -INFINITY) {
     g.min_y = s.y(s.top) + q.min_p;
     g.floor = bin_of(s.below(g.min_y));
   }
   if (q.top_k < a.vocab) {
-    g.want = (uint32_t)q.top_k;
-    for (g.by_k = 0; g.by_k < kBins - 1 && t.count[g.by_k] < g.want; ++g.by_k) {
-      g.want -= t.count[g.by_k];
-      g.before += t.mass[g.by_k];
-    }
+    const uint64_t hit = __builtin_amdgcn_ballot_w64(
+        lane < kBins && (lane == kBins - 1 || bins.count_before + bins.count >= (uint32_t)q.top_k));
+    g.by_k = __builtin_ctzll(hit);
+    g.want = (uint32_t)q.top_k - __shfl(bins.count_before, g.by_k);
+    g.before = __shfl(bins.before, g.by_k);
     g.lo = 0;
     g.hi = g.by_k;
   } else if (q.top_p < 1.0) {
     double before;
-    g.by_p = mass_bin(t, kBins - 1, q.top_p * g.whole, before);
+    g.by_p = bins.reach(q.top_p * g.whole, kBins - 1, lane, before);
     g.lo = min(g.by_p, g.floor);
     g.hi = g.by_p;
   } else if (g.floor < kBins) {
     g.lo = g.hi = g.floor;
   }
+  const uint32_t upto = bins.count_before + bins.count;
+  g.listed = g.hi < g.lo ? 0 : __shfl(upto, g.hi) - __shfl(bins.count_before, g.lo);
   return g;
-}
-
-// Tokens of the list; more than it can hold: the pick goes over the row instead.
-__device__ __forceinline__ uint32_t list_length(const RowTally& t, const Range& g) {
-  uint32_t n = 0;
-  for (int b = g.lo; b <= g.hi; ++b) n += t.count[b];
-  return n;
 }
 
 // grid = (parts, rows), 256 threads: the part's tokens of the bins lo .. hi
@@ -421,8 +454,8 @@ __global__ __launch_bounds__(256) void sample_gather_kernel(SampleArgs a) {
   if (q.none || q.greedy || !(top > -INFINITY)) return;
   const Scale s(q.to_octaves, top);
   read_tally<256>(a, s, row, tid, tally);
-  const Range g = find_range(a, q, s, tally);
-  if (g.hi < g.lo || list_length(tally, g) > (uint32_t)a.list_cap) return;
+  const Range g = find_range(a, q, s, LaneBins(tally, lane), lane);
+  if (g.hi < g.lo || g.listed > (uint32_t)a.list_cap) return;
   if (tid < 64) {   // the part's place: the tokens of the parts in front of it
     uint32_t n = 0;
     if (lane < a.parts)
@@ -760,10 +793,10 @@ __global__ __launch_bounds__(kPickThreads) void sample_pick_kernel(SampleArgs a)
   const Scale s(q.to_octaves, top);
   fill_exp2(sh.table, tid);
   read_tally<kPickThreads>(a, s, row, tid, sh.tally);
-  const Range g = find_range(a, q, s, sh.tally);
-  const uint32_t listed = list_length(sh.tally, g);
-  Picker<T> pick{a, r, s, sh, listed <= (uint32_t)a.list_cap ? a.list + (size_t)row * a.list_cap : nullptr,
-                 (int)listed, tid};
+  const LaneBins bins(sh.tally, lane);
+  const Range g = find_range(a, q, s, bins, lane);
+  Picker<T> pick{a, r, s, sh, g.listed <= (uint32_t)a.list_cap ? a.list + (size_t)row * a.list_cap : nullptr,
+                 (int)g.listed, tid};
 
   // Where top-k ends, then top-p of what it leaves.
   Cut cut{kBins, 0, 0, 0.0};
@@ -774,7 +807,7 @@ __global__ __launch_bounds__(kPickThreads) void sample_pick_kernel(SampleArgs a)
     const double goal = q.top_p * whole;
     double before = g.before;
     int bin = g.by_k;
-    if (by_mass) bin = mass_bin(sh.tally, min(cut.bin, kBins - 1), goal, before);
+    if (by_mass) bin = bins.reach(goal, min(cut.bin, kBins - 1), lane, before);
     const Cut end = pick.find_cut(bin, by_mass, g.want, before, goal);
     if (!by_mass) whole = before + end.kept;
     // Both may end at one value: the fewer ties.  Otherwise top-p's is the higher one, but for roundings.

@@ -386,12 +386,24 @@ __global__ __launch_bounds__(256, 2) void paged_attention_rows_kernel(PagedArgs 
 // of row ql, and the probabilities, rounded to fp16, are the B operand of O^T
 // = V^T . P^T once V^T's key slots follow the same order: slot 8 h + 4 j + e
 // of a 16-key step holds key 8 j + 4 h + e.
+constexpr float kLag = 8.f;
 constexpr int kTileRows = 128;
 constexpr int kTileKeys = 64;
 constexpr int kTileKBytes = kTileKeys * kPagedDim * 2;
 constexpr int kTileStage = 2 * kTileKBytes;   // K block, then V^T block
 
 typedef float float16_t __attribute__((ext_vector_type(16)));
+
+// Masks of __builtin_amdgcn_sched_group_barrier.
+constexpr int kSchedMfma = 0x8, kSchedLdsRead = 0x100;
+
+// The larger of lane l and lane l ^ 32.
+__device__ __forceinline__ float max_halves(float v) {
+  const uint32_t u = __builtin_bit_cast(uint32_t, v);
+  const auto r = __builtin_amdgcn_permlane32_swap(u, u, false, false);   // (low half twice, high half twice)
+  const uint32_t lo = r[0], hi = r[1];
+  return fmaxf(__builtin_bit_cast(float, lo), __builtin_bit_cast(float, hi));
+}
 
 __device__ __forceinline__ int vt_offset(int d, int pos) {
   return kTileKBytes + d * (kTileKeys * 2) + ((((pos >> 3) ^ ((d >> 1) & 7))) << 4) + (pos & 7) * 2;
@@ -513,6 +525,14 @@ __global__ __launch_bounds__(256, 2) void paged_attention_tile_kernel(PagedArgs 
           sc[kt] = __builtin_amdgcn_mfma_f32_32x32x16_f16(ka, qf[ks], sc[kt], 0, 0, 0);
         }
       }
+      // Six fragments ahead of the matrix cores.
+      __builtin_amdgcn_sched_group_barrier(kSchedLdsRead, 6, 0);
+#pragma unroll
+      for (int u = 0; u < 10; ++u) {
+        __builtin_amdgcn_sched_group_barrier(kSchedMfma, 1, 0);
+        __builtin_amdgcn_sched_group_barrier(kSchedLdsRead, 1, 0);
+      }
+      __builtin_amdgcn_sched_group_barrier(kSchedMfma, 6, 0);
       if (bad) {
 #pragma unroll
         for (int kt = 0; kt < 2; ++kt)
@@ -528,48 +548,64 @@ __global__ __launch_bounds__(256, 2) void paged_attention_tile_kernel(PagedArgs 
             sc[kt][e] = hidden(k0 + 32 * kt + 8 * (e >> 2) + 4 * hh + (e & 3)) ? -INFINITY : sc[kt][e];
           }
       }
-      float mb = -INFINITY;
+      float m2[2] = {-INFINITY, -INFINITY};
 #pragma unroll
-      for (int kt = 0; kt < 2; ++kt)
+      for (int e = 0; e < 16; ++e)
 #pragma unroll
-        for (int e = 0; e < 16; ++e) mb = fmaxf(mb, sc[kt][e]);
-      mb = fmaxf(mb, __shfl_xor(mb, 32));
+        for (int kt = 0; kt < 2; ++kt) m2[kt] = fmaxf(m2[kt], sc[kt][e]);
+      const float mb = max_halves(fmaxf(m2[0], m2[1]));
+      // The reference of the exponents follows the largest score only once that
+      // is kLag octaves ahead in some row (of 32 rows nearly every block would
+      // move one): the probabilities, at most 2^kLag, are as exact in fp16 and
+      // the sums in fp32 have room.
       const float m_new = fmaxf(m_run, mb * a.scale_log2);   // scale > 0
-      const float m_use = m_new == -INFINITY ? 0.f : m_new;
-      const float alpha = exp2_hw(m_run - m_use);
-      m_run = m_new;
-      half8_t pb[2][2];
-      float ls = 0.f;
-#pragma unroll
-      for (int kt = 0; kt < 2; ++kt)
-#pragma unroll
-        for (int st = 0; st < 2; ++st)
-#pragma unroll
-          for (int e = 0; e < 8; ++e) {
-            const float pv = exp2_hw(__builtin_fmaf(sc[kt][8 * st + e], a.scale_log2, -m_use));
-            ls += pv;
-            pb[kt][st][e] = (half_t)pv;
-          }
-      l_run = l_run * alpha + ls;
-      if (__builtin_amdgcn_ballot_w64(alpha != 1.f) != 0) {
+      if (__builtin_amdgcn_ballot_w64(m_new > m_run + kLag) != 0) {
+        const float alpha = exp2_hw(m_run - (m_new == -INFINITY ? 0.f : m_new));
+        m_run = m_new;
+        l_run *= alpha;
 #pragma unroll
         for (int dt = 0; dt < 4; ++dt)
 #pragma unroll
           for (int e = 0; e < 16; ++e) acc[dt][e] *= alpha;
       }
-#pragma unroll
-      for (int dt = 0; dt < 4; ++dt) {
+      const float m_use = m_run == -INFINITY ? 0.f : m_run;
+      // Sixteen keys at a time, and beside each product with the values two of the next sixteen's probabilities per
+      // lane and the fragment of the next sixteen's values; the scheduler, left alone, puts every read right in front
+      // of its product and waits for it.
+      auto values = [&](int s4, int dt) {
         const int d = 32 * dt + ql;
+        return *reinterpret_cast<const half8_t*>(base + kTileKBytes + d * (kTileKeys * 2) +
+                                                 (((2 * s4 + hh) ^ ((d >> 1) & 7)) << 4));
+      };
+      float ls = 0.f;
+      auto probability = [&](int s4, int e) {
+        const float pv = exp2_hw(__builtin_fmaf(sc[s4 >> 1][8 * (s4 & 1) + e], a.scale_log2, -m_use));
+        ls += pv;
+        return (half_t)pv;
+      };
+      half8_t va[4], pb;
 #pragma unroll
-        for (int kt = 0; kt < 2; ++kt)
+      for (int dt = 0; dt < 4; ++dt) va[dt] = values(0, dt);
 #pragma unroll
-          for (int st = 0; st < 2; ++st) {
-            const int c = 2 * (2 * kt + st) + hh;
-            const half8_t va = *reinterpret_cast<const half8_t*>(base + kTileKBytes + d * (kTileKeys * 2) +
-                                                                 ((c ^ ((d >> 1) & 7)) << 4));
-            acc[dt] = __builtin_amdgcn_mfma_f32_32x32x16_f16(va, pb[kt][st], acc[dt], 0, 0, 0);
+      for (int e = 0; e < 8; ++e) pb[e] = probability(0, e);
+      __builtin_amdgcn_sched_barrier(0);
+#pragma unroll
+      for (int s4 = 0; s4 < 4; ++s4) {
+        half8_t next = pb;
+#pragma unroll
+        for (int dt = 0; dt < 4; ++dt) {
+          const half8_t v = va[dt];
+          if (s4 < 3) va[dt] = values(s4 + 1, dt);
+          acc[dt] = __builtin_amdgcn_mfma_f32_32x32x16_f16(v, pb, acc[dt], 0, 0, 0);
+          if (s4 < 3) {
+            next[2 * dt] = probability(s4 + 1, 2 * dt);
+            next[2 * dt + 1] = probability(s4 + 1, 2 * dt + 1);
           }
+          __builtin_amdgcn_sched_barrier(0);
+        }
+        pb = next;
       }
+      l_run += ls;
     };
 
     load_block(c0);

@@ -378,9 +378,9 @@ __global__ __launch_bounds__(256, 2) void paged_attention_rows_kernel(PagedArgs 
 // Chunks of prompts and trees of many tokens: tiles of 128 rows, grid and
 // places as above.  Wave w owns the rows 32 w .. 32 w + 31 of the tile; all
 // four share the keys and values, 64 at a time through two stages of LDS:
-//   K [key][d], 16-byte chunk c of row r at slot c ^ (r & 15);
-//   V^T [d][key slot], chunk c of row d at slot c ^ ((d >> 1) & 7), so that the
-//   lanes of a fragment read hit distinct banks.
+//   K [key][d] in rows of 272 bytes and V^T [d][key slot] in rows of 144: the 16
+//   lanes that a 16-byte read serves at once are 4 (of 64) banks apart, and every
+//   fragment is one address and a constant.
 // Scores are computed transposed on 32x32x16 (A = 32 keys, B = 32 rows): lane
 // (l % 32, l / 32) = (ql, hh) holds in register r key 8 (r / 4) + 4 hh + r % 4
 // of row ql, and the probabilities, rounded to fp16, are the B operand of O^T
@@ -389,8 +389,9 @@ __global__ __launch_bounds__(256, 2) void paged_attention_rows_kernel(PagedArgs 
 constexpr float kLag = 8.f;
 constexpr int kTileRows = 128;
 constexpr int kTileKeys = 64;
-constexpr int kTileKBytes = kTileKeys * kPagedDim * 2;
-constexpr int kTileStage = 2 * kTileKBytes;   // K block, then V^T block
+constexpr int kKRow = kPagedDim * 2 + 16, kVRow = kTileKeys * 2 + 16;   // bytes
+constexpr int kTileKBytes = kTileKeys * kKRow;
+constexpr int kTileStage = kTileKBytes + kPagedDim * kVRow;   // K block, then V^T block
 
 typedef float float16_t __attribute__((ext_vector_type(16)));
 
@@ -403,10 +404,6 @@ __device__ __forceinline__ float max_halves(float v) {
   const auto r = __builtin_amdgcn_permlane32_swap(u, u, false, false);   // (low half twice, high half twice)
   const uint32_t lo = r[0], hi = r[1];
   return fmaxf(__builtin_bit_cast(float, lo), __builtin_bit_cast(float, hi));
-}
-
-__device__ __forceinline__ int vt_offset(int d, int pos) {
-  return kTileKBytes + d * (kTileKeys * 2) + ((((pos >> 3) ^ ((d >> 1) & 7))) << 4) + (pos & 7) * 2;
 }
 
 __global__ __launch_bounds__(256, 2) void paged_attention_tile_kernel(PagedArgs a) {
@@ -496,7 +493,7 @@ __global__ __launch_bounds__(256, 2) void paged_attention_tile_kernel(PagedArgs 
 #pragma unroll
       for (int u = 0; u < 4; ++u) {
         const int row = 16 * u + (tid >> 4), c = tid & 15;
-        *reinterpret_cast<uint4_t*>(base + row * 256 + ((c ^ (row & 15)) << 4)) = kr[u];
+        *reinterpret_cast<uint4_t*>(base + row * kKRow + 16 * c) = kr[u];
       }
       // Keys 4 g .. 4 g + 3 (g = tid % 16) land in the slots pos .. pos + 3.
       const int gq = tid & 15, kk = (4 * gq) & 15;
@@ -508,7 +505,7 @@ __global__ __launch_bounds__(256, 2) void paged_attention_tile_kernel(PagedArgs 
         uint2_t w;
         w.x = __builtin_amdgcn_perm(vr[1][dd >> 1], vr[0][dd >> 1], sel);
         w.y = __builtin_amdgcn_perm(vr[3][dd >> 1], vr[2][dd >> 1], sel);
-        *reinterpret_cast<uint2_t*>(base + vt_offset(d0 + dd, pos)) = w;
+        *reinterpret_cast<uint2_t*>(base + kTileKBytes + (d0 + dd) * kVRow + 2 * pos) = w;
       }
     };
     auto step = [&](const uint8_t* base, int k0, bool masked) {
@@ -520,8 +517,7 @@ __global__ __launch_bounds__(256, 2) void paged_attention_tile_kernel(PagedArgs 
         const int row = 32 * kt + ql;
 #pragma unroll
         for (int ks = 0; ks < 8; ++ks) {
-          const int c = 2 * ks + hh;
-          const half8_t ka = *reinterpret_cast<const half8_t*>(base + row * 256 + ((c ^ (row & 15)) << 4));
+          const half8_t ka = *reinterpret_cast<const half8_t*>(base + row * kKRow + 16 * hh + 32 * ks);
           sc[kt] = __builtin_amdgcn_mfma_f32_32x32x16_f16(ka, qf[ks], sc[kt], 0, 0, 0);
         }
       }
@@ -573,21 +569,23 @@ __global__ __launch_bounds__(256, 2) void paged_attention_tile_kernel(PagedArgs 
       // lane and the fragment of the next sixteen's values; the scheduler, left alone, puts every read right in front
       // of its product and waits for it.
       auto values = [&](int s4, int dt) {
-        const int d = 32 * dt + ql;
-        return *reinterpret_cast<const half8_t*>(base + kTileKBytes + d * (kTileKeys * 2) +
-                                                 (((2 * s4 + hh) ^ ((d >> 1) & 7)) << 4));
+        return *reinterpret_cast<const half8_t*>(base + kTileKBytes + (32 * dt + ql) * kVRow + 16 * hh + 32 * s4);
       };
-      float ls = 0.f;
-      auto probability = [&](int s4, int e) {
-        const float pv = exp2_hw(__builtin_fmaf(sc[s4 >> 1][8 * (s4 & 1) + e], a.scale_log2, -m_use));
-        ls += pv;
-        return (half_t)pv;
+      // Two at a time.  Their sum is of the probabilities as rounded: the weights of the values then add up to one.
+      auto probabilities = [&](int s4, int e, half8_t& to) {
+        half2_t p2;
+#pragma unroll
+        for (int u = 0; u < 2; ++u)
+          p2[u] = (half_t)exp2_hw(__builtin_fmaf(sc[s4 >> 1][8 * (s4 & 1) + e + u], a.scale_log2, -m_use));
+        to[e] = p2[0];
+        to[e + 1] = p2[1];
+        l_run = __builtin_amdgcn_fdot2(p2, half2_t{(half_t)1.f, (half_t)1.f}, l_run, false);
       };
       half8_t va[4], pb;
 #pragma unroll
       for (int dt = 0; dt < 4; ++dt) va[dt] = values(0, dt);
 #pragma unroll
-      for (int e = 0; e < 8; ++e) pb[e] = probability(0, e);
+      for (int e = 0; e < 8; e += 2) probabilities(0, e, pb);
       __builtin_amdgcn_sched_barrier(0);
 #pragma unroll
       for (int s4 = 0; s4 < 4; ++s4) {
@@ -597,15 +595,11 @@ __global__ __launch_bounds__(256, 2) void paged_attention_tile_kernel(PagedArgs 
           const half8_t v = va[dt];
           if (s4 < 3) va[dt] = values(s4 + 1, dt);
           acc[dt] = __builtin_amdgcn_mfma_f32_32x32x16_f16(v, pb, acc[dt], 0, 0, 0);
-          if (s4 < 3) {
-            next[2 * dt] = probability(s4 + 1, 2 * dt);
-            next[2 * dt + 1] = probability(s4 + 1, 2 * dt + 1);
-          }
+          if (s4 < 3) probabilities(s4 + 1, 2 * dt, next);
           __builtin_amdgcn_sched_barrier(0);
         }
         pb = next;
       }
-      l_run += ls;
     };
 
     load_block(c0);
@@ -724,10 +718,10 @@ PagedPlan paged_plan(int64_t tokens, int64_t sequences, int64_t G, int64_t KV, i
   p.tiles = (tokens * G + p.rows - 1) / p.rows + sequences;
   const int64_t most = tokens * ((G + p.rows - 1) / p.rows);
   if (p.tiles > most) p.tiles = most;
-  const int64_t target = p.rows == 16 ? 1024 : 512;
+  const int64_t target = p.rows == 16 ? 1024 : 1024;
   p.min_blocks = p.rows == 16 ? 4 : 8;
   const int64_t blocks = width * page_size / kKeys + 1;
-  p.spare = blocks > p.min_blocks && p.tiles * KV < 4 * target ? (target + KV - 1) / KV : 0;
+  p.spare = blocks > p.min_blocks && p.tiles * KV < (p.rows == 16 ? 4 : 1) * target ? (target + KV - 1) / KV : 0;
   p.slots = p.tiles + p.spare;
   p.bytes = p.spare ? (size_t)p.slots * KV * p.rows * (kPagedDim + 2) * 4 : 0;
   return p;

@@ -667,8 +667,19 @@ __global__ __launch_bounds__(256) void paged_attention_merge_kernel(PagedArgs a)
   const bool refused = a.mask != nullptr && p.s.count > kMaxTreeTokens;
   for (int row = 4 * blockIdx.y + wave; row < end; row += 4 * gridDim.y) {
     auto at = [&](int chunk) { return ((size_t)slot_of(p, p.tile, chunk) * a.KV + kvh) * R + row; };
-    float M = -INFINITY;
-    for (int c0 = 0; c0 < p.chunks; c0 += 64)
+    // The first 64 chunks' maxima and sums and the first outputs are requested together.
+    constexpr int kAhead = 16;
+    const int n0 = min(64, p.chunks);
+    float2_t ml = lane < n0 ? a.part_ml[at(lane)] : float2_t{-INFINITY, 0.f};
+    float2_t o[kAhead];
+    auto load = [&](int c) {
+#pragma unroll
+      for (int u = 0; u < kAhead; ++u)
+        o[u] = *reinterpret_cast<const float2_t*>(a.part_o + at(min(c + u, p.chunks - 1)) * D + 2 * lane);
+    };
+    load(0);
+    float M = ml.x;
+    for (int c0 = 64; c0 < p.chunks; c0 += 64)
       if (c0 + lane < p.chunks) M = fmaxf(M, a.part_ml[at(c0 + lane)].x);
     M = wave_max_rl(M);
     const float Mu = M == -INFINITY ? 0.f : M;
@@ -676,16 +687,13 @@ __global__ __launch_bounds__(256) void paged_attention_merge_kernel(PagedArgs a)
     float2_t num = {0.f, 0.f};
     for (int c0 = 0; c0 < p.chunks; c0 += 64) {
       const int n = min(64, p.chunks - c0);
-      const float2_t ml = lane < n ? a.part_ml[at(c0 + lane)] : float2_t{-INFINITY, 0.f};
+      if (c0 > 0) ml = lane < n ? a.part_ml[at(c0 + lane)] : float2_t{-INFINITY, 0.f};
       const float w = exp2_hw(ml.x - Mu);
       den += wave_sum_rl(w * ml.y);
-      for (int c = 0; c < n; c += 8) {
-        float2_t o[8];
+      for (int c = 0; c < n; c += kAhead) {
+        if (c0 + c > 0) load(c0 + c);
 #pragma unroll
-        for (int u = 0; u < 8; ++u)
-          o[u] = *reinterpret_cast<const float2_t*>(a.part_o + at(c0 + min(c + u, n - 1)) * D + 2 * lane);
-#pragma unroll
-        for (int u = 0; u < 8; ++u)
+        for (int u = 0; u < kAhead; ++u)
           if (c + u < n) num += lane_f(w, min(c + u, 63)) * o[u];
       }
     }

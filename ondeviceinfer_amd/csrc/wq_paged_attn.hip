@@ -721,7 +721,10 @@ struct PagedPlan {
 
 PagedPlan paged_plan(int64_t tokens, int64_t sequences, int64_t G, int64_t KV, int64_t width, int64_t page_size) {
   PagedPlan p{};
-  p.rows = tokens * G > 32 * sequences ? kTileRows : 16;
+  // On average more than 48 rows per sequence take the large tiles, with the merge 16 us and up: 7 tokens of 40 / 8
+  // heads behind 4000 take 15.9 us in small tiles and 18.5 in large ones, 10 take 22.3 and 19.8 (batch 8: 10 tokens
+  // 39.0 and 38.1, 16 tokens 50.0 and 45.3).
+  p.rows = tokens * G > 48 * sequences ? kTileRows : 16;
   // sum_b ceil(count_b G / R) <= ceil(tokens G / R) + sequences, and no more tiles than rows.
   p.tiles = (tokens * G + p.rows - 1) / p.rows + sequences;
   const int64_t most = tokens * ((G + p.rows - 1) / p.rows);

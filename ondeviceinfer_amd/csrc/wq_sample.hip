@@ -155,28 +155,26 @@ __device__ __forceinline__ int bin_at(int depth) {
 __device__ __forceinline__ int bin_of(double below) { return bin_at((int)fmin(below, 64.0)); }
 __device__ __forceinline__ int bin_depth(int bin) { return bin < 8 ? bin : 8 + 4 * (bin - 8); }   // its first octave
 
-// 2^z: z = n / 32 + r with |r| <= 1 / 64, 2^(n/32) from a table of 32 and an
-// exponent, 2^r = e^(r ln 2) by its series to the fifth power (the next term
-// is below 3e-15 of the sum).
+// 2^(y - base): the fraction of y is k / 256 + r, 2^(k/256) comes from a table,
+// 2^r = e^(r ln 2) is its series to the fourth power (the next term is below
+// 2e-15 of the sum), and the whole octaves go into the exponent.
 struct Exp2Table {
-  double v[32];
+  double v[256];
 };
 
 __device__ __forceinline__ void fill_exp2(Exp2Table& t, int tid) {
-  if (tid < 32) t.v[tid] = exp2((double)tid / 32.0);
+  if (tid < 256) t.v[tid] = exp2((double)tid / 256.0);
 }
 
-__device__ __forceinline__ double exp2_64(double z, const Exp2Table& t) {
-  const double y = fmax(z, -1100.0);
-  const double n = rint(y * 32.0);
-  const double x = (y - n * (1.0 / 32.0)) * 0.69314718055994530942;
-  double s = x * (1.0 / 120.0) + 1.0 / 24.0;
-  s = s * x + 1.0 / 6.0;
+__device__ __forceinline__ double exp2_64(double y, double base, const Exp2Table& t) {
+  const double whole = floor(y), f = fmax(y - whole, 0.0);   // 0 for -inf, whose difference is NaN
+  const int k = (int)(f * 256.0);
+  const double x = (f - (double)k * (1.0 / 256.0)) * 0.69314718055994530942;
+  double s = x * (1.0 / 24.0) + 1.0 / 6.0;
   s = s * x + 0.5;
   s = s * x + 1.0;
   s = s * x + 1.0;
-  const int k = (int)n;
-  return z < -1080.0 ? 0.0 : ldexp(s * t.v[k & 31], k >> 5);
+  return ldexp(s * t.v[k], (int)fmax(whole - base, -1100.0));
 }
 
 // (best, at) the better of two of a row's largest: NaN first, then the larger, then the lower index.
@@ -259,7 +257,7 @@ __global__ __launch_bounds__(kTallyThreads) void sample_tally_kernel(SampleArgs 
       const double y = s.y(v[e]);
       const int b = bin_of(s.below(y));
       if ((in >> e) & 1) {
-        add_lds(&mass[b][tid], exp2_64(y - s.base, table));
+        add_lds(&mass[b][tid], exp2_64(y, s.base, table));
         add_lds(&count[b][tid], 1u);
       }
     }
@@ -311,9 +309,28 @@ struct RowTally {
   double scale[kMaxParts];    // 2^-octaves
 };
 
+// A thread's share of the row's tallies, requested before the row's settings are known.
+template <int THREADS>
+struct TallyShare {
+  static constexpr int N = kMaxParts * kBins / THREADS;
+  double mass[N];
+  uint32_t count[N];
+
+  __device__ __forceinline__ TallyShare(const SampleArgs& a, int row, int tid) {
+    const size_t from = (size_t)row * a.parts * kBins;
+#pragma unroll
+    for (int i = 0; i < N; ++i) {
+      const int e = min(tid + i * THREADS, a.parts * kBins - 1);
+      mass[i] = a.mass[from + e];
+      count[i] = a.count[from + e];
+    }
+  }
+};
+
 // By THREADS >= 256 threads, with barriers; the sums in a fixed order.
 template <int THREADS>
-__device__ __forceinline__ void read_tally(const SampleArgs& a, const Scale& s, int row, int tid, RowTally& t) {
+__device__ __forceinline__ void read_tally(const SampleArgs& a, const Scale& s, int row, int tid,
+                                           const TallyShare<THREADS>& share, RowTally& t) {
   const size_t from = (size_t)row * a.parts;
   if (tid < a.parts) {
     const float top = a.peak[from + tid].x;
@@ -323,9 +340,10 @@ __device__ __forceinline__ void read_tally(const SampleArgs& a, const Scale& s, 
     t.shift[tid] = (int)fmin(down, 64.0);
     t.scale[tid] = down < 1074.0 ? ldexp(1.0, -(int)down) : 0.0;
   }
-  for (int e = tid; e < a.parts * kBins; e += THREADS) {
-    (&t.raw_mass[0][0])[e] = a.mass[from * kBins + e];
-    (&t.raw_count[0][0])[e] = a.count[from * kBins + e];
+#pragma unroll
+  for (int i = 0; i < TallyShare<THREADS>::N; ++i) {   // past the last part: repeats, never read
+    (&t.raw_mass[0][0])[tid + i * THREADS] = share.mass[i];
+    (&t.raw_count[0][0])[tid + i * THREADS] = share.count[i];
   }
   __syncthreads();
   for (int e = tid; e < a.parts * kBins; e += THREADS) {
@@ -402,6 +420,8 @@ struct LaneBins {
     before = m - mass;
     count_before = n - count;
   }
+  __device__ __forceinline__ uint32_t first_of(int bin) const { return __shfl(count_before, bin); }
+  __device__ __forceinline__ uint32_t tokens_of(int bin) const { return __shfl(count, bin); }
   __device__ __forceinline__ double whole() const { return __shfl(before + mass, kBins - 1); }
   // The first bin up to `last` at which the mass reaches `goal`, and the mass in front of it.
   __device__ __forceinline__ int reach(double goal, int last, int lane, double& in_front) const {
@@ -448,12 +468,13 @@ __global__ __launch_bounds__(256) void sample_gather_kernel(SampleArgs a) {
   __shared__ RowTally tally;
   __shared__ int offset, end;
   const int row = blockIdx.y, part = blockIdx.x, tid = threadIdx.x, lane = tid & 63;
+  const TallyShare<256> share(a, row, tid);
   const Ask q = read_ask(a, row);
   int first;
   const float top = row_peak(a, row, lane, first);
   if (q.none || q.greedy || !(top > -INFINITY)) return;
   const Scale s(q.to_octaves, top);
-  read_tally<256>(a, s, row, tid, tally);
+  read_tally<256>(a, s, row, tid, share, tally);
   const Range g = find_range(a, q, s, LaneBins(tally, lane), lane);
   if (g.hi < g.lo || g.listed > (uint32_t)a.list_cap) return;
   if (tid < 64) {   // the part's place: the tokens of the parts in front of it
@@ -484,12 +505,15 @@ __global__ __launch_bounds__(256) void sample_gather_kernel(SampleArgs a) {
 #pragma unroll
     for (int e = 0; e < E; ++e) {
       const int b = bin_of(s.below(s.y(v[e])));
-      if (((in >> e) & 1) && b >= g.lo && b <= g.hi) {
+      if (((in >> e) & 1) & (int)(b >= g.lo) & (int)(b <= g.hi)) {
         const int to = atomicAdd(&offset, 1);
         if (to < limit) list[to] = float2_t{v[e], __builtin_bit_cast(float, r.index(c) + e)};
       }
     }
   }
+  // The place was counted by the tally; an entry that came out differently here would be no token, not an old one.
+  __syncthreads();
+  for (int i = offset + tid; i < limit; i += 256) list[i] = float2_t{0.f, __builtin_bit_cast(float, -1)};
 }
 
 // The order of the values as unsigned numbers, in as many bytes as the type has.
@@ -568,7 +592,8 @@ struct Picker {
       for (int i = tid; i < listed; i += kPickThreads) {
         const float2_t e = list[i];
         const float y = e.y;
-        f(e.x, __builtin_bit_cast(int, y));
+        const int index = __builtin_bit_cast(int, y);
+        if (index >= 0) f(e.x, index);
       }
     } else {
       for (int c = tid; c < r.chunks; c += kPickThreads) {
@@ -614,7 +639,7 @@ struct Picker {
         d = 255 - (int)((k >> (8 * byte)) & 255);
       }
       atomicAdd(&sh.step_count[d], 1u);
-      atomicAdd(&sh.step_mass[d], (unsigned long long)rint(exp2_64(y - s.base, sh.table) * unit));
+      atomicAdd(&sh.step_mass[d], (unsigned long long)rint(exp2_64(y, s.base, sh.table) * unit));
     });
     __syncthreads();
     if (tid < 64) {   // four steps per lane
@@ -676,6 +701,70 @@ struct Picker {
     __syncthreads();
   }
 
+  // Puts the (at most kMostSorted, `most` expected) tokens that `take` picks in
+  // order and leaves their weights beside them; their number.
+  template <typename F>
+  __device__ __forceinline__ int sort(F take, int most) {
+    __syncthreads();
+    if (tid == 0) sh.n = 0;
+    __syncthreads();
+    each([&](float v, int index) {
+      if (!take(v, s.y(v))) return;
+      const int to = atomicAdd(&sh.n, 1);
+      if (to < kMostSorted) sh.order[to] = order_of(v, index);
+    });
+    __syncthreads();
+    const int n = min(sh.n, min(most, kMostSorted));
+    uint64_t mine = ~0ull;
+    int rank = 0;
+    if (tid < n) {
+      mine = sh.order[tid];
+#pragma unroll 4
+      for (int j = 0; j < n; ++j) rank += sh.order[j] < mine;
+    }
+    __syncthreads();
+    if (tid < n) {
+      sh.order[rank] = mine;
+      sh.weight[rank] = exp2_64(s.y(Key<T>::value(~(uint32_t)(mine >> 32))), s.base, sh.table);
+    }
+    __syncthreads();
+    return n;
+  }
+
+  // The end among the sorted tokens first .. first + n - 1, all of them bin
+  // `bin`'s from where `above` of its mass lies in front: after `left` of them,
+  // or where the mass `goal` is reached; the first stays in any case.
+  __device__ __forceinline__ Cut end_in(int bin, bool by_mass, double before, double goal, int first, int n, int left,
+                                        double above) {
+    // 64 at a time, by every wave for itself.
+    const int lane = tid & 63;
+    double run = above;
+    int stay = 0;
+    for (int j0 = 0; j0 < n; j0 += 64) {
+      const int j = j0 + lane;
+      const double w = j < n ? sh.weight[first + j] : 0.0;
+      double upto = w;
+#pragma unroll
+      for (int o = 1; o < 64; o <<= 1) {
+        const double u = __shfl_up(upto, o);
+        if (lane >= o) upto += u;
+      }
+      const bool in = (j < n) & ((j == 0) | (by_mass ? before + run + (upto - w) < goal : j < left));
+      const int k = __popcll(__builtin_amdgcn_ballot_w64(in));   // the lanes 0 .. k - 1
+      if (k == 0) break;
+      stay += k;
+      run += __shfl(upto, k - 1);
+      if (k < 64) break;
+    }
+    stay = max(stay, 1);
+    const uint32_t end = (uint32_t)(sh.order[first + stay - 1] >> 32);
+    int ties = 0;
+    for (int j0 = 0; j0 < stay; j0 += 64)
+      ties += __popcll(__builtin_amdgcn_ballot_w64(
+          (j0 + lane < stay) & ((uint32_t)(sh.order[first + min(j0 + lane, stay - 1)] >> 32) == end)));
+    return Cut{bin, ~end, (uint32_t)ties, run};
+  }
+
   // Where the count `want`, or the mass `goal` of which `before` lies in front
   // of the bin, is reached among the tokens of bin `bin`.
   __device__ __forceinline__ Cut find_cut(int bin, bool by_mass, uint32_t want, double before, double goal) {
@@ -701,68 +790,11 @@ struct Picker {
     }
     Cut cut{bin, 0, 0, 0.0};
     if (few) {
-      const int n = sh.n;
-      __syncthreads();
-      if (tid == 0) sh.n = 0;
-      __syncthreads();
-      each([&](float v, int index) {
-        const double y = s.y(v);
-        if (bin_of(s.below(y)) != bin || sub_of(bin, y) != sub) return;
-        const int to = atomicAdd(&sh.n, 1);
-        if (to < kMostSorted) sh.order[to] = order_of(v, index);
-      });
-      __syncthreads();
-      uint64_t mine = ~0ull;
-      int rank = 0;
-      if (tid < n) {
-        mine = sh.order[tid];
-        for (int j = 0; j < n; ++j) rank += sh.order[j] < mine;
-      }
-      __syncthreads();
-      if (tid < n) {
-        sh.order[rank] = mine;
-        sh.weight[rank] = exp2_64(s.y(Key<T>::value(~(uint32_t)(mine >> 32))) - s.base, sh.table);
-      }
-      __syncthreads();
-      if (tid < 64) {   // how many stay, 64 at a time, and the ones among them that equal the last
-        double run = sh.above;
-        int stay = 0;
-        for (int j0 = 0; j0 < n; j0 += 64) {
-          const double w = j0 + tid < n ? sh.weight[j0 + tid] : 0.0;
-          double upto = w;
-#pragma unroll
-          for (int o = 1; o < 64; o <<= 1) {
-            const double u = __shfl_up(upto, o);
-            if (tid >= o) upto += u;
-          }
-          const int j = j0 + tid;
-          const bool in = j < n && (j == 0 || (by_mass ? before + run + (upto - w) < goal : j < (int)sh.left));
-          const int k = __popcll(__builtin_amdgcn_ballot_w64(in));   // the lanes 0 .. k - 1
-          if (k == 0) break;
-          stay += k;
-          run += __shfl(upto, k - 1);
-          if (k < 64) break;
-        }
-        stay = max(stay, 1);
-        const uint32_t end = (uint32_t)(sh.order[stay - 1] >> 32);
-        int ties = 0;
-        for (int j0 = 0; j0 < stay; j0 += 64)
-          ties += __popcll(__builtin_amdgcn_ballot_w64(j0 + tid < stay && (uint32_t)(sh.order[min(j0 + tid, stay - 1)] >> 32) == end));
-        if (tid == 0) {
-          sh.left = ~end;
-          sh.ties = (uint32_t)ties;
-          sh.above = run;
-        }
-      }
-      __syncthreads();
-      cut.key = sh.left;
-      cut.ties = sh.ties;
-      cut.kept = sh.above;
-      __syncthreads();
-      return cut;
+      const int n = sort([&](float v, double y) { return bin_of(s.below(y)) == bin && sub_of(bin, y) == sub; }, sh.n);
+      return end_in(bin, by_mass, before, goal, 0, n, (int)sh.left, sh.above);
     }
     cut.key = prefix;
-    const double w = exp2_64(s.y(Key<T>::value(prefix)) - s.base, sh.table);
+    const double w = exp2_64(s.y(Key<T>::value(prefix)), s.base, sh.table);
     if (by_mass) {
       const double need = ceil((goal - before - sh.above) / w);
       cut.ties = need >= (double)sh.n ? (uint32_t)sh.n : (uint32_t)fmax(need, 1.0);
@@ -782,6 +814,7 @@ __global__ __launch_bounds__(kPickThreads) void sample_pick_kernel(SampleArgs a)
   __shared__ PickShared sh;
   const int row = blockIdx.x, tid = threadIdx.x, lane = tid & 63;
   const int wave = __builtin_amdgcn_readfirstlane(tid >> 6);
+  const TallyShare<kPickThreads> share(a, row, tid);
   const Ask q = read_ask(a, row);
   int first;
   const float top = row_peak(a, row, lane, first);
@@ -792,7 +825,7 @@ __global__ __launch_bounds__(kPickThreads) void sample_pick_kernel(SampleArgs a)
   const Row<T> r(a, row);
   const Scale s(q.to_octaves, top);
   fill_exp2(sh.table, tid);
-  read_tally<kPickThreads>(a, s, row, tid, sh.tally);
+  read_tally<kPickThreads>(a, s, row, tid, share, sh.tally);
   const LaneBins bins(sh.tally, lane);
   const Range g = find_range(a, q, s, bins, lane);
   Picker<T> pick{a, r, s, sh, g.listed <= (uint32_t)a.list_cap ? a.list + (size_t)row * a.list_cap : nullptr,
@@ -801,6 +834,11 @@ __global__ __launch_bounds__(kPickThreads) void sample_pick_kernel(SampleArgs a)
   // Where top-k ends, then top-p of what it leaves.
   Cut cut{kBins, 0, 0, 0.0};
   double whole = g.whole;
+  // A short list is put in order as a whole, for both.
+  const bool cuts = g.by_k < kBins || q.top_p < 1.0;
+  const bool ordered = cuts && g.listed <= (uint32_t)min(a.list_cap, kMostSorted);
+  int sorted = 0;
+  if (ordered) sorted = pick.sort([](float, double) { return true; }, (int)g.listed);
   for (int stage = 0; stage < 2; ++stage) {
     const bool by_mass = stage == 1;
     if (by_mass ? q.top_p == 1.0 : g.by_k == kBins) continue;
@@ -808,7 +846,14 @@ __global__ __launch_bounds__(kPickThreads) void sample_pick_kernel(SampleArgs a)
     double before = g.before;
     int bin = g.by_k;
     if (by_mass) bin = bins.reach(goal, min(cut.bin, kBins - 1), lane, before);
-    const Cut end = pick.find_cut(bin, by_mass, g.want, before, goal);
+    Cut end;
+    if (ordered) {
+      const int from = (int)(bins.first_of(bin) - bins.first_of(g.lo));
+      const int n = min((int)bins.tokens_of(bin), sorted - from);
+      end = pick.end_in(bin, by_mass, before, goal, max(min(from, sorted - 1), 0), n, (int)g.want, 0.0);
+    } else {
+      end = pick.find_cut(bin, by_mass, g.want, before, goal);
+    }
     if (!by_mass) whole = before + end.kept;
     // Both may end at one value: the fewer ties.  Otherwise top-p's is the higher one, but for roundings.
     if (end.bin < cut.bin || end.key > cut.key) cut = end;
@@ -824,7 +869,7 @@ __global__ __launch_bounds__(kPickThreads) void sample_pick_kernel(SampleArgs a)
     const uint32_t k = Key<T>::of(v);
     return k > cut.key ? 1 : k == cut.key ? 2 : 0;
   };
-  auto weight = [&](double y) { return exp2_64(y - s.base, sh.table); };
+  auto weight = [&](double y) { return exp2_64(y, s.base, sh.table); };
 
   // What stays of every part: the bins in front of the edge, and its own tokens of the edge.
   const int bits = a.mass_bits + bin_depth(edge) - 1;
@@ -909,19 +954,34 @@ __global__ __launch_bounds__(kPickThreads) void sample_pick_kernel(SampleArgs a)
     for (int w = 0; w < wave; ++w) ties0 += sh.wave_n[w];
     ties0 += x - mine;
   }
-  double m = 0.0;
-  uint32_t ties = ties0;
-  for (int c = t0; c < t1; ++c) {
-    float v[E];
-    const uint32_t in = r.load(c, v);
+  // f(index, weight) over the thread's remaining tokens; the weights of a chunk are computed side by side.
+  auto walk = [&](auto f) {
+    uint32_t ties = ties0;
+    for (int c = t0; c < t1; ++c) {
+      float v[E];
+      const uint32_t in = r.load(c, v);
+      int st[E];
+      double w[E];
 #pragma unroll
-    for (int e = 0; e < E; ++e) {
-      if (!((in >> e) & 1)) continue;
-      const double y = s.y(v[e]);
-      const int st = stays(v[e], y);
-      if (st == 1 || (st == 2 && ties++ < cut.ties)) m += weight(y);
+      for (int e = 0; e < E; ++e) {
+        const double y = s.y(v[e]);
+        w[e] = weight(y);
+        st[e] = (in >> e) & 1 ? stays(v[e], y) : 0;
+      }
+#pragma unroll
+      for (int e = 0; e < E; ++e) {
+        const bool tie = st[e] == 2;
+        f(r.index(c) + e, (st[e] == 1) | (tie & (ties < cut.ties)) ? w[e] : 0.0);
+        ties += tie;
+      }
     }
-  }
+  };
+  double m = 0.0;
+  int last = -1;
+  walk([&](int index, double w) {
+    m += w;
+    last = w > 0.0 ? index : last;
+  });
   double x = m;
 #pragma unroll
   for (int o = 1; o < 64; o <<= 1) {
@@ -933,26 +993,19 @@ __global__ __launch_bounds__(kPickThreads) void sample_pick_kernel(SampleArgs a)
   double sum = 0.0;
   for (int w = 0; w < wave; ++w) sum += sh.wave_d[w];
   sum += x - m;
-  // The first token at which the running weight exceeds the target; failing that (roundings) the last that stays.
-  int hit = INT_MAX, last = -1;
-  ties = ties0;
-  for (int c = t0; c < t1; ++c) {
-    float v[E];
-    const uint32_t in = r.load(c, v);
-#pragma unroll
-    for (int e = 0; e < E; ++e) {
-      if (!((in >> e) & 1)) continue;
-      const double y = s.y(v[e]);
-      const int st = stays(v[e], y);
-      if (st == 1 || (st == 2 && ties++ < cut.ties)) {
-        const double w = weight(y);
-        sum += w;
-        if (w > 0.0) {
-          last = r.index(c) + e;
-          if (sum > target && hit == INT_MAX) hit = last;
-        }
+  // The first token at which the running weight exceeds the target: in the one thread whose share it lies in.  Failing
+  // that (roundings) the last that stays.
+  int hit = INT_MAX;
+  if (sum <= target && sum + m > target) {
+    hit = last;
+    bool found = false;
+    walk([&](int index, double w) {
+      sum += w;
+      if (!found & (sum > target) & (w > 0.0)) {
+        hit = index;
+        found = true;
       }
-    }
+    });
   }
 #pragma unroll
   for (int o = 32; o > 0; o >>= 1) {

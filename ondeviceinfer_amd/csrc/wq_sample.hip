@@ -22,12 +22,16 @@
 #include <limits.h>
 #include <math.h>
 
+// Every kernel has to find a token in the same octave: a product that the
+// compiler keeps unrounded in one place (y - floor(y) as one fused operation)
+// is another number than the rounded one it is compared with elsewhere.
+#pragma clang fp contract(off)
+
 namespace wq {
 namespace {
 
 constexpr int kBins = 16;
 constexpr int kMaxParts = 64;
-constexpr int kTallyThreads = 256;
 constexpr int kPickThreads = 1024;
 constexpr int kSub = 256;              // steps of a bin, or of a byte of the key
 constexpr int kMostSorted = 512;       // tokens of one step put in order at once
@@ -135,15 +139,18 @@ __device__ __forceinline__ Ask read_ask(const SampleArgs& a, int row) {
 struct Scale {
   double to_octaves, base;
   float top;
+  bool infinite;
 
-  __device__ __forceinline__ Scale(double per_logit, float largest) : to_octaves(per_logit), top(largest) {
-    base = isinf(largest) ? 3.0 : 4.0 * floor(0.25 * floor((double)largest * per_logit)) + 3.0;
+  __device__ __forceinline__ Scale(double per_logit, float largest)
+      : to_octaves(per_logit), top(largest), infinite(isinf(largest)) {
+    base = infinite ? 3.0 : 4.0 * floor(0.25 * floor((double)largest * per_logit)) + 3.0;
   }
   __device__ __forceinline__ double y(float v) const {
-    if (isinf(top)) return v == top && top > 0.f ? 0.0 : -INFINITY;
-    return (double)v * to_octaves;
+    const float u = infinite ? (((v == top) & (top > 0.f)) ? 0.f : -INFINITY) : v;
+    return (double)u * to_octaves;
   }
-  __device__ __forceinline__ double below(double y) const { return base - floor(y); }   // whole octaves
+  // Whole octaves below the base, 1100 for as many or more (2^-1100 is nothing).
+  __device__ __forceinline__ int below(double y) const { return (int)fmin(base - floor(y), 1100.0); }
 };
 
 // Bins of octaves below the base: eight of one octave, seven of four, and all
@@ -152,12 +159,12 @@ struct Scale {
 __device__ __forceinline__ int bin_at(int depth) {
   return depth < 8 ? max(depth, 0) : min(8 + ((depth - 8) >> 2), kBins - 1);
 }
-__device__ __forceinline__ int bin_of(double below) { return bin_at((int)fmin(below, 64.0)); }
 __device__ __forceinline__ int bin_depth(int bin) { return bin < 8 ? bin : 8 + 4 * (bin - 8); }   // its first octave
 
-// 2^(y - base): the fraction of y is k / 256 + r, 2^(k/256) comes from a table,
-// 2^r = e^(r ln 2) is its series to the fourth power (the next term is below
-// 2e-15 of the sum), and the whole octaves go into the exponent.
+// 2^(y - base), `below` whole octaves of it split off already: the fraction of
+// y is (k + t) / 256, 2^(k/256) comes from a table, 2^(t/256) = e^(t ln 2 /
+// 256) is its series to the fourth power (the next term is below 2e-15 of the
+// sum).
 struct Exp2Table {
   double v[256];
 };
@@ -166,15 +173,16 @@ __device__ __forceinline__ void fill_exp2(Exp2Table& t, int tid) {
   if (tid < 256) t.v[tid] = exp2((double)tid / 256.0);
 }
 
-__device__ __forceinline__ double exp2_64(double y, double base, const Exp2Table& t) {
-  const double whole = floor(y), f = fmax(y - whole, 0.0);   // 0 for -inf, whose difference is NaN
-  const int k = (int)(f * 256.0);
-  const double x = (f - (double)k * (1.0 / 256.0)) * 0.69314718055994530942;
-  double s = x * (1.0 / 24.0) + 1.0 / 6.0;
-  s = s * x + 0.5;
-  s = s * x + 1.0;
-  s = s * x + 1.0;
-  return ldexp(s * t.v[k], (int)fmax(whole - base, -1100.0));
+__device__ __forceinline__ double exp2_64(double y, int below, const Exp2Table& table) {
+  constexpr double c = 0.69314718055994530942 / 256.0;
+  const double f = 256.0 * fmax(y - floor(y), 0.0);   // 0 for -inf, whose difference is NaN
+  const int k = (int)f;
+  const double t = f - (double)k;
+  double s = __builtin_fma(t, c * c * c * c / 24.0, c * c * c / 6.0);
+  s = __builtin_fma(s, t, c * c / 2.0);
+  s = __builtin_fma(s, t, c);
+  s = __builtin_fma(s, t, 1.0);
+  return ldexp(s * table.v[k], -below);
 }
 
 // (best, at) the better of two of a row's largest: NaN first, then the larger, then the lower index.
@@ -200,31 +208,33 @@ __device__ __forceinline__ void add_lds(V* at, V v) {
   __hip_atomic_fetch_add(at, v, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_WORKGROUP);
 }
 
-// grid = (parts, rows), 256 threads.  Every thread adds to its own column of
-// the bins in LDS: no two lanes meet in a bank for longer than the access
-// takes, and the additions happen in a fixed order.
+// grid = (a workgroup per four parts, rows), a wave per part.  Every lane adds
+// to its own column of the wave's bins in LDS: no two lanes meet in a bank for
+// longer than the access takes, and the additions happen in a fixed order.
 template <typename T>
-__global__ __launch_bounds__(kTallyThreads) void sample_tally_kernel(SampleArgs a) {
+__global__ __launch_bounds__(256) void sample_tally_kernel(SampleArgs a) {
   constexpr int E = Row<T>::E;
-  __shared__ double mass[kBins][kTallyThreads];
-  __shared__ uint32_t count[kBins][kTallyThreads];
+  __shared__ double mass_of[4][kBins][64];
+  __shared__ uint32_t count_of[4][kBins][64];
   __shared__ Exp2Table table;
-  __shared__ float sv[4];
-  __shared__ int si[4];
-  const int row = blockIdx.y, part = blockIdx.x, tid = threadIdx.x;
+  const int row = blockIdx.y, tid = threadIdx.x, lane = tid & 63;
+  const int wave = __builtin_amdgcn_readfirstlane(tid >> 6);
+  const int part = 4 * blockIdx.x + wave;
+  double (&mass)[kBins][64] = mass_of[wave];
+  uint32_t (&count)[kBins][64] = count_of[wave];
   const Ask q = read_ask(a, row);
   const Row<T> r(a, row);
-  const int c0 = part * r.per_part, c1 = min(c0 + r.per_part, r.chunks);
+  const int c0 = min(part * r.per_part, r.chunks), c1 = min(c0 + r.per_part, r.chunks);
   fill_exp2(table, tid);
 #pragma unroll
   for (int b = 0; b < kBins; ++b) {
-    mass[b][tid] = 0.0;
-    count[b][tid] = 0;
+    mass[b][lane] = 0.0;
+    count[b][lane] = 0;
   }
   float best = -INFINITY;
   int at = INT_MAX;
   bool nan = false;
-  for (int c = c0 + tid; c < c1; c += kTallyThreads) {
+  for (int c = c0 + lane; c < c1; c += 64) {
     float v[E];
     r.load(c, v);
 #pragma unroll
@@ -238,41 +248,35 @@ __global__ __launch_bounds__(kTallyThreads) void sample_tally_kernel(SampleArgs 
   }
   if (nan) best = NAN;
   wave_peak(best, at);
-  if ((tid & 63) == 0) {
-    sv[tid >> 6] = best;
-    si[tid >> 6] = at;
-  }
-  __syncthreads();
-  best = sv[0];
-  at = si[0];
-  for (int w = 1; w < 4; ++w) keep_peak(best, at, sv[w], si[w]);
-  if (tid == 0) a.peak[(size_t)row * a.parts + part] = float2_t{best, __builtin_bit_cast(float, at)};
+  __syncthreads();   // the table
+  if (part >= a.parts) return;
+  if (lane == 0) a.peak[(size_t)row * a.parts + part] = float2_t{best, __builtin_bit_cast(float, at)};
   if (q.none || q.greedy || best != best) return;   // the pick needs no weights
   const Scale s(q.to_octaves, best);
-  for (int c = c0 + tid; c < c1; c += kTallyThreads) {
+  for (int c = c0 + lane; c < c1; c += 64) {
     float v[E];
     const uint32_t in = r.load(c, v);
 #pragma unroll
     for (int e = 0; e < E; ++e) {
       const double y = s.y(v[e]);
-      const int b = bin_of(s.below(y));
-      if ((in >> e) & 1) {
-        add_lds(&mass[b][tid], exp2_64(y, s.base, table));
-        add_lds(&count[b][tid], 1u);
-      }
+      const int below = s.below(y), b = bin_at(below);
+      const double w = exp2_64(y, below, table);
+      const uint32_t one = (in >> e) & 1;   // 0: not of the row
+      add_lds(&mass[b][lane], one ? w : 0.0);
+      add_lds(&count[b][lane], one);
     }
   }
-  __syncthreads();
-  // Thread (b, j) adds the columns j, j + 16, ...; then the 16 lanes of a bin.
-  const int b = tid >> 4, j = tid & 15;
+  // Lane (b, j) adds the columns j, j + 4, ...; then the four lanes of a bin.
+  const int b = lane >> 2, j = lane & 3;
   double m = 0.0;
   uint32_t n = 0;
-  for (int k = j; k < kTallyThreads; k += 16) {
-    m += mass[b][k];
-    n += count[b][k];
+#pragma unroll
+  for (int k = 0; k < 64; k += 4) {
+    m += mass[b][k + j];
+    n += count[b][k + j];
   }
 #pragma unroll
-  for (int o = 8; o > 0; o >>= 1) {
+  for (int o = 2; o > 0; o >>= 1) {
     m += __shfl_xor(m, o);
     n += __shfl_xor(n, o);
   }
@@ -437,7 +441,7 @@ __device__ __forceinline__ Range find_range(const SampleArgs& a, const Ask& q, c
   Range g{kBins, kBins, kBins, 0, -1, 0, 0.0, bins.whole(), -INFINITY};
   if (q.min_p > -INFINITY) {
     g.min_y = s.y(s.top) + q.min_p;
-    g.floor = bin_of(s.below(g.min_y));
+    g.floor = bin_at(s.below(g.min_y));
   }
   if (q.top_k < a.vocab) {
     const uint64_t hit = __builtin_amdgcn_ballot_w64(
@@ -460,68 +464,13 @@ __device__ __forceinline__ Range find_range(const SampleArgs& a, const Ask& q, c
   return g;
 }
 
-// grid = (parts, rows), 256 threads: the part's tokens of the bins lo .. hi
-// go to its place in the row's list (their order there does not matter).
-template <typename T>
-__global__ __launch_bounds__(256) void sample_gather_kernel(SampleArgs a) {
-  constexpr int E = Row<T>::E;
-  __shared__ RowTally tally;
-  __shared__ int offset, end;
-  const int row = blockIdx.y, part = blockIdx.x, tid = threadIdx.x, lane = tid & 63;
-  const TallyShare<256> share(a, row, tid);
-  const Ask q = read_ask(a, row);
-  int first;
-  const float top = row_peak(a, row, lane, first);
-  if (q.none || q.greedy || !(top > -INFINITY)) return;
-  const Scale s(q.to_octaves, top);
-  read_tally<256>(a, s, row, tid, share, tally);
-  const Range g = find_range(a, q, s, LaneBins(tally, lane), lane);
-  if (g.hi < g.lo || g.listed > (uint32_t)a.list_cap) return;
-  if (tid < 64) {   // the part's place: the tokens of the parts in front of it
-    uint32_t n = 0;
-    if (lane < a.parts)
-      for (int b = g.lo; b <= g.hi; ++b) n += tally.part_count[lane][b];
-    uint32_t upto = n;
-#pragma unroll
-    for (int o = 1; o < 64; o <<= 1) {
-      const uint32_t u = __shfl_up(upto, o);
-      if (lane >= o) upto += u;
-    }
-    if (lane == part) {
-      offset = (int)(upto - n);
-      end = (int)upto;
-    }
-  }
-  __syncthreads();
-  if (offset == end) return;
-  const Row<T> r(a, row);
-  const int c1 = min((part + 1) * r.per_part, r.chunks);
-  float2_t* list = a.list + (size_t)row * a.list_cap;
-  const int limit = end;
-  __syncthreads();
-  for (int c = part * r.per_part + tid; c < c1; c += 256) {
-    float v[E];
-    const uint32_t in = r.load(c, v);
-#pragma unroll
-    for (int e = 0; e < E; ++e) {
-      const int b = bin_of(s.below(s.y(v[e])));
-      if (((in >> e) & 1) & (int)(b >= g.lo) & (int)(b <= g.hi)) {
-        const int to = atomicAdd(&offset, 1);
-        if (to < limit) list[to] = float2_t{v[e], __builtin_bit_cast(float, r.index(c) + e)};
-      }
-    }
-  }
-  // The place was counted by the tally; an entry that came out differently here would be no token, not an old one.
-  __syncthreads();
-  for (int i = offset + tid; i < limit; i += 256) list[i] = float2_t{0.f, __builtin_bit_cast(float, -1)};
-}
-
 // The order of the values as unsigned numbers, in as many bytes as the type has.
 template <typename T>
 struct Key;
 template <>
 struct Key<half_t> {
   static constexpr int kBytes = 2;
+  static constexpr uint32_t kLowest = 0x03ffu, kHighest = 0xfc00u;   // of -inf and +inf
   static __device__ __forceinline__ uint32_t of(float v) {
     const half_t h = (half_t)v;   // exact: v came from fp16
     const uint32_t u = __builtin_bit_cast(uint16_t, h);
@@ -535,6 +484,7 @@ struct Key<half_t> {
 template <>
 struct Key<float> {
   static constexpr int kBytes = 4;
+  static constexpr uint32_t kLowest = 0x007fffffu, kHighest = 0xff800000u;
   static __device__ __forceinline__ uint32_t of(float v) {
     const uint32_t u = __builtin_bit_cast(uint32_t, v);
     return u & 0x80000000u ? ~u : (u | 0x80000000u);
@@ -544,6 +494,86 @@ struct Key<float> {
     return __builtin_bit_cast(float, u);
   }
 };
+
+// The smallest value whose bin is at most `bin` (bins fall as values rise),
+// found by the wave 64 keys at a time.
+template <typename T>
+__device__ __forceinline__ float lowest_of(const Scale& s, int bin, int lane) {
+  uint32_t lo = Key<T>::kLowest, n = Key<T>::kHighest - Key<T>::kLowest + 1;   // the key lies in lo .. lo + n - 1
+  while (n > 1) {
+    const uint32_t step = (n + 63) / 64;
+    const uint32_t k = min(lo + lane * step, Key<T>::kHighest);
+    const uint64_t in = __builtin_amdgcn_ballot_w64(bin_at(s.below(s.y(Key<T>::value(k)))) <= bin);
+    // The first probe that is in, or the stretch behind the last one.
+    const int first = in ? __builtin_ctzll(in) : 64;
+    if (first == 0) return Key<T>::value(lo);
+    const uint32_t next = lo + (first - 1) * step + 1;
+    const uint32_t end = first == 64 ? lo + n : lo + first * step + 1;
+    n = min(end, lo + n) - next;
+    lo = next;
+  }
+  return Key<T>::value(lo);
+}
+
+// Where the parts' tokens of the bins lo .. hi lie in the list, part `lane`'s.
+__device__ __forceinline__ void list_places(const RowTally& t, const Range& g, int parts, int lane, uint32_t& from,
+                                            uint32_t& to) {
+  uint32_t n = 0;
+  if (lane < parts)
+    for (int b = g.lo; b <= g.hi; ++b) n += t.part_count[lane][b];
+  to = n;
+#pragma unroll
+  for (int o = 1; o < 64; o <<= 1) {
+    const uint32_t u = __shfl_up(to, o);
+    if (lane >= o) to += u;
+  }
+  from = to - n;
+}
+
+// grid = (a workgroup per four parts, rows), a wave per part: its tokens of the
+// bins lo .. hi go to its place in the row's list.
+template <typename T>
+__global__ __launch_bounds__(256) void sample_gather_kernel(SampleArgs a) {
+  constexpr int E = Row<T>::E;
+  __shared__ RowTally tally;
+  const int row = blockIdx.y, tid = threadIdx.x, lane = tid & 63;
+  const int part = 4 * blockIdx.x + __builtin_amdgcn_readfirstlane(tid >> 6);
+  const TallyShare<256> share(a, row, tid);
+  const Ask q = read_ask(a, row);
+  int first;
+  const float top = row_peak(a, row, lane, first);
+  if (q.none || q.greedy || !(top > -INFINITY)) return;
+  const Scale s(q.to_octaves, top);
+  read_tally<256>(a, s, row, tid, share, tally);
+  const Range g = find_range(a, q, s, LaneBins(tally, lane), lane);
+  if (g.hi < g.lo || g.listed > (uint32_t)a.list_cap || part >= a.parts) return;
+  uint32_t from, to;
+  list_places(tally, g, a.parts, lane, from, to);
+  int at = __builtin_amdgcn_readlane((int)from, part);
+  const int end = __builtin_amdgcn_readlane((int)to, part);
+  if (at == end) return;
+  const float least = g.hi == kBins - 1 ? -INFINITY : lowest_of<T>(s, g.hi, lane);
+  const float above = g.lo == 0 ? NAN : lowest_of<T>(s, g.lo - 1, lane);   // NaN: no bound
+  const Row<T> r(a, row);
+  const int c0 = part * r.per_part, c1 = min(c0 + r.per_part, r.chunks);
+  float2_t* list = a.list + (size_t)row * a.list_cap;
+  for (int c = c0; c < c1; c += 64) {
+    float v[E];
+    const uint32_t in = c + lane < c1 ? r.load(c + lane, v) : 0u;
+#pragma unroll
+    for (int e = 0; e < E; ++e) {
+      const bool take = (bool)((in >> e) & 1) & (v[e] >= least) & !(v[e] >= above);
+      const uint64_t mask = __builtin_amdgcn_ballot_w64(take);
+      if (mask == 0) continue;
+      const int to_at = at + (int)__builtin_amdgcn_mbcnt_hi((uint32_t)(mask >> 32),
+                                                            __builtin_amdgcn_mbcnt_lo((uint32_t)mask, 0u));
+      if (take && to_at < end) list[to_at] = float2_t{v[e], __builtin_bit_cast(float, r.index(c + lane) + e)};
+      at += __popcll(mask);
+    }
+  }
+  // The place was counted by the tally; an entry that came out differently here would be no token, not an old one.
+  for (int i = at + lane; i < end; i += 64) list[i] = float2_t{0.f, __builtin_bit_cast(float, -1)};
+}
 
 // The value at which a cut ends, among the row's tokens of one bin.
 struct Cut {
@@ -559,7 +589,7 @@ struct PickShared {
   uint32_t step_count[kSub];
   unsigned long long step_mass[kSub];
   uint64_t order[kMostSorted];    // (order of the value, index), the first of the order smallest
-  double weight[kMostSorted];
+  double upto[kMostSorted];       // weights of the tokens up to each
   double part_mass[kMaxParts];
   unsigned long long part_edge[kMaxParts];
   uint32_t part_ties[kMaxParts];
@@ -606,6 +636,11 @@ struct Picker {
     }
   }
 
+  __device__ __forceinline__ double weight_of(float v) const {
+    const double y = s.y(v);
+    return exp2_64(y, s.below(y), sh.table);
+  }
+
   __device__ __forceinline__ uint64_t order_of(float v, int index) const {
     return ((uint64_t)(~Key<T>::of(v)) << 32) | (uint32_t)index;
   }
@@ -631,7 +666,7 @@ struct Picker {
     __syncthreads();
     each([&](float v, int) {
       const double y = s.y(v);
-      if (bin_of(s.below(y)) != bin) return;
+      if (bin_at(s.below(y)) != bin) return;
       int d = sub_of(bin, y);
       if (byte < Key<T>::kBytes) {
         const uint32_t k = Key<T>::of(v);
@@ -639,7 +674,7 @@ struct Picker {
         d = 255 - (int)((k >> (8 * byte)) & 255);
       }
       atomicAdd(&sh.step_count[d], 1u);
-      atomicAdd(&sh.step_mass[d], (unsigned long long)rint(exp2_64(y, s.base, sh.table) * unit));
+      atomicAdd(&sh.step_mass[d], (unsigned long long)rint(exp2_64(y, s.below(y), sh.table) * unit));
     });
     __syncthreads();
     if (tid < 64) {   // four steps per lane
@@ -715,18 +750,32 @@ struct Picker {
     });
     __syncthreads();
     const int n = min(sh.n, min(most, kMostSorted));
+    // Each token's rank, by as many threads as there are for it.
+    int each_by = 64;
+    while (each_by > 2 && n * each_by > kPickThreads) each_by >>= 1;
+    const int i = tid / each_by;
     uint64_t mine = ~0ull;
     int rank = 0;
-    if (tid < n) {
-      mine = sh.order[tid];
+    if (i < n) {
+      mine = sh.order[i];
 #pragma unroll 4
-      for (int j = 0; j < n; ++j) rank += sh.order[j] < mine;
+      for (int j = tid & (each_by - 1); j < n; j += each_by) rank += sh.order[j] < mine;
     }
+    for (int o = each_by >> 1; o > 0; o >>= 1) rank += __shfl_xor(rank, o);
     __syncthreads();
-    if (tid < n) {
-      sh.order[rank] = mine;
-      sh.weight[rank] = exp2_64(s.y(Key<T>::value(~(uint32_t)(mine >> 32))), s.base, sh.table);
+    if (i < n && (tid & (each_by - 1)) == 0) sh.order[rank] = mine;
+    __syncthreads();
+    const int lane = tid & 63, wave = tid >> 6;
+    double x = tid < n ? weight_of(Key<T>::value(~(uint32_t)(sh.order[tid] >> 32))) : 0.0;
+#pragma unroll
+    for (int o = 1; o < 64; o <<= 1) {
+      const double u = __shfl_up(x, o);
+      if (lane >= o) x += u;
     }
+    if (lane == 63) sh.wave_d[wave] = x;
+    __syncthreads();
+    for (int w = 0; w < wave; ++w) x += sh.wave_d[w];
+    if (tid < n) sh.upto[tid] = x;
     __syncthreads();
     return n;
   }
@@ -736,33 +785,13 @@ struct Picker {
   // or where the mass `goal` is reached; the first stays in any case.
   __device__ __forceinline__ Cut end_in(int bin, bool by_mass, double before, double goal, int first, int n, int left,
                                         double above) {
-    // 64 at a time, by every wave for itself.
-    const int lane = tid & 63;
-    double run = above;
-    int stay = 0;
-    for (int j0 = 0; j0 < n; j0 += 64) {
-      const int j = j0 + lane;
-      const double w = j < n ? sh.weight[first + j] : 0.0;
-      double upto = w;
-#pragma unroll
-      for (int o = 1; o < 64; o <<= 1) {
-        const double u = __shfl_up(upto, o);
-        if (lane >= o) upto += u;
-      }
-      const bool in = (j < n) & ((j == 0) | (by_mass ? before + run + (upto - w) < goal : j < left));
-      const int k = __popcll(__builtin_amdgcn_ballot_w64(in));   // the lanes 0 .. k - 1
-      if (k == 0) break;
-      stay += k;
-      run += __shfl(upto, k - 1);
-      if (k < 64) break;
-    }
-    stay = max(stay, 1);
+    const double front = first > 0 ? sh.upto[first - 1] : 0.0;
+    const double run = tid > 0 && tid < n ? above + (sh.upto[first + tid - 1] - front) : above;
+    const bool in = (tid < n) & ((tid == 0) | (by_mass ? before + run < goal : tid < left));
+    const int stay = max(__syncthreads_count(in), 1);
     const uint32_t end = (uint32_t)(sh.order[first + stay - 1] >> 32);
-    int ties = 0;
-    for (int j0 = 0; j0 < stay; j0 += 64)
-      ties += __popcll(__builtin_amdgcn_ballot_w64(
-          (j0 + lane < stay) & ((uint32_t)(sh.order[first + min(j0 + lane, stay - 1)] >> 32) == end)));
-    return Cut{bin, ~end, (uint32_t)ties, run};
+    const int ties = __syncthreads_count((tid < stay) & ((uint32_t)(sh.order[first + min(tid, stay - 1)] >> 32) == end));
+    return Cut{bin, ~end, (uint32_t)ties, above + (sh.upto[first + stay - 1] - front)};
   }
 
   // Where the count `want`, or the mass `goal` of which `before` lies in front
@@ -790,11 +819,11 @@ struct Picker {
     }
     Cut cut{bin, 0, 0, 0.0};
     if (few) {
-      const int n = sort([&](float v, double y) { return bin_of(s.below(y)) == bin && sub_of(bin, y) == sub; }, sh.n);
+      const int n = sort([&](float v, double y) { return bin_at(s.below(y)) == bin && sub_of(bin, y) == sub; }, sh.n);
       return end_in(bin, by_mass, before, goal, 0, n, (int)sh.left, sh.above);
     }
     cut.key = prefix;
-    const double w = exp2_64(s.y(Key<T>::value(prefix)), s.base, sh.table);
+    const double w = weight_of(Key<T>::value(prefix));
     if (by_mass) {
       const double need = ceil((goal - before - sh.above) / w);
       cut.ties = need >= (double)sh.n ? (uint32_t)sh.n : (uint32_t)fmax(need, 1.0);
@@ -860,34 +889,56 @@ __global__ __launch_bounds__(kPickThreads) void sample_pick_kernel(SampleArgs a)
     else if (end.key == cut.key) cut.ties = min(cut.ties, end.ties);
   }
   const int edge = min(cut.bin, g.floor);   // the only bin of which some tokens stay and some go
-  // 1: stays, 2: stays while there are ties left.
-  auto stays = [&](float v, double y) -> int {
-    const int b = bin_of(s.below(y));
-    if (b != edge) return b < edge;
-    if (y < g.min_y) return 0;
-    if (b < cut.bin) return 1;
-    const uint32_t k = Key<T>::of(v);
-    return k > cut.key ? 1 : k == cut.key ? 2 : 0;
-  };
-  auto weight = [&](double y) { return exp2_64(y, s.base, sh.table); };
+  // Bins, keys and y all rise with the value: 1 stays, 2 stays while there are ties left.
+  const float last_value = cut.bin < kBins ? Key<T>::value(cut.key) : -INFINITY;
+  const double min_y = g.min_y;
+  auto stays = [&](float v, double y) -> int { return y >= min_y ? (int)(v > last_value) + 2 * (int)(v == last_value) : 0; };
+  auto weight = [&](double y) { return exp2_64(y, s.below(y), sh.table); };
 
-  // What stays of every part: the bins in front of the edge, and its own tokens of the edge.
+  // What stays of every part: the bins in front of the edge, and its own tokens of the edge, a wave per part.
   const int bits = a.mass_bits + bin_depth(edge) - 1;
   const double unit = ldexp(1.0, bits), per_unit = ldexp(1.0, -bits);
-  if (tid < kMaxParts) {
-    sh.part_edge[tid] = 0;
-    sh.part_ties[tid] = 0;
-  }
-  __syncthreads();
-  if (edge < kBins)
-    pick.each([&](float v, int index) {
+  uint32_t list_from = 0, list_to = 0;
+  list_places(sh.tally, g, a.parts, lane, list_from, list_to);
+  for (int p = wave; p < a.parts; p += kPickThreads / 64) {
+    unsigned long long m = 0;
+    uint32_t ties = 0;
+    auto add = [&](float v) {
       const double y = s.y(v);
-      if (bin_of(s.below(y)) != edge) return;
+      if (bin_at(s.below(y)) != edge) return;
       const int st = stays(v, y);
-      const int p = (index + r.lead) / E / r.per_part;
-      if (st == 1) atomicAdd(&sh.part_edge[p], (unsigned long long)rint(weight(y) * unit));
-      if (st == 2) atomicAdd(&sh.part_ties[p], 1u);
-    });
+      if (st == 1) m += (unsigned long long)rint(weight(y) * unit);
+      ties += st == 2;
+    };
+    if (edge < kBins && sh.tally.part_count[p][edge] != 0) {
+      if (pick.list != nullptr) {
+        const int to = __builtin_amdgcn_readlane((int)list_to, p);
+        for (int i = __builtin_amdgcn_readlane((int)list_from, p) + lane; i < to; i += 64) {
+          const float2_t e = pick.list[i];
+          const float index = e.y;
+          if (__builtin_bit_cast(int, index) >= 0) add(e.x);
+        }
+      } else {
+        const int c1 = min((p + 1) * r.per_part, r.chunks);
+        for (int c = p * r.per_part + lane; c < c1; c += 64) {
+          float v[E];
+          const uint32_t in = r.load(c, v);
+#pragma unroll
+          for (int e = 0; e < E; ++e)
+            if ((in >> e) & 1) add(v[e]);
+        }
+      }
+#pragma unroll
+      for (int o = 32; o > 0; o >>= 1) {
+        m += __shfl_xor(m, o);
+        ties += __shfl_xor(ties, o);
+      }
+    }
+    if (lane == 0) {
+      sh.part_edge[p] = m;
+      sh.part_ties[p] = ties;
+    }
+  }
   __syncthreads();
   if (wave == 0) {   // a part per lane
     double m = 0.0;
@@ -954,34 +1005,27 @@ __global__ __launch_bounds__(kPickThreads) void sample_pick_kernel(SampleArgs a)
     for (int w = 0; w < wave; ++w) ties0 += sh.wave_n[w];
     ties0 += x - mine;
   }
-  // f(index, weight) over the thread's remaining tokens; the weights of a chunk are computed side by side.
-  auto walk = [&](auto f) {
+  double m = 0.0;
+  int last = -1;
+  {
     uint32_t ties = ties0;
     for (int c = t0; c < t1; ++c) {
       float v[E];
       const uint32_t in = r.load(c, v);
-      int st[E];
-      double w[E];
 #pragma unroll
       for (int e = 0; e < E; ++e) {
         const double y = s.y(v[e]);
-        w[e] = weight(y);
-        st[e] = (in >> e) & 1 ? stays(v[e], y) : 0;
-      }
-#pragma unroll
-      for (int e = 0; e < E; ++e) {
-        const bool tie = st[e] == 2;
-        f(r.index(c) + e, (st[e] == 1) | (tie & (ties < cut.ties)) ? w[e] : 0.0);
+        const int st = (in >> e) & 1 ? stays(v[e], y) : 0;
+        const bool tie = st == 2;
+        const bool in_draw = (st == 1) | (tie & (ties < cut.ties));
         ties += tie;
+        if (__builtin_amdgcn_ballot_w64(in_draw) == 0) continue;   // of a filtered row most waves have nothing here
+        const double w = in_draw ? weight(y) : 0.0;
+        m += w;
+        last = w > 0.0 ? r.index(c) + e : last;
       }
     }
-  };
-  double m = 0.0;
-  int last = -1;
-  walk([&](int index, double w) {
-    m += w;
-    last = w > 0.0 ? index : last;
-  });
+  }
   double x = m;
 #pragma unroll
   for (int o = 1; o < 64; o <<= 1) {
@@ -993,19 +1037,39 @@ __global__ __launch_bounds__(kPickThreads) void sample_pick_kernel(SampleArgs a)
   double sum = 0.0;
   for (int w = 0; w < wave; ++w) sum += sh.wave_d[w];
   sum += x - m;
-  // The first token at which the running weight exceeds the target: in the one thread whose share it lies in.  Failing
-  // that (roundings) the last that stays.
+  // The first token at which the running weight exceeds the target: in the one thread's run where it does, a token per
+  // lane of that thread's wave.  Failing that (roundings) the last that stays.
   int hit = INT_MAX;
-  if (sum <= target && sum + m > target) {
-    hit = last;
-    bool found = false;
-    walk([&](int index, double w) {
-      sum += w;
-      if (!found & (sum > target) & (w > 0.0)) {
-        hit = index;
-        found = true;
+  const uint64_t mine = __builtin_amdgcn_ballot_w64(sum <= target && sum + m > target);
+  if (mine != 0) {
+    const int l = __builtin_ctzll(mine);
+    const int f0 = __builtin_amdgcn_readlane(t0, l), f1 = __builtin_amdgcn_readlane(t1, l);
+    double before = __shfl(sum, l);
+    uint32_t ties = (uint32_t)__builtin_amdgcn_readlane((int)ties0, l);
+    hit = __builtin_amdgcn_readlane(last, l);
+    const int j1 = min(r.index(f1), r.vocab);
+    for (int j0 = max(r.index(f0), 0); j0 < j1; j0 += 64) {
+      const int j = j0 + lane;
+      const float v = j < j1 ? (float)r.base[j] + 0.f : 0.f;
+      const double y = s.y(v);
+      const int st = j < j1 ? stays(v, y) : 0;
+      const uint64_t tied = __builtin_amdgcn_ballot_w64(st == 2);
+      const uint32_t in_front = ties + (uint32_t)__popcll(tied & ((1ull << lane) - 1));
+      const double w = (st == 1) | ((st == 2) & (in_front < cut.ties)) ? weight(y) : 0.0;
+      double upto = w;
+#pragma unroll
+      for (int o = 1; o < 64; o <<= 1) {
+        const double u = __shfl_up(upto, o);
+        if (lane >= o) upto += u;
       }
-    });
+      const uint64_t past = __builtin_amdgcn_ballot_w64((w > 0.0) & (before + upto > target));
+      if (past) {
+        hit = j0 + __builtin_ctzll(past);
+        break;
+      }
+      before += __shfl(upto, 63);
+      ties += (uint32_t)__popcll(tied);
+    }
   }
 #pragma unroll
   for (int o = 32; o > 0; o >>= 1) {
@@ -1026,11 +1090,11 @@ __global__ __launch_bounds__(kPickThreads) void sample_pick_kernel(SampleArgs a)
   }
 }
 
-// Parts of a row: about four workgroups per compute unit over all rows, each
-// with at least 4096 tokens.
+// Parts of a row, a wave each: sixteen waves per compute unit over all rows,
+// and at least 1024 tokens each.
 int sample_parts(int64_t rows, int64_t vocab) {
-  int64_t p = (1024 + rows - 1) / rows;
-  const int64_t most = (vocab + 4095) / 4096;
+  int64_t p = (4096 + rows - 1) / rows;
+  const int64_t most = (vocab + 1023) / 1024;
   if (p > most) p = most;
   if (p > kMaxParts) p = kMaxParts;
   return (int)(p < 1 ? 1 : p);
@@ -1059,8 +1123,8 @@ int sample_check(int64_t rows, int64_t vocab) {
 
 template <typename T>
 int launch_sample(const SampleArgs& a, hipStream_t s) {
-  const dim3 grid((unsigned)a.parts, (unsigned)a.rows);
-  hipLaunchKernelGGL(sample_tally_kernel<T>, grid, dim3(kTallyThreads), 0, s, a);
+  const dim3 grid((unsigned)((a.parts + 3) / 4), (unsigned)a.rows);
+  hipLaunchKernelGGL(sample_tally_kernel<T>, grid, dim3(256), 0, s, a);
   int rc = check_launch("sample_tally");
   if (rc != WQ_OK) return rc;
   hipLaunchKernelGGL(sample_gather_kernel<T>, grid, dim3(256), 0, s, a);

@@ -208,33 +208,35 @@ __device__ __forceinline__ void add_lds(V* at, V v) {
   __hip_atomic_fetch_add(at, v, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_WORKGROUP);
 }
 
-// grid = (a workgroup per four parts, rows), a wave per part.  Every lane adds
-// to its own column of the wave's bins in LDS: no two lanes meet in a bank for
-// longer than the access takes, and the additions happen in a fixed order.
-template <typename T>
+// grid = (workgroups of 4 / W parts, rows): W = 1 wave per part, or all four
+// where few rows leave waves to spare (sample_waves).  Every thread adds to its
+// own column of the bins in LDS: no two lanes meet in a bank for longer than
+// the access takes, and the additions happen in a fixed order.
+template <typename T, int W>
 __global__ __launch_bounds__(256) void sample_tally_kernel(SampleArgs a) {
   constexpr int E = Row<T>::E;
-  __shared__ double mass_of[4][kBins][64];
-  __shared__ uint32_t count_of[4][kBins][64];
+  __shared__ double mass[kBins][256];
+  __shared__ uint32_t count[kBins][256];
   __shared__ Exp2Table table;
+  __shared__ float sv[4];
+  __shared__ int si[4];
   const int row = blockIdx.y, tid = threadIdx.x, lane = tid & 63;
   const int wave = __builtin_amdgcn_readfirstlane(tid >> 6);
-  const int part = 4 * blockIdx.x + wave;
-  double (&mass)[kBins][64] = mass_of[wave];
-  uint32_t (&count)[kBins][64] = count_of[wave];
+  const int part = blockIdx.x * (4 / W) + (W == 1 ? wave : 0);
+  const int mine = W == 1 ? lane : tid;   // of the part's 64 W threads
   const Ask q = read_ask(a, row);
   const Row<T> r(a, row);
   const int c0 = min(part * r.per_part, r.chunks), c1 = min(c0 + r.per_part, r.chunks);
   fill_exp2(table, tid);
 #pragma unroll
   for (int b = 0; b < kBins; ++b) {
-    mass[b][lane] = 0.0;
-    count[b][lane] = 0;
+    mass[b][tid] = 0.0;
+    count[b][tid] = 0;
   }
   float best = -INFINITY;
   int at = INT_MAX;
   bool nan = false;
-  for (int c = c0 + lane; c < c1; c += 64) {
+  for (int c = c0 + mine; c < c1; c += 64 * W) {
     float v[E];
     r.load(c, v);
 #pragma unroll
@@ -248,12 +250,21 @@ __global__ __launch_bounds__(256) void sample_tally_kernel(SampleArgs a) {
   }
   if (nan) best = NAN;
   wave_peak(best, at);
-  __syncthreads();   // the table
+  if (lane == 0) {
+    sv[wave] = best;
+    si[wave] = at;
+  }
+  __syncthreads();
+  if (W > 1) {
+    best = sv[0];
+    at = si[0];
+    for (int w = 1; w < W; ++w) keep_peak(best, at, sv[w], si[w]);
+  }
   if (part >= a.parts) return;
-  if (lane == 0) a.peak[(size_t)row * a.parts + part] = float2_t{best, __builtin_bit_cast(float, at)};
+  if (mine == 0) a.peak[(size_t)row * a.parts + part] = float2_t{best, __builtin_bit_cast(float, at)};
   if (q.none || q.greedy || best != best) return;   // the pick needs no weights
   const Scale s(q.to_octaves, best);
-  for (int c = c0 + lane; c < c1; c += 64) {
+  for (int c = c0 + mine; c < c1; c += 64 * W) {
     float v[E];
     const uint32_t in = r.load(c, v);
 #pragma unroll
@@ -262,21 +273,22 @@ __global__ __launch_bounds__(256) void sample_tally_kernel(SampleArgs a) {
       const int below = s.below(y), b = bin_at(below);
       const double w = exp2_64(y, below, table);
       const uint32_t one = (in >> e) & 1;   // 0: not of the row
-      add_lds(&mass[b][lane], one ? w : 0.0);
-      add_lds(&count[b][lane], one);
+      add_lds(&mass[b][tid], one ? w : 0.0);
+      add_lds(&count[b][tid], one);
     }
   }
-  // Lane (b, j) adds the columns j, j + 4, ...; then the four lanes of a bin.
-  const int b = lane >> 2, j = lane & 3;
+  if (W > 1) __syncthreads();
+  // 4 W threads per bin: thread (b, j) adds the columns j, j + 4 W, ...
+  const int b = mine / (4 * W), j = mine % (4 * W), from = tid - mine;
   double m = 0.0;
   uint32_t n = 0;
 #pragma unroll
-  for (int k = 0; k < 64; k += 4) {
-    m += mass[b][k + j];
-    n += count[b][k + j];
+  for (int k = 0; k < 64 * W; k += 4 * W) {
+    m += mass[b][from + k + j];
+    n += count[b][from + k + j];
   }
 #pragma unroll
-  for (int o = 2; o > 0; o >>= 1) {
+  for (int o = 2 * W; o > 0; o >>= 1) {
     m += __shfl_xor(m, o);
     n += __shfl_xor(n, o);
   }
@@ -530,14 +542,16 @@ __device__ __forceinline__ void list_places(const RowTally& t, const Range& g, i
   from = to - n;
 }
 
-// grid = (a workgroup per four parts, rows), a wave per part: its tokens of the
-// bins lo .. hi go to its place in the row's list.
-template <typename T>
+// grid = (workgroups of 4 / W parts, rows) as for the tally: a part's tokens of
+// the bins lo .. hi go to its place in the row's list, in no order.
+template <typename T, int W>
 __global__ __launch_bounds__(256) void sample_gather_kernel(SampleArgs a) {
   constexpr int E = Row<T>::E;
   __shared__ RowTally tally;
+  __shared__ int next[4];   // W > 1: the part's next entry, in next[0]
   const int row = blockIdx.y, tid = threadIdx.x, lane = tid & 63;
-  const int part = 4 * blockIdx.x + __builtin_amdgcn_readfirstlane(tid >> 6);
+  const int wave = __builtin_amdgcn_readfirstlane(tid >> 6);
+  const int part = blockIdx.x * (4 / W) + (W == 1 ? wave : 0);
   const TallyShare<256> share(a, row, tid);
   const Ask q = read_ask(a, row);
   int first;
@@ -552,12 +566,16 @@ __global__ __launch_bounds__(256) void sample_gather_kernel(SampleArgs a) {
   int at = __builtin_amdgcn_readlane((int)from, part);
   const int end = __builtin_amdgcn_readlane((int)to, part);
   if (at == end) return;
+  if (W > 1) {
+    if (tid == 0) next[0] = at;
+    __syncthreads();
+  }
   const float least = g.hi == kBins - 1 ? -INFINITY : lowest_of<T>(s, g.hi, lane);
   const float above = g.lo == 0 ? NAN : lowest_of<T>(s, g.lo - 1, lane);   // NaN: no bound
   const Row<T> r(a, row);
   const int c0 = part * r.per_part, c1 = min(c0 + r.per_part, r.chunks);
   float2_t* list = a.list + (size_t)row * a.list_cap;
-  for (int c = c0; c < c1; c += 64) {
+  for (int c = c0 + (W == 1 ? 0 : 64 * wave); c < c1; c += 64 * W) {
     float v[E];
     const uint32_t in = c + lane < c1 ? r.load(c + lane, v) : 0u;
 #pragma unroll
@@ -565,14 +583,25 @@ __global__ __launch_bounds__(256) void sample_gather_kernel(SampleArgs a) {
       const bool take = (bool)((in >> e) & 1) & (v[e] >= least) & !(v[e] >= above);
       const uint64_t mask = __builtin_amdgcn_ballot_w64(take);
       if (mask == 0) continue;
+      const int n = __popcll(mask);
+      if (W > 1) {
+        int first_at = 0;
+        if (lane == 0) first_at = atomicAdd(&next[0], n);
+        at = __builtin_amdgcn_readfirstlane(first_at);
+      }
       const int to_at = at + (int)__builtin_amdgcn_mbcnt_hi((uint32_t)(mask >> 32),
                                                             __builtin_amdgcn_mbcnt_lo((uint32_t)mask, 0u));
       if (take && to_at < end) list[to_at] = float2_t{v[e], __builtin_bit_cast(float, r.index(c + lane) + e)};
-      at += __popcll(mask);
+      at += n;
     }
   }
   // The place was counted by the tally; an entry that came out differently here would be no token, not an old one.
-  for (int i = at + lane; i < end; i += 64) list[i] = float2_t{0.f, __builtin_bit_cast(float, -1)};
+  if (W > 1) {
+    __syncthreads();
+    at = next[0];
+  }
+  for (int i = at + (W == 1 ? lane : tid); i < end; i += 64 * W)
+    list[i] = float2_t{0.f, __builtin_bit_cast(float, -1)};
 }
 
 // The value at which a cut ends, among the row's tokens of one bin.
@@ -598,6 +627,7 @@ struct PickShared {
   int wave_i[16];
   // what one thread found for all
   int step, n;
+  int taken;   // tokens taken so far by sort(), zero between two of them
   uint32_t left, ties;
   double above, target;
   int part;
@@ -740,16 +770,13 @@ struct Picker {
   // order and leaves their weights beside them; their number.
   template <typename F>
   __device__ __forceinline__ int sort(F take, int most) {
-    __syncthreads();
-    if (tid == 0) sh.n = 0;
-    __syncthreads();
     each([&](float v, int index) {
       if (!take(v, s.y(v))) return;
-      const int to = atomicAdd(&sh.n, 1);
+      const int to = atomicAdd(&sh.taken, 1);
       if (to < kMostSorted) sh.order[to] = order_of(v, index);
     });
     __syncthreads();
-    const int n = min(sh.n, min(most, kMostSorted));
+    const int n = min(sh.taken, min(most, kMostSorted));
     // Each token's rank, by as many threads as there are for it.
     int each_by = 64;
     while (each_by > 2 && n * each_by > kPickThreads) each_by >>= 1;
@@ -776,6 +803,7 @@ struct Picker {
     __syncthreads();
     for (int w = 0; w < wave; ++w) x += sh.wave_d[w];
     if (tid < n) sh.upto[tid] = x;
+    if (tid == 0) sh.taken = 0;
     __syncthreads();
     return n;
   }
@@ -786,12 +814,25 @@ struct Picker {
   __device__ __forceinline__ Cut end_in(int bin, bool by_mass, double before, double goal, int first, int n, int left,
                                         double above) {
     const double front = first > 0 ? sh.upto[first - 1] : 0.0;
-    const double run = tid > 0 && tid < n ? above + (sh.upto[first + tid - 1] - front) : above;
-    const bool in = (tid < n) & ((tid == 0) | (by_mass ? before + run < goal : tid < left));
-    const int stay = max(__syncthreads_count(in), 1);
+    int stay = min(left, n);
+    if (by_mass) {   // token j > 0 stays while what lies in front of it is below the goal; the sums rise with j
+      int lo = 1, hi = max(n, 1);
+      while (lo < hi) {
+        const int j = (lo + hi) >> 1;
+        if (before + (above + (sh.upto[first + j - 1] - front)) < goal) lo = j + 1;
+        else hi = j;
+      }
+      stay = lo;
+    }
+    stay = max(stay, 1);
     const uint32_t end = (uint32_t)(sh.order[first + stay - 1] >> 32);
-    const int ties = __syncthreads_count((tid < stay) & ((uint32_t)(sh.order[first + min(tid, stay - 1)] >> 32) == end));
-    return Cut{bin, ~end, (uint32_t)ties, above + (sh.upto[first + stay - 1] - front)};
+    int lo = 0, hi = stay - 1;   // the first of the tokens that equal the last
+    while (lo < hi) {
+      const int j = (lo + hi) >> 1;
+      if ((uint32_t)(sh.order[first + j] >> 32) == end) hi = j;
+      else lo = j + 1;
+    }
+    return Cut{bin, ~end, (uint32_t)(stay - lo), above + (sh.upto[first + stay - 1] - front)};
   }
 
   // Where the count `want`, or the mass `goal` of which `before` lies in front
@@ -854,6 +895,7 @@ __global__ __launch_bounds__(kPickThreads) void sample_pick_kernel(SampleArgs a)
   const Row<T> r(a, row);
   const Scale s(q.to_octaves, top);
   fill_exp2(sh.table, tid);
+  if (tid == 0) sh.taken = 0;
   read_tally<kPickThreads>(a, s, row, tid, share, sh.tally);
   const LaneBins bins(sh.tally, lane);
   const Range g = find_range(a, q, s, bins, lane);
@@ -895,12 +937,16 @@ __global__ __launch_bounds__(kPickThreads) void sample_pick_kernel(SampleArgs a)
   auto stays = [&](float v, double y) -> int { return y >= min_y ? (int)(v > last_value) + 2 * (int)(v == last_value) : 0; };
   auto weight = [&](double y) { return exp2_64(y, s.below(y), sh.table); };
 
-  // What stays of every part: the bins in front of the edge, and its own tokens of the edge, a wave per part.
+  // What stays of every part: the bins in front of the edge, and its own tokens of the edge, sixteen lanes per part.
+  static_assert(kPickThreads == 16 * kMaxParts, "sixteen lanes per part");
   const int bits = a.mass_bits + bin_depth(edge) - 1;
   const double unit = ldexp(1.0, bits), per_unit = ldexp(1.0, -bits);
-  uint32_t list_from = 0, list_to = 0;
-  list_places(sh.tally, g, a.parts, lane, list_from, list_to);
-  for (int p = wave; p < a.parts; p += kPickThreads / 64) {
+  {
+    uint32_t from, to;
+    list_places(sh.tally, g, a.parts, lane, from, to);
+    const int p = tid >> 4;
+    from = __shfl(from, p);
+    to = __shfl(to, p);
     unsigned long long m = 0;
     uint32_t ties = 0;
     auto add = [&](float v) {
@@ -910,17 +956,16 @@ __global__ __launch_bounds__(kPickThreads) void sample_pick_kernel(SampleArgs a)
       if (st == 1) m += (unsigned long long)rint(weight(y) * unit);
       ties += st == 2;
     };
-    if (edge < kBins && sh.tally.part_count[p][edge] != 0) {
+    if (p < a.parts && edge < kBins && sh.tally.part_count[p][edge] != 0) {
       if (pick.list != nullptr) {
-        const int to = __builtin_amdgcn_readlane((int)list_to, p);
-        for (int i = __builtin_amdgcn_readlane((int)list_from, p) + lane; i < to; i += 64) {
+        for (uint32_t i = from + (tid & 15); i < to; i += 16) {
           const float2_t e = pick.list[i];
           const float index = e.y;
           if (__builtin_bit_cast(int, index) >= 0) add(e.x);
         }
       } else {
         const int c1 = min((p + 1) * r.per_part, r.chunks);
-        for (int c = p * r.per_part + lane; c < c1; c += 64) {
+        for (int c = p * r.per_part + (tid & 15); c < c1; c += 16) {
           float v[E];
           const uint32_t in = r.load(c, v);
 #pragma unroll
@@ -928,13 +973,13 @@ __global__ __launch_bounds__(kPickThreads) void sample_pick_kernel(SampleArgs a)
             if ((in >> e) & 1) add(v[e]);
         }
       }
-#pragma unroll
-      for (int o = 32; o > 0; o >>= 1) {
-        m += __shfl_xor(m, o);
-        ties += __shfl_xor(ties, o);
-      }
     }
-    if (lane == 0) {
+#pragma unroll
+    for (int o = 8; o > 0; o >>= 1) {
+      m += __shfl_xor(m, o);
+      ties += __shfl_xor(ties, o);
+    }
+    if ((tid & 15) == 0) {
       sh.part_edge[p] = m;
       sh.part_ties[p] = ties;
     }
@@ -1121,17 +1166,26 @@ int sample_check(int64_t rows, int64_t vocab) {
   return WQ_OK;
 }
 
-template <typename T>
+// Waves per part: all four of a workgroup while that leaves at most four
+// workgroups per compute unit.
+int sample_waves(const SampleArgs& a) { return (int64_t)a.parts * a.rows <= 1024 ? 4 : 1; }
+
+template <typename T, int W>
 int launch_sample(const SampleArgs& a, hipStream_t s) {
-  const dim3 grid((unsigned)((a.parts + 3) / 4), (unsigned)a.rows);
-  hipLaunchKernelGGL(sample_tally_kernel<T>, grid, dim3(256), 0, s, a);
+  const dim3 grid((unsigned)((a.parts * W + 3) / 4), (unsigned)a.rows);
+  hipLaunchKernelGGL((sample_tally_kernel<T, W>), grid, dim3(256), 0, s, a);
   int rc = check_launch("sample_tally");
   if (rc != WQ_OK) return rc;
-  hipLaunchKernelGGL(sample_gather_kernel<T>, grid, dim3(256), 0, s, a);
+  hipLaunchKernelGGL((sample_gather_kernel<T, W>), grid, dim3(256), 0, s, a);
   rc = check_launch("sample_gather");
   if (rc != WQ_OK) return rc;
   hipLaunchKernelGGL(sample_pick_kernel<T>, dim3((unsigned)a.rows), dim3(kPickThreads), 0, s, a);
   return check_launch("sample_pick");
+}
+
+template <typename T>
+int launch_sample(const SampleArgs& a, hipStream_t s) {
+  return sample_waves(a) == 4 ? launch_sample<T, 4>(a, s) : launch_sample<T, 1>(a, s);
 }
 
 }  // namespace

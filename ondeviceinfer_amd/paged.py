@@ -11,11 +11,15 @@ drafted tokens side by side.
 """
 from __future__ import annotations
 
-from typing import NamedTuple
+from dataclasses import dataclass
+from typing import NamedTuple, Sequence
 
+import torch
 from torch import Tensor
 
 from . import _native
+
+MAX_TREE_TOKENS = 64   # drafted tokens of one sequence in one step: one bit of the mask each
 
 
 class PagedBatch(NamedTuple):
@@ -63,3 +67,146 @@ def paged_attention(query: Tensor, key_pages: Tensor, value_pages: Tensor, batch
     behind the last sequence keep what ``out`` held."""
     return _native.paged_attention(query, key_pages, value_pages, batch.page_table, batch.query_starts, batch.seq_lens,
                                    scale, tree_mask, out, workspace)
+
+
+def tree_layout(parents: Sequence[int]) -> tuple[list[int], list[int]]:
+    """``(masks, depths)`` of a tree of drafted tokens: token ``i`` follows token
+    ``parents[i] < i``, or the cached tokens where that is -1.  A mask has the
+    bits of the token's ancestors and its own; the depth of a token that follows
+    the cached ones is 0."""
+    if len(parents) > MAX_TREE_TOKENS:
+        raise ValueError(f'at most {MAX_TREE_TOKENS} drafted tokens per sequence, got {len(parents)}')
+    masks, depths = [], []
+    for i, parent in enumerate(parents):
+        if not -1 <= parent < i:
+            raise ValueError(f'parent of token {i} must be -1 or an earlier token, got {parent}')
+        masks.append((masks[parent] if parent >= 0 else 0) | (1 << i))
+        depths.append(depths[parent] + 1 if parent >= 0 else 0)
+    return masks, depths
+
+
+class PagedKVCache:
+    """The keys and values of all layers in one pool of pages,
+    ``[2, layers, pages, kv_heads, page_size, head_dim]`` (K then V), shared by
+    any number of sequences.
+
+    A sequence is an integer handed out by ``add``; its pages are taken from
+    the pool as it grows and given back by ``truncate`` and ``free``.  The
+    bookkeeping is the host's; a step's ``PagedBatch`` carries it to the
+    device."""
+
+    def __init__(self, *, num_layers: int, num_pages: int, num_key_value_heads: int, head_dim: int,
+                 device: torch.device | str, dtype: torch.dtype = torch.float16, page_size: int = 16) -> None:
+        if num_pages <= 0:
+            raise ValueError(f'num_pages must be positive, got {num_pages}')
+        if page_size <= 0 or page_size % 16:
+            raise ValueError(f'page_size must be a positive multiple of 16, got {page_size}')
+        self.page_size, self.num_pages, self.device = page_size, num_pages, torch.device(device)
+        self._block = torch.empty((2, num_layers, num_pages, num_key_value_heads, page_size, head_dim), device=device,
+                                  dtype=dtype)
+        self.key_pages = list(self._block[0].unbind(0))
+        self.value_pages = list(self._block[1].unbind(0))
+        self._free = list(range(num_pages - 1, -1, -1))
+        self._pages: dict[int, list[int]] = {}
+        self._lengths: dict[int, int] = {}
+        self._next = 0
+
+    @property
+    def free_pages(self) -> int:
+        return len(self._free)
+
+    @property
+    def storage_bytes(self) -> int:
+        return self._block.numel() * self._block.element_size()
+
+    def add(self) -> int:
+        """A new, empty sequence."""
+        seq = self._next
+        self._next += 1
+        self._pages[seq], self._lengths[seq] = [], 0
+        return seq
+
+    def length(self, seq: int) -> int:
+        return self._lengths[seq]
+
+    def free(self, seq: int) -> None:
+        """Forget a sequence; its pages go back to the pool."""
+        self._free.extend(reversed(self._pages.pop(seq)))
+        del self._lengths[seq]
+
+    def truncate(self, seq: int, length: int) -> None:
+        """Forget a sequence's positions from ``length`` on."""
+        if not 0 <= length <= self._lengths[seq]:
+            raise ValueError(f'sequence {seq} has {self._lengths[seq]} positions, cannot keep {length}')
+        pages = self._pages[seq]
+        while len(pages) * self.page_size >= length + self.page_size:
+            self._free.append(pages.pop())
+        self._lengths[seq] = length
+
+    def extend(self, sequences: Sequence[int], counts: Sequence[int]) -> PagedBatch:
+        """Room for ``counts[i]`` new tokens of ``sequences[i]``, and the batch
+        that a step over them takes.  Raises before anything changes when the
+        pool has too few pages."""
+        if len(sequences) != len(counts) or len(set(sequences)) != len(sequences):
+            raise ValueError('a step takes each of its sequences once, with a count each')
+        if any(n < 0 for n in counts):
+            raise ValueError('counts must not be negative')
+        lens = [self._lengths[s] + n for s, n in zip(sequences, counts)]
+        want = [-(-n // self.page_size) - len(self._pages[s]) for s, n in zip(sequences, lens)]
+        if sum(want) > len(self._free):
+            raise ValueError(f'KV cache capacity exceeded: {sum(want)} more pages needed, {len(self._free)} free')
+        for s, n, more in zip(sequences, lens, want):
+            self._pages[s].extend(self._free.pop() for _ in range(more))
+            self._lengths[s] = n
+        width = max([1, *(len(self._pages[s]) for s in sequences)])
+        rows = [self._pages[s] + [-1] * (width - len(self._pages[s])) for s in sequences]
+        starts = [0]
+        for n in counts:
+            starts.append(starts[-1] + n)
+        # One copy to the device for all three.
+        flat = torch.tensor([x for row in rows for x in row] + starts + lens, dtype=torch.int32).to(self.device)
+        table = len(rows) * width
+        return PagedBatch(flat[:table].view(len(rows), width), flat[table:table + len(starts)],
+                          flat[table + len(starts):])
+
+    def keep(self, seq: int, start: int, accepted: Sequence[int]) -> None:
+        """Of the tokens from position ``start`` on (a step's drafted ones) keep
+        those ``accepted`` (indices from ``start``, ascending), moved up to
+        follow it without gaps, in all layers; forget the others."""
+        length = self._lengths[seq]
+        if any(b <= a for a, b in zip(accepted, accepted[1:])):
+            raise ValueError('accepted tokens must be in ascending order')
+        if not 0 <= start <= length or (accepted and not (0 <= accepted[0] and start + accepted[-1] < length)):
+            raise ValueError(f'accepted tokens must lie in the positions {start} .. {length - 1} of sequence {seq}')
+        pages, size = self._pages[seq], self.page_size
+        moves = [(start + j, start + i) for i, j in enumerate(accepted) if i != j]
+        if moves:
+            index = torch.tensor([(pages[a // size], a % size, pages[b // size], b % size) for a, b in moves]).to(
+                self.device)
+            from_page, from_row, to_page, to_row = index.unbind(1)
+            # The rows are read before any is written.
+            self._block[:, :, to_page, :, to_row] = self._block[:, :, from_page, :, from_row]
+        self.truncate(seq, start + len(accepted))
+
+
+@dataclass
+class PagedStep:
+    """One forward step over a paged cache: the new tokens of its sequences,
+    handed to the decoder layers in the place of a cache."""
+
+    cache: PagedKVCache
+    batch: PagedBatch
+    cos_table: Tensor
+    sin_table: Tensor
+    scale: float
+    positions: Tensor | None = None
+    tree_mask: Tensor | None = None
+
+    def attend(self, layer_idx: int, qkv: Tensor, q_heads: int, q_norm: Tensor | None, k_norm: Tensor | None,
+               eps: float) -> Tensor:
+        """``[tokens, q_heads, head_dim]`` attention output of the fused
+        projection's rows, their keys and values appended to the layer's pages."""
+        keys, values = self.cache.key_pages[layer_idx], self.cache.value_pages[layer_idx]
+        query = paged_append(qkv, keys, values, self.batch, q_heads=q_heads, q_norm=q_norm, k_norm=k_norm, eps=eps,
+                             cos_table=self.cos_table, sin_table=self.sin_table, positions=self.positions)
+        return paged_attention(query, keys, values, self.batch, scale=self.scale, tree_mask=self.tree_mask)

@@ -102,6 +102,7 @@ from .attention import cached_scaled_dot_product_attention  # noqa: E402
 from .cache import KVCache, ResidentKVCache, kv_block  # noqa: E402
 from .functional import add_rms_norm, rms_norm  # noqa: E402
 from .layers import RotaryEmbedding, apply_rotary_pos_emb  # noqa: E402
+from .paged import PagedKVCache, PagedStep, tree_layout  # noqa: E402
 
 QKV_FUSED = 'self_attn.qkv_proj.weight'
 GATE_UP_FUSED = 'mlp.gate_up_proj.weight'
@@ -179,7 +180,10 @@ def quantized_decoder_layer_forward(hidden_states: Tensor, weights: Mapping[str,
     in the gate_up and down GEMMs' epilogues.  INT8 layers bound for the
     decode graph run their fused q|k|v and gate|up W8A16 weights the same way.  With a resident batch-1 cache the q/k norms, RoPE and
     cache append run as one HIP kernel and the causal attention as another
-    (``wq_prefill_attention``, reading the cache rows in place).
+    (``wq_prefill_attention``, reading the cache rows in place).  A
+    ``PagedStep`` as the cache makes ``hidden_states`` ``[1, tokens, hidden]``
+    the new tokens of many sequences (``wq_paged_append``,
+    ``wq_paged_attention``; ``cos`` and ``sin`` are the step's own).
     """
     def linear(inputs, name):
         if linear_backend is not None:
@@ -196,7 +200,13 @@ def quantized_decoder_layer_forward(hidden_states: Tensor, weights: Mapping[str,
         qkv = linear(states, QKV_FUSED)
     elif linear_backend is None:
         qkv = _int8_fused_linear(states, weights, QKV_FUSED, 3, stats)
-    if (qkv is not None and batch_size == 1 and d == 128 and qkv.is_cuda and qkv.dtype == torch.float16
+    if isinstance(cache, PagedStep):
+        if qkv is None:
+            qkv = torch.cat([linear(states, f'self_attn.{p}_proj.weight') for p in 'qkv'], dim=-1)
+        attention_output = cache.attend(
+            layer_idx, qkv.reshape(query_length, -1), hq, weights['self_attn.q_norm.weight'],
+            weights['self_attn.k_norm.weight'], eps).transpose(0, 1).unsqueeze(0)
+    elif (qkv is not None and batch_size == 1 and d == 128 and qkv.is_cuda and qkv.dtype == torch.float16
             and isinstance(cache, ResidentKVCache) and cache.batch_size == 1
             and cos.dtype == torch.float16 and tuple(cos.shape) == (1, query_length, d)):
         # Resident batch-1 cache: q/k norm, RoPE and the cache append in one
@@ -653,6 +663,93 @@ class QuantizedQwen3ForCausalLM:
         cache._decode_graph = entry['graph']
         return cache
 
+    def make_paged_cache(self, *, num_pages: int, page_size: int = 16) -> PagedKVCache:
+        """A pool of pages for this model's layers (``forward_paged``)."""
+        cfg = self.config
+        return PagedKVCache(num_layers=cfg.num_hidden_layers, num_pages=num_pages, page_size=page_size,
+                            num_key_value_heads=cfg.num_key_value_heads, head_dim=cfg.head_dim, device=self.device,
+                            dtype=self.dtype)
+
+    def _rope_tables(self, positions: int) -> tuple[Tensor, Tensor]:
+        """cos / sin rows for at least ``positions`` positions, kept and doubled as sequences grow."""
+        tables = getattr(self, '_rope', None)
+        if tables is None or tables[0].shape[0] < positions:
+            rows = 1024
+            while rows < positions:
+                rows *= 2
+            tables = self._rope = self.rotary_emb.table(rows, self.device, self.dtype)
+        return tables
+
+    @torch.inference_mode()
+    def forward_paged(self, input_ids: Tensor, cache: PagedKVCache, sequences, counts, *, tree_parents=None,
+                      all_logits: bool = False) -> CausalLMOutput:
+        """One step of many sequences over a paged cache.
+
+        ``input_ids`` int64 ``[sum(counts)]``, the ``counts[i]`` new tokens of
+        ``sequences[i]`` one after another (single tokens, prompts or chunks of
+        prompts, in any mix); the logits come back as ``[sequences, vocab]`` of
+        each one's last token, or with ``all_logits`` of all tokens.  With
+        ``tree_parents`` (per sequence the list ``tree_layout`` takes) the new
+        tokens are drafted ones that form a tree behind the sequence's
+        positions, at most 64 each; ``PagedKVCache.keep`` then drops the
+        rejected ones."""
+        if input_ids.dim() != 1 or input_ids.shape[0] != sum(counts):
+            raise ValueError(f'input_ids must be [{sum(counts)}], got shape {tuple(input_ids.shape)}')
+        if not all_logits and any(n <= 0 for n in counts):
+            raise ValueError('a sequence without new tokens has no last token')
+        if input_ids.shape[0] == 0:
+            raise ValueError('a step needs at least one token')
+        cfg = self.config
+        past = [cache.length(s) for s in sequences]
+        positions = tree_mask = None
+        if tree_parents is not None:
+            if [len(p) for p in tree_parents] != list(counts):
+                raise ValueError('tree_parents must name a parent for every new token')
+            layouts = [tree_layout(p) for p in tree_parents]
+            masks = [m - (1 << 64) if m >> 63 else m for masks, _ in layouts for m in masks]
+            depths = [n + d for n, (_, depths) in zip(past, layouts) for d in depths]
+            tree_mask = torch.tensor(masks, dtype=torch.int64).to(self.device)
+            positions = torch.tensor(depths, dtype=torch.int32).to(self.device)
+        batch = cache.extend(sequences, counts)
+        try:
+            hidden_states = self._paged_layers(input_ids, PagedStep(
+                cache, batch, *self._rope_tables(max(n + c for n, c in zip(past, counts))),
+                1.0 / float(cfg.head_dim) ** 0.5, positions, tree_mask))
+        except BaseException:
+            for seq, n in zip(sequences, past):   # the step's positions hold nothing
+                cache.truncate(seq, n)
+            raise
+        hidden_states = hidden_states[0]
+        if not all_logits and len(counts) < hidden_states.shape[0]:
+            hidden_states = hidden_states[batch.query_starts[1:].long() - 1]
+        hidden_states = rms_norm(hidden_states.contiguous(), self.final_norm, cfg.rms_norm_eps)
+        return CausalLMOutput(logits=self._logits(hidden_states), cache=cache)
+
+    def _paged_layers(self, input_ids: Tensor, step: PagedStep) -> Tensor:
+        """The decoder layers over a step's tokens, ``[1, tokens, hidden]``."""
+        hidden_states = _native.embed_rows(self.embedding_table(), input_ids.to(self.device).contiguous()).unsqueeze(0)
+        self.runtime.begin_forward()
+        for layer_idx in range(self.config.num_hidden_layers):
+            hidden_states = quantized_decoder_layer_forward(
+                hidden_states, self.runtime.weights_for(layer_idx), self.config, layer_idx, step.cos_table,
+                step.sin_table, self._forward_scratch, cache=step, stats=self.compute_stats,
+                linear_backend=self.linear_backend)
+            if self.layer_probe_callback is not None:
+                self.layer_probe_callback(layer_idx, hidden_states)
+            self.runtime.after_layer(layer_idx)
+        self.runtime.end_forward()
+        return hidden_states
+
+    def _logits(self, hidden_states: Tensor) -> Tensor:
+        """The LM head over normalized rows ``[..., hidden]``."""
+        if self.lm_head_w4 is None:
+            return F.linear(hidden_states, self.lm_head)
+        p = self.lm_head_w4
+        flat = hidden_states.reshape(-1, p.k).contiguous()
+        logits = _native.w4a16_linear(flat, p.tiles, p.meta, p.n, p.group_size,
+                                      workspace=p.workspace if flat.shape[0] <= 4 else None)
+        return logits.view(*hidden_states.shape[:-1], p.n)
+
     @torch.inference_mode()
     def __call__(self, input_ids: Tensor, *, cache: KVCache | None = None, position_ids: Tensor | None = None,
                  logits_to_keep: int = 0, **_: object) -> CausalLMOutput:
@@ -704,12 +801,4 @@ class QuantizedQwen3ForCausalLM:
         if logits_to_keep > 0:
             hidden_states = hidden_states[:, -logits_to_keep:, :].contiguous()
         hidden_states = rms_norm(hidden_states, self.final_norm, self.config.rms_norm_eps)
-        if self.lm_head_w4 is not None:
-            p = self.lm_head_w4
-            flat = hidden_states.reshape(-1, p.k).contiguous()
-            logits = _native.w4a16_linear(flat, p.tiles, p.meta, p.n, p.group_size,
-                                          workspace=p.workspace if flat.shape[0] <= 4 else None)
-            logits = logits.view(*hidden_states.shape[:-1], p.n)
-        else:
-            logits = F.linear(hidden_states, self.lm_head)
-        return CausalLMOutput(logits=logits, cache=cache)
+        return CausalLMOutput(logits=self._logits(hidden_states), cache=cache)

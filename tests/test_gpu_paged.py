@@ -338,3 +338,110 @@ def test_append_takes_given_positions(gpu):
     for t, at in enumerate((30, 31, 31, 32)):
         want = expected_rows(qkv[t].view(4, D)[:2], None, cos[at], sin[at], 1e-6)
         assert (got[t].double() - want).abs().max() <= want.abs().max() * HALF_ULP + 1e-5
+
+
+# ----------------------------------------------------------------------------- graphs, streams
+
+def decode_inputs(pool, seed):
+    gen = torch.Generator().manual_seed(seed)
+    return (2 * torch.randn(pool.tokens, (pool.hq + 2 * pool.hkv) * D, generator=gen)).half()
+
+
+def decode_step(qkv, k, v, batch, cos, sin, hq, scale):
+    q = paged_append(qkv, k, v, batch, q_heads=hq, q_norm=None, k_norm=None, eps=1e-6, cos_table=cos, sin_table=sin)
+    return q, paged_attention(q, k, v, batch, scale=scale)
+
+
+@pytest.mark.parametrize('long', [False, True])
+def test_captured_steps_follow_the_lengths(gpu, long):
+    """One graph of a decode step, replayed while the sequences grow (by the graph itself): every replay equals the
+    eager step on a copy; two graphs of the same shapes replayed in turn on two streams do not disturb each other."""
+    past = [2000, 40, 700] if long else [20, 40, 7]
+    scale = 1.0 / math.sqrt(D)
+    cos, sin = (t.to(gpu) for t in tables(4096))
+
+    def world(seed):
+        pool = Pool([1, 1, 1], [p + 8 for p in past], hq=10, hkv=2, page=16, seed=seed)
+        k, v, batch = pool.to(gpu)
+        k.nan_to_num_(0.5)
+        v.nan_to_num_(0.5)
+        batch.seq_lens.copy_(torch.tensor([p + 1 for p in past], dtype=torch.int32))
+        return pool, k, v, batch, torch.zeros(3, 14 * D, dtype=torch.float16, device=gpu)
+
+    worlds = [world(1), world(2)]
+    graphs = []
+    for pool, k, v, batch, qkv in worlds:
+        decode_step(qkv, k, v, batch, cos, sin, 10, scale)        # before the capture, on the same rows
+        torch.cuda.synchronize()
+        graph = torch.cuda.CUDAGraph()
+        with torch.cuda.graph(graph):
+            outs = decode_step(qkv, k, v, batch, cos, sin, 10, scale)
+            batch.seq_lens.add_(1)
+        batch.seq_lens.copy_(torch.tensor([p + 1 for p in past], dtype=torch.int32))
+        graphs.append((graph, outs))
+    eager = [(k.clone(), v.clone(), PagedBatch(*(t.clone() for t in batch))) for _, k, v, batch, _ in worlds]
+    streams = [torch.cuda.Stream(), torch.cuda.Stream()]
+    for turn in range(5):
+        want = []
+        for w, (pool, k, v, batch, qkv) in enumerate(worlds):
+            x = decode_inputs(pool, 10 * turn + w).to(gpu)
+            qkv.copy_(x)
+            ek, ev, eb = eager[w]
+            want.append(decode_step(x, ek, ev, eb, cos, sin, 10, scale))
+            eb.seq_lens.add_(1)
+        torch.cuda.synchronize()
+        for (graph, _), stream in zip(graphs, streams):
+            with torch.cuda.stream(stream):
+                graph.replay()
+        torch.cuda.synchronize()
+        for w, (_, outs) in enumerate(graphs):
+            for got, ref in zip(outs, want[w]):
+                assert torch.equal(got, ref), (turn, w)
+            assert torch.equal(worlds[w][1], eager[w][0]) and torch.equal(worlds[w][2], eager[w][1])
+
+
+def test_calls_on_two_streams_at_once(gpu):
+    """The same shapes on two streams without a workspace of one's own: each call has its own partials."""
+    worlds = []
+    for seed in (3, 4):
+        pool = Pool([1] * 4, [1500, 900, 2200, 30], hq=10, hkv=2, page=16, seed=seed)
+        k, v, batch = pool.to(gpu)
+        worlds.append((pool.rand(4, 10, D).to(gpu), k, v, batch))
+    want = [paged_attention(q, k, v, b, scale=0.1).clone() for q, k, v, b in worlds]
+    torch.cuda.synchronize()
+    streams = [torch.cuda.Stream(), torch.cuda.Stream()]
+    got = [[], []]
+    for _ in range(20):
+        for i, (q, k, v, b) in enumerate(worlds):
+            with torch.cuda.stream(streams[i]):
+                got[i].append(paged_attention(q, k, v, b, scale=0.1))
+    torch.cuda.synchronize()
+    for i in range(2):
+        assert all(torch.equal(g, want[i]) for g in got[i])
+
+
+def test_refusals(gpu):
+    pool = Pool([1, 1], [20, 30], hq=4, hkv=2, page=16, seed=5)
+    k, v, batch = pool.to(gpu)
+    q = pool.rand(2, 4, D).to(gpu)
+    bad = [
+        (TypeError, dict(query=q.float())), (ValueError, dict(query=q[0])), (ValueError, dict(query=q[:, :, :64])),
+        (ValueError, dict(query=q.transpose(0, 1))), (TypeError, dict(key_pages=k.float())),
+        (ValueError, dict(value_pages=v[:-1])), (ValueError, dict(key_pages=k.transpose(1, 2))),
+        (ValueError, dict(key_pages=k[:1].expand(k.shape))), (ValueError, dict(scale=0.0)),
+        (ValueError, dict(scale=float('nan'))), (TypeError, dict(tree_mask=torch.zeros(2, device=gpu))),
+        (ValueError, dict(tree_mask=torch.zeros(3, dtype=torch.int64, device=gpu))),
+        (ValueError, dict(out=torch.empty(2, 4, 64, dtype=torch.float16, device=gpu))),
+        (TypeError, dict(batch=batch._replace(page_table=batch.page_table.long()))),
+        (ValueError, dict(batch=batch._replace(page_table=batch.page_table[:1]))),
+        (ValueError, dict(batch=batch._replace(query_starts=batch.query_starts[:2]))),
+        (ValueError, dict(batch=batch._replace(seq_lens=batch.seq_lens.cpu()))),
+    ]
+    good = dict(query=q, key_pages=k, value_pages=v, batch=batch, scale=0.1)
+    for error, change in bad:
+        with pytest.raises(error):
+            paged_attention(**{**good, **change})
+    long = batch._replace(page_table=torch.zeros(2, 300, dtype=torch.int32, device=gpu))
+    with pytest.raises(ValueError, match='workspace'):
+        paged_attention(**{**good, 'batch': long}, workspace=torch.empty(16, dtype=torch.uint8, device=gpu))
+    assert paged_attention(**{**good, 'query': q[:0], 'batch': batch._replace(query_starts=batch.query_starts * 0)}).shape == (0, 4, D)

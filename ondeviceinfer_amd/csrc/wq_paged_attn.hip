@@ -152,6 +152,20 @@ __device__ __forceinline__ Groups load_groups(const PagedArgs& a, int b, int fir
   return g;
 }
 
+// A hidden position's probability is 0, and 0 times a value that is infinite or
+// NaN is NaN.  Where a step of keys may hide some of them, such values are
+// taken as 0 and their positions' scores as NaN (before the hidden ones are
+// set to -inf): a row that attends one becomes NaN, the others do not see it.
+__device__ __forceinline__ bool any_not_finite(uint4_t v) {
+  bool any = false;
+#pragma unroll
+  for (int w = 0; w < 4; ++w) {
+    const uint32_t u = v[w];
+    any |= ((u & 0x7c00u) == 0x7c00u) | ((u & 0x7c000000u) == 0x7c000000u);
+  }
+  return any;
+}
+
 // What a row may attend of its sequence's positions.  Bit operations only, no
 // branches: of the short-circuit form (key < keys && (tree ? ... : ...)) inside
 // the unrolled score loops hipcc 7.2 loses the assignment of the hidden lanes.
@@ -278,6 +292,16 @@ __global__ __launch_bounds__(256, 2) void paged_attention_rows_kernel(PagedArgs 
       }
       if (more) load_keys(blk + 1);
       if (k0 + kKeys > ragged || k0 + kKeys > keys) {
+        // Lane (i, kb) looks at its eight values of the keys whose scores the lanes (.., kb) hold.
+#pragma unroll
+        for (int e = 0; e < 8; ++e) {
+          const bool odd = any_not_finite(vr[e]);
+          const uint64_t lanes = __builtin_amdgcn_ballot_w64(odd);
+          if (lanes != 0) {
+            if (odd) vr[e] = uint4_t{0u, 0u, 0u, 0u};
+            if ((lanes >> (16 * kb)) & 0xffffu) sc[e >> 2][e & 3] = NAN;
+          }
+        }
 #pragma unroll
         for (int h = 0; h < 2; ++h)
 #pragma unroll
@@ -409,6 +433,8 @@ __device__ __forceinline__ float max_halves(float v) {
 __global__ __launch_bounds__(256, 2) void paged_attention_tile_kernel(PagedArgs a) {
   constexpr int R = kTileRows, D = kPagedDim;
   extern __shared__ __attribute__((aligned(16))) uint8_t smem[];
+  // Per stage, for the keys 4 g + e: bit g of word e, and one such set from each wave that stored values.
+  __shared__ uint32_t odd_keys[2][4][4];
   const int tid = threadIdx.x, lane = tid & 63;
   const int wave = __builtin_amdgcn_readfirstlane(tid >> 6);
   const int ql = lane & 31, hh = lane >> 5;
@@ -431,6 +457,7 @@ __global__ __launch_bounds__(256, 2) void paged_attention_tile_kernel(PagedArgs 
   const int wave_keys = r0 < rows ? keys_of(r0 + 31) : 0;
   const int ragged = tree ? p.s.base : p.s.base + min(r0, rows - 1) / a.G + 1;   // first key that not all its rows attend
   const Sight hidden = row_sight(a, p.s, tok, keys);
+  const int tile_ragged = min(keys, tree ? p.s.base : p.s.base + p.tile * R / a.G + 1);
   // Chunks are cut in steps of kKeys; here a step is two of those.
   const int blocks = (p.s.blocks + 1) >> 1;
   const int per = blocks / p.chunks, extra = blocks % p.chunks;
@@ -489,6 +516,15 @@ __global__ __launch_bounds__(256, 2) void paged_attention_tile_kernel(PagedArgs 
         for (int e = 0; e < 4; ++e)
           if (kb * kTileKeys + 4 * (tid & 15) + e >= keys) vr[e] = uint4_t{0u, 0u, 0u, 0u};
       }
+      if (kb * kTileKeys + kTileKeys > tile_ragged) {
+#pragma unroll
+        for (int e = 0; e < 4; ++e) {
+          const bool odd = any_not_finite(vr[e]);
+          const uint64_t lanes = __builtin_amdgcn_ballot_w64(odd);   // lane 16 c + g: key 4 g + e
+          if (odd) vr[e] = uint4_t{0u, 0u, 0u, 0u};
+          if (lane == 0) odd_keys[st][wave][e] = (uint32_t)(lanes | lanes >> 16 | lanes >> 32 | lanes >> 48) & 0xffffu;
+        }
+      }
       uint8_t* base = smem + st * kTileStage;
 #pragma unroll
       for (int u = 0; u < 4; ++u) {
@@ -508,7 +544,7 @@ __global__ __launch_bounds__(256, 2) void paged_attention_tile_kernel(PagedArgs 
         *reinterpret_cast<uint2_t*>(base + kTileKBytes + (d0 + dd) * kVRow + 2 * pos) = w;
       }
     };
-    auto step = [&](const uint8_t* base, int k0, bool masked) {
+    auto step = [&](const uint8_t* base, int st, int k0, bool masked) {
       float16_t sc[2];
 #pragma unroll
       for (int kt = 0; kt < 2; ++kt) {
@@ -535,6 +571,20 @@ __global__ __launch_bounds__(256, 2) void paged_attention_tile_kernel(PagedArgs 
 #pragma unroll
           for (int e = 0; e < 16; ++e)
             if ((bad >> (2 * kt + (e >> 3))) & 1) sc[kt][e] = NAN;
+      }
+      if (k0 + kTileKeys > tile_ragged) {
+        uint32_t odd[4];
+#pragma unroll
+        for (int e = 0; e < 4; ++e)
+          odd[e] = __builtin_amdgcn_readfirstlane(odd_keys[st][0][e] | odd_keys[st][1][e] | odd_keys[st][2][e] |
+                                                  odd_keys[st][3][e]);
+        if (odd[0] | odd[1] | odd[2] | odd[3]) {
+#pragma unroll
+          for (int kt = 0; kt < 2; ++kt)
+#pragma unroll
+            for (int e = 0; e < 16; ++e)
+              sc[kt][e] = (odd[e & 3] >> (8 * kt + 2 * (e >> 2) + hh)) & 1 ? NAN : sc[kt][e];
+        }
       }
       if (masked) {
 #pragma unroll
@@ -615,7 +665,7 @@ __global__ __launch_bounds__(256, 2) void paged_attention_tile_kernel(PagedArgs 
       const bool more = kb + 1 < c1;
       if (more) load_block(kb + 1);
       const int k0 = kb * kTileKeys;
-      if (k0 < wave_keys) step(smem + st * kTileStage, k0, k0 + kTileKeys > ragged || k0 + kTileKeys > keys);
+      if (k0 < wave_keys) step(smem + st * kTileStage, st, k0, k0 + kTileKeys > ragged || k0 + kTileKeys > keys);
       if (more) store_block(st ^ 1, kb + 1);   // that stage was last read before the previous barrier
       bad = bad_next;
       __syncthreads();

@@ -225,6 +225,47 @@ def test_positions_without_a_page_give_nan(gpu):
     check(paged_attention(query.to(gpu), k, v, PagedBatch(table, batch.query_starts, batch.seq_lens), scale=0.1), want, tol)
 
 
+@pytest.mark.parametrize('tree', [False, True])
+@pytest.mark.parametrize('count', [6, 60])          # small tiles, large tiles
+@pytest.mark.parametrize('what', [float('nan'), float('inf'), -float('inf')])
+def test_what_is_not_attended_has_no_influence(gpu, what, count, tree):
+    """Infinite and NaN keys and values of a later token, or of another branch, beside rows that do not attend it."""
+    pool = Pool([count, 1], [75, 40], hq=8, hkv=2, page=16, seed=count)
+    query = pool.rand(count + 1, 8, D)
+    masks = [(1 << i) | ((1 << min(i, 4)) - 1) for i in range(count)] + [1] if tree else None   # 0 .. 3, then leaves
+    want, tol = expected_attention(pool, query, 0.1, masks)
+    clean = [t for t in range(count + 1) if t == count or (t != 5 if tree else t < 5)]
+    for at, page_row in ((5, 80),):                       # token 5 of sequence 0 is its position 80
+        slot = pool.table[0, page_row // 16].item()
+        pool.v[slot, 1, page_row % 16, 17] = what
+        pool.k[slot, 0, page_row % 16, 3] = what
+        pool.v[slot, 0, page_row % 16, 100] = what
+    k, v, batch = pool.to(gpu)
+    mask = None if masks is None else torch.tensor([signed(m) for m in masks], dtype=torch.int64, device=gpu)
+    got = paged_attention(query.to(gpu), k, v, batch, scale=0.1, tree_mask=mask)
+    check(got[clean], want[clean], tol[clean])
+    attended = [5] if tree else list(range(5, count))
+    assert not torch.isfinite(got[attended][:, 4:, 17]).any() and not torch.isfinite(got[attended][:, :4, 100]).any()
+
+
+def test_large_tiles_with_bad_pages_and_empty_rows(gpu):
+    """As the single tokens': a page outside the pool, a length past the table, lengths below the new tokens."""
+    new, past = [60, 50, 40, 45], [40, 100, 30, -44]
+    pool = Pool(new, past, hq=8, hkv=2, page=16, seed=9, extra_width=0)
+    query = pool.rand(195, 8, D)
+    want, tol = expected_attention(pool, query, 0.1)
+    k, v, batch = pool.to(gpu)
+    table, lens = batch.page_table.clone(), batch.seq_lens.clone()
+    table[0, 4] = k.shape[0] + 5            # positions 64 .. 79 of 100: tokens 24 .. of sequence 0
+    table[1, 2] = -3                        # cached positions
+    lens[2] = 16 * table.shape[1] + 20      # the last 20 of 40 tokens lie past the table
+    got = paged_attention(query.to(gpu), k, v, PagedBatch(table, batch.query_starts, lens), scale=0.1)
+    assert torch.isnan(got[24:60]).all() and torch.isnan(got[60:110]).all() and torch.isnan(got[110 + 20:150]).all()
+    check(got[:24], want[:24], tol[:24])
+    assert (got[150:194] == 0).all()        # 45 new tokens, one position
+    check(got[150:], want[150:], tol[150:])
+
+
 def test_starts_out_of_order_touch_only_their_sequence(gpu):
     pool = Pool([2, 3, 1], [20, 30, 40], hq=4, hkv=2, page=16, seed=6)
     query = pool.rand(6, 4, D)

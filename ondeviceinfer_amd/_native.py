@@ -191,6 +191,8 @@ def _require_gpu(*tensors: torch.Tensor | None) -> torch.device:
 
 
 def _check(t: torch.Tensor, dtype: torch.dtype, shape: tuple, name: str) -> None:
+    if t.dtype == dtype and t.shape == shape and t.is_contiguous():   # the usual case first: 0.3 us a tensor
+        return
     if t.dtype != dtype:
         raise TypeError(f'{name}: expected {dtype}, got {t.dtype}')
     if tuple(t.shape) != tuple(shape):

@@ -701,61 +701,81 @@ __global__ __launch_bounds__(256, 2) void paged_attention_tile_kernel(PagedArgs 
     }
 }
 
+// Over the 32 lanes of a half wave.
+__device__ __forceinline__ float half_max(float v) {
+  v = row_max16(v);
+  return fmaxf(v, __shfl_xor(v, 16));
+}
+__device__ __forceinline__ float half_sum(float v) {
+  v = row_sum16(v);
+  return v + __shfl_xor(v, 16);
+}
+
 // The chunks of split tiles joined: grid = (tiles the call can have * KV,
-// parts of R rows), a wave per row and turn, two elements of d per lane.  The
-// weights 2^(m_c - M) of up to 64 chunks are held one per lane and read out as
-// each chunk is added, in chunk order.
+// parts of R rows).  A row and turn takes a wave in small tiles, which have few
+// rows and up to a hundred chunks, and half a wave in large ones, whose many
+// rows of a few chunks are bound by the latency of each (one wave per row: 28
+// us for 82 MB of partials, half a wave: 16).  The weights 2^(m_c - M) of as
+// many chunks as there are lanes are held one per lane and read out as each
+// chunk is added, in chunk order.
 template <int R>
 __global__ __launch_bounds__(256) void paged_attention_merge_kernel(PagedArgs a) {
   constexpr int D = kPagedDim;
   const int lane = threadIdx.x & 63;
-  const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
   const int kvh = blockIdx.x % a.KV;
   const Place p = find_place<R, true>(a, blockIdx.x / a.KV, lane);
   if (!p.found || p.chunks == 1 || p.slot0 + (int64_t)p.s.tiles * p.chunks > a.slots) return;
   const int end = min(R, p.s.count * a.G - p.tile * R);
   const bool refused = a.mask != nullptr && p.s.count > kMaxTreeTokens;
-  for (int row = 4 * blockIdx.y + wave; row < end; row += 4 * gridDim.y) {
+  constexpr int kLanes = R == 16 ? 64 : 32, kRows = 64 / kLanes, E = D / kLanes;   // lanes of a row, rows of a wave
+  typedef float vec_t __attribute__((ext_vector_type(E)));
+  typedef half_t out_t __attribute__((ext_vector_type(E)));
+  const int half = lane / kLanes, l = lane % kLanes;
+  for (int row0 = kRows * (4 * blockIdx.y + (threadIdx.x >> 6)); row0 < end; row0 += 4 * kRows * gridDim.y) {
+    const int row = min(row0 + half, end - 1);   // an odd last row: twice
     auto at = [&](int chunk) { return ((size_t)slot_of(p, p.tile, chunk) * a.KV + kvh) * R + row; };
-    // The first 64 chunks' maxima and sums and the first outputs are requested together.
-    constexpr int kAhead = 16;
-    const int n0 = min(64, p.chunks);
-    float2_t ml = lane < n0 ? a.part_ml[at(lane)] : float2_t{-INFINITY, 0.f};
-    float2_t o[kAhead];
+    // The first chunks' maxima and sums and the first outputs are requested together.
+    constexpr int kAhead = R == 16 ? 16 : 8;
+    const int n0 = min(kLanes, p.chunks);
+    float2_t ml = l < n0 ? a.part_ml[at(l)] : float2_t{-INFINITY, 0.f};
+    vec_t o[kAhead];
     auto load = [&](int c) {
 #pragma unroll
       for (int u = 0; u < kAhead; ++u)
-        o[u] = *reinterpret_cast<const float2_t*>(a.part_o + at(min(c + u, p.chunks - 1)) * D + 2 * lane);
+        o[u] = *reinterpret_cast<const vec_t*>(a.part_o + at(min(c + u, p.chunks - 1)) * D + E * l);
     };
     load(0);
     float M = ml.x;
-    for (int c0 = 64; c0 < p.chunks; c0 += 64)
-      if (c0 + lane < p.chunks) M = fmaxf(M, a.part_ml[at(c0 + lane)].x);
-    M = wave_max_rl(M);
+    for (int c0 = kLanes; c0 < p.chunks; c0 += kLanes)
+      if (c0 + l < p.chunks) M = fmaxf(M, a.part_ml[at(c0 + l)].x);
+    M = kRows == 1 ? wave_max_rl(M) : half_max(M);
     const float Mu = M == -INFINITY ? 0.f : M;
     float den = 0.f;
-    float2_t num = {0.f, 0.f};
-    for (int c0 = 0; c0 < p.chunks; c0 += 64) {
-      const int n = min(64, p.chunks - c0);
-      if (c0 > 0) ml = lane < n ? a.part_ml[at(c0 + lane)] : float2_t{-INFINITY, 0.f};
+    vec_t num = 0.f;
+    for (int c0 = 0; c0 < p.chunks; c0 += kLanes) {
+      const int n = min(kLanes, p.chunks - c0);
+      if (c0 > 0) ml = l < n ? a.part_ml[at(c0 + l)] : float2_t{-INFINITY, 0.f};
       const float w = exp2_hw(ml.x - Mu);
-      den += wave_sum_rl(w * ml.y);
+      den += kRows == 1 ? wave_sum_rl(w * ml.y) : half_sum(w * ml.y);
       for (int c = 0; c < n; c += kAhead) {
         if (c0 + c > 0) load(c0 + c);
 #pragma unroll
         for (int u = 0; u < kAhead; ++u)
-          if (c + u < n) num += lane_f(w, min(c + u, 63)) * o[u];
+          if (c + u < n) {
+            const float wl = lane_f(w, min(c + u, kLanes - 1)), wh = lane_f(w, min(c + u, kLanes - 1) + 64 - kLanes);
+            num += (half ? wh : wl) * o[u];
+          }
       }
     }
     const int rr = p.tile * R + row, t = rr / a.G;
-    half2_t h;
+    out_t h;
 #pragma unroll
-    for (int e = 0; e < 2; ++e) {
+    for (int e = 0; e < E; ++e) {
       const float n = num[e];
       h[e] = refused ? (half_t)NAN : den == 0.f ? (half_t)0.f : (half_t)(n / den);
     }
-    half_t* dst = a.out + ((size_t)(p.s.start + t) * a.H + kvh * a.G + rr - t * a.G) * D + 2 * lane;
-    *reinterpret_cast<half2_t*>(dst) = h;
+    half_t* dst = a.out + ((size_t)(p.s.start + t) * a.H + kvh * a.G + rr - t * a.G) * D + E * l;
+    *reinterpret_cast<out_t*>(dst) = h;
   }
 }
 

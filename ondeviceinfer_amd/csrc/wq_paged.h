@@ -52,7 +52,8 @@ inline int paged_pool_check(int64_t head_dim, int64_t kv_heads, int64_t key_page
              "table_width must be positive and table_width * page_size <= 2^30");
   WQ_REQUIRE(sequences >= 0 && sequences <= kMaxSequences, WQ_ERR_INVALID_ARGUMENT,
              "sequences must be in [0, %d] (got %lld)", kMaxSequences, (long long)sequences);
-  WQ_REQUIRE(tokens >= 0 && tokens <= (1 << 24), WQ_ERR_INVALID_ARGUMENT, "tokens must be in [0, 2^24]");
+  WQ_REQUIRE(tokens >= 0 && tokens < (1 << 24), WQ_ERR_INVALID_ARGUMENT, "tokens must be in [0, 2^24) (got %lld)",
+             (long long)tokens);
   return WQ_OK;
 }
 

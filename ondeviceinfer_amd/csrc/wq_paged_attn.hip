@@ -780,8 +780,14 @@ __global__ __launch_bounds__(256) void paged_attention_merge_kernel(PagedArgs a)
 }
 
 // Which kernel a call takes, and its places of the grid per kv head: the tiles
-// the call can have at most, and as many more for chunks as bring the
-// workgroups to about four (small tiles) or two (large ones) per compute unit.
+// the call can have at most, and as many more for chunks.  Small tiles: the
+// three workgroups that a compute unit holds (seven drafted tokens behind 4100:
+// 22.3 us with four, 17.5 with three, 18.8 with two; the decode batches within
+// 2 %).  Large ones: four where two are resident, since the tiles of a ragged
+// batch differ in length (six chunks 120 us with two, 108 with four, 123 with
+// eight; twelve trees 133, 126, 127).  Where the tiles alone give small ones
+// sixteen or large ones four per compute unit nothing is split and nothing
+// merged.
 struct PagedPlan {
   int rows;                 // of a tile
   int64_t tiles, spare, slots;
@@ -799,7 +805,7 @@ PagedPlan paged_plan(int64_t tokens, int64_t sequences, int64_t G, int64_t KV, i
   p.tiles = (tokens * G + p.rows - 1) / p.rows + sequences;
   const int64_t most = tokens * ((G + p.rows - 1) / p.rows);
   if (p.tiles > most) p.tiles = most;
-  const int64_t target = p.rows == 16 ? 1024 : 1024;
+  const int64_t target = p.rows == 16 ? 768 : 1024;
   p.min_blocks = p.rows == 16 ? 4 : 8;
   const int64_t blocks = width * page_size / kKeys + 1;
   p.spare = blocks > p.min_blocks && p.tiles * KV < (p.rows == 16 ? 4 : 1) * target ? (target + KV - 1) / KV : 0;
@@ -863,7 +869,8 @@ extern "C" int wq_paged_attention(const uint16_t* q, int64_t tokens, int64_t q_h
   WQ_REQUIRE(plan.bytes == 0 || (workspace && workspace_bytes >= plan.bytes && (uintptr_t)workspace % 16 == 0),
              WQ_ERR_WORKSPACE, "paged attention needs a 16-byte aligned workspace of %zu bytes (got %zu)", plan.bytes,
              workspace_bytes);
-  WQ_REQUIRE(plan.slots * kv_heads <= 0x7fffffff, WQ_ERR_UNSUPPORTED, "too many tokens for one call");
+  WQ_REQUIRE(plan.slots * kv_heads <= 0xffffff, WQ_ERR_UNSUPPORTED,   // a grid holds 2^32 threads
+             "too many tokens for one call: %lld workgroups", (long long)(plan.slots * kv_heads));
   PagedArgs a{};
   a.q = reinterpret_cast<const half_t*>(q);
   a.kp = reinterpret_cast<const half_t*>(key_pages);

@@ -266,6 +266,32 @@ def test_large_tiles_with_bad_pages_and_empty_rows(gpu):
     check(got[150:], want[150:], tol[150:])
 
 
+@pytest.mark.parametrize('count', [1, 40])
+def test_pages_beyond_32_bit_offsets(gpu, count):
+    """Pages 2^30 elements apart: the last one starts 6 GiB into the pool."""
+    pool = Pool([count], [50 - count], hq=4, hkv=2, page=16, seed=14)
+    block = torch.empty(3 * 2 ** 30 + 2 * 2 * 16 * D, dtype=torch.float16, device=gpu)
+    k = block.as_strided((4, 2, 16, D), (2 ** 30, 16 * D, D, 1))
+    v = block.as_strided((4, 2, 16, D), (2 ** 30, 16 * D, D, 1), 2 * 16 * D)
+    table = torch.tensor([[3, 1, 2, 0]], dtype=torch.int32)
+    for e in range(4):
+        k[table[0, e]], v[table[0, e]] = pool.k[pool.table[0, e]].to(gpu), pool.v[pool.table[0, e]].to(gpu)
+    _, _, batch = pool.to(gpu)
+    batch = batch._replace(page_table=table.to(gpu))
+    query = pool.rand(count, 4, D)
+    want, tol = expected_attention(pool, query, 0.1)
+    check(paged_attention(query.to(gpu), k, v, batch, scale=0.1), want, tol)
+    cos, sin = tables()
+    qkv = pool.rand(count, 8 * D).to(gpu)
+    near_k, near_v, near = pool.to(gpu)
+    args = dict(q_heads=4, q_norm=None, k_norm=None, eps=1e-6, cos_table=cos.to(gpu), sin_table=sin.to(gpu))
+    q = paged_append(qkv, k, v, batch, **args)
+    assert torch.equal(q, paged_append(qkv, near_k, near_v, near, **args))
+    for e in range(4):
+        for far, close in ((k, near_k), (v, near_v)):
+            assert torch.equal(far[table[0, e]].view(torch.int16), close[pool.table[0, e]].view(torch.int16))
+
+
 def test_starts_out_of_order_touch_only_their_sequence(gpu):
     pool = Pool([2, 3, 1], [20, 30, 40], hq=4, hkv=2, page=16, seed=6)
     query = pool.rand(6, 4, D)

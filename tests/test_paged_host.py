@@ -166,7 +166,7 @@ def attention_args(**change):
     (dict(scale=float('inf')), _native.WQ_ERR_INVALID_ARGUMENT), (dict(ks=4000), _native.WQ_ERR_INVALID_ARGUMENT),
     (dict(vs=4100), _native.WQ_ERR_INVALID_ARGUMENT), (dict(pages=0), _native.WQ_ERR_INVALID_ARGUMENT),
     (dict(mask=20), _native.WQ_ERR_INVALID_ARGUMENT), (dict(starts=18), _native.WQ_ERR_INVALID_ARGUMENT),
-    (dict(tokens=(1 << 24) + 1), _native.WQ_ERR_INVALID_ARGUMENT), (dict(width=200), _native.WQ_ERR_WORKSPACE),
+    (dict(tokens=1 << 24), _native.WQ_ERR_INVALID_ARGUMENT), (dict(width=200), _native.WQ_ERR_WORKSPACE),
     (dict(hq=3), _native.WQ_ERR_INVALID_ARGUMENT), (dict(tokens=0), _native.WQ_OK), (dict(seqs=0), _native.WQ_OK)])
 def test_attention_refuses_before_any_launch(change, code):
     assert status('wq_paged_attention', *attention_args(**change)) == code

@@ -185,6 +185,13 @@ __device__ __forceinline__ Sight row_sight(const PagedArgs& a, const Seq& s, int
   return Sight{min(s.base + tok, keys - 1), s.base, 0};
 }
 
+// Sixteen bytes; non-temporal where every key is read by one workgroup only.
+template <bool ONCE>
+__device__ __forceinline__ uint4_t stream_load(const half_t* p) {
+  const uint4_t* q = reinterpret_cast<const uint4_t*>(p);
+  return ONCE ? __builtin_nontemporal_load(q) : *q;
+}
+
 // grid = slots * KV workgroups of four waves (flat id f: kv head f % KV, place
 // f / KV; with 8 kv heads the workgroups of one head share an XCD's L2).  Wave
 // w takes the w-th quarter of the chunk's 32-key steps and runs its own online
@@ -202,6 +209,7 @@ __device__ __forceinline__ Sight row_sight(const PagedArgs& a, const Seq& s, int
 // The next step's keys are requested as soon as the scores have consumed the
 // present ones, the values likewise, so that both are in flight during the
 // softmax of the other.
+template <bool ONCE>
 __global__ __launch_bounds__(256, 2) void paged_attention_rows_kernel(PagedArgs a) {
   constexpr int R = 16, D = kPagedDim;
   __shared__ __attribute__((aligned(16))) float red[kWaves][R][D];
@@ -258,7 +266,7 @@ __global__ __launch_bounds__(256, 2) void paged_attention_rows_kernel(PagedArgs 
         const half_t* src = kbase + (size_t)__builtin_amdgcn_readlane(g.page, l) * a.k_stride +
                             (size_t)__builtin_amdgcn_readlane(g.row, l) * D;
 #pragma unroll
-        for (int ks = 0; ks < 4; ++ks) kr[h][ks] = *reinterpret_cast<const uint4_t*>(src + 32 * ks);
+        for (int ks = 0; ks < 4; ++ks) kr[h][ks] = stream_load<ONCE>(src + 32 * ks);
         kbad[h] = (g.bad >> l) & 1;
       }
     };
@@ -269,7 +277,7 @@ __global__ __launch_bounds__(256, 2) void paged_attention_rows_kernel(PagedArgs 
         const half_t* src = vbase + (size_t)__builtin_amdgcn_readlane(g.page, l) * a.v_stride +
                             (size_t)__builtin_amdgcn_readlane(g.row, l) * D;
 #pragma unroll
-        for (int e = 0; e < 4; ++e) vr[4 * h + e] = *reinterpret_cast<const uint4_t*>(src + (size_t)e * D);
+        for (int e = 0; e < 4; ++e) vr[4 * h + e] = stream_load<ONCE>(src + (size_t)e * D);
       }
     };
     load_keys(w0);
@@ -783,7 +791,9 @@ __global__ __launch_bounds__(256) void paged_attention_merge_kernel(PagedArgs a)
 // the call can have at most, and as many more for chunks.  Small tiles: the
 // three workgroups that a compute unit holds (seven drafted tokens behind 4100:
 // 22.3 us with four, 17.5 with three, 18.8 with two; the decode batches within
-// 2 %).  Large ones: four where two are resident, since the tiles of a ragged
+// 2 %), and ten per tile up to eight per unit where many tiles of unequal
+// length are to end together (24 sequences 68 -> 64 us, 64 long ones 396 ->
+// 380, of which two thirds more would cost 400).  Large ones: four where two are resident, since the tiles of a ragged
 // batch differ in length (six chunks 120 us with two, 108 with four, 123 with
 // eight; twelve trees 133, 126, 127).  Where the tiles alone give small ones
 // sixteen or large ones four per compute unit nothing is split and nothing
@@ -809,6 +819,10 @@ PagedPlan paged_plan(int64_t tokens, int64_t sequences, int64_t G, int64_t KV, i
   p.min_blocks = p.rows == 16 ? 4 : 8;
   const int64_t blocks = width * page_size / kKeys + 1;
   p.spare = blocks > p.min_blocks && p.tiles * KV < (p.rows == 16 ? 4 : 1) * target ? (target + KV - 1) / KV : 0;
+  if (p.rows == 16 && p.spare > 0) {
+    const int64_t many = 10 * p.tiles < 2048 / KV ? 10 * p.tiles : 2048 / KV;
+    if (p.spare < many) p.spare = many;
+  }
   p.slots = p.tiles + p.spare;
   p.bytes = p.spare ? (size_t)p.slots * KV * p.rows * (kPagedDim + 2) * 4 : 0;
   return p;
@@ -897,8 +911,12 @@ extern "C" int wq_paged_attention(const uint16_t* q, int64_t tokens, int64_t q_h
   a.spare = (int)plan.spare;
   a.min_blocks = plan.min_blocks;
   const dim3 grid((unsigned)(plan.slots * kv_heads));
-  if (plan.rows == 16)
-    hipLaunchKernelGGL(paged_attention_rows_kernel, grid, dim3(256), 0, as_stream(stream), a);
+  // One tile per sequence on average: single tokens.  64 long sequences 424 us, with non-temporal loads 397; seven
+  // drafted tokens, three tiles that share their keys through the L2, 17.5 and 18.6.
+  if (plan.rows == 16 && tokens * a.G <= 16 * sequences)
+    hipLaunchKernelGGL(paged_attention_rows_kernel<true>, grid, dim3(256), 0, as_stream(stream), a);
+  else if (plan.rows == 16)
+    hipLaunchKernelGGL(paged_attention_rows_kernel<false>, grid, dim3(256), 0, as_stream(stream), a);
   else
     hipLaunchKernelGGL(paged_attention_tile_kernel, grid, dim3(256), 2 * kTileStage, as_stream(stream), a);
   rc = check_launch("paged_attention");

@@ -22,7 +22,11 @@ struct AppendArgs {
 // lanes of one DPP row, eight each, so a wave loads and stores four heads with
 // one 16-byte access per lane; the sum of squares is a row reduction and the
 // rotation's other half, d +- 64, is the lane eight away, a row rotation.
-// Wave w of part y takes the head quads 4y + w, 4 (y + parts) + w, ...
+// Wave w of part y takes the head quads 4y + w, 4 (y + parts) + w, ...  The
+// projection is read once, non-temporally (34 -> 30 us for 4100 tokens of 56
+// heads, 5.6 TB/s over what is read and written); q and the pages are what the
+// attention reads next and stay in the caches.  Bound by memory; a single
+// token by its three dependent loads (starts, page number, table row).
 __global__ __launch_bounds__(256) void paged_append_kernel(AppendArgs a) {
   const int lane = threadIdx.x & 63;
   const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
@@ -34,7 +38,8 @@ __global__ __launch_bounds__(256) void paged_append_kernel(AppendArgs a) {
   const half_t* src = a.qkv + (size_t)t * heads * kPagedDim + 8 * c;
   int quad = 4 * blockIdx.y + wave;
   // The first quad's rows are on their way while the token finds its place.
-  uint4_t next = *reinterpret_cast<const uint4_t*>(src + (size_t)min(4 * quad + sub, heads - 1) * kPagedDim);
+  uint4_t next = __builtin_nontemporal_load(
+      reinterpret_cast<const uint4_t*>(src + (size_t)min(4 * quad + sub, heads - 1) * kPagedDim));
 
   const int b = sequence_of(a.starts, a.sequences, t, lane);
   if (b < 0 || b >= a.sequences) return;
@@ -58,7 +63,8 @@ __global__ __launch_bounds__(256) void paged_append_kernel(AppendArgs a) {
   for (; quad < quads; quad += step) {
     const uint4_t raw = next;
     if (quad + step < quads)
-      next = *reinterpret_cast<const uint4_t*>(src + (size_t)min(4 * (quad + step) + sub, heads - 1) * kPagedDim);
+      next = __builtin_nontemporal_load(
+          reinterpret_cast<const uint4_t*>(src + (size_t)min(4 * (quad + step) + sub, heads - 1) * kPagedDim));
     const int h = 4 * quad + sub;   // past the last head in the last quad's spare lanes: computed, not stored
     const bool is_q = h < a.H;
     const half8_t x8 = __builtin_bit_cast(half8_t, raw);
@@ -146,6 +152,8 @@ extern "C" int wq_paged_append(const uint16_t* qkv, int64_t tokens, int64_t q_he
   a.num_pages = (int)num_pages;
   a.page_size = (int)page_size;
   const int quads = (int)((q_heads + 2 * kv_heads + 3) / 4);
+  // Few tokens: as many workgroups as there are quads of heads for their waves (one token 2.8 us).  Many: one
+  // workgroup per token, which then looks up its sequence, page and table rows once (4100 tokens 30 us against 42).
   const int parts = tokens <= 256 ? (quads + 3) / 4 : 1;
   hipLaunchKernelGGL(paged_append_kernel, dim3((unsigned)tokens, (unsigned)parts), dim3(256), 0, as_stream(stream), a);
   return check_launch("paged_append");

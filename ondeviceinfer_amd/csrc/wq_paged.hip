@@ -23,7 +23,7 @@ struct AppendArgs {
 // one 16-byte access per lane; the sum of squares is a row reduction and the
 // rotation's other half, d +- 64, is the lane eight away, a row rotation.
 // Wave w of part y takes the head quads 4y + w, 4 (y + parts) + w, ...  The
-// projection is read once, non-temporally (34 -> 30 us for 4100 tokens of 56
+// projection is read once, non-temporally (34 -> 30 us for 5844 tokens of 56
 // heads, 5.6 TB/s over what is read and written); q and the pages are what the
 // attention reads next and stay in the caches.  Bound by memory; a single
 // token by its three dependent loads (starts, page number, table row).
@@ -153,7 +153,7 @@ extern "C" int wq_paged_append(const uint16_t* qkv, int64_t tokens, int64_t q_he
   a.page_size = (int)page_size;
   const int quads = (int)((q_heads + 2 * kv_heads + 3) / 4);
   // Few tokens: as many workgroups as there are quads of heads for their waves (one token 2.8 us).  Many: one
-  // workgroup per token, which then looks up its sequence, page and table rows once (4100 tokens 30 us against 42).
+  // workgroup per token, which then looks up its sequence, page and table rows once (5844 tokens 30 us against 42).
   const int parts = tokens <= 256 ? (quads + 3) / 4 : 1;
   hipLaunchKernelGGL(paged_append_kernel, dim3((unsigned)tokens, (unsigned)parts), dim3(256), 0, as_stream(stream), a);
   return check_launch("paged_append");

@@ -208,7 +208,10 @@ __device__ __forceinline__ uint4_t stream_load(const half_t* p) {
 //   output  lane (i, kb) holds row i, d = 8 (4 kb + v) + t in acc[t][v].
 // The next step's keys are requested as soon as the scores have consumed the
 // present ones, the values likewise, so that both are in flight during the
-// softmax of the other.
+// softmax of the other.  Bound by the cache's bytes: 2.27 GB of 64 sequences in
+// 375 us, 6.1 TB/s with 160 registers and three workgroups per compute unit;
+// one sequence of 4101 positions (16.8 MB) by latency, 9 us and 6 more for the
+// merge: the starts, the page numbers, the keys, the values one after another.
 template <bool ONCE>
 __global__ __launch_bounds__(256, 2) void paged_attention_rows_kernel(PagedArgs a) {
   constexpr int R = 16, D = kPagedDim;
@@ -417,7 +420,13 @@ __global__ __launch_bounds__(256, 2) void paged_attention_rows_kernel(PagedArgs 
 // (l % 32, l / 32) = (ql, hh) holds in register r key 8 (r / 4) + 4 hh + r % 4
 // of row ql, and the probabilities, rounded to fp16, are the B operand of O^T
 // = V^T . P^T once V^T's key slots follow the same order: slot 8 h + 4 j + e
-// of a 16-key step holds key 8 j + 4 h + e.
+// of a 16-key step holds key 8 j + 4 h + e.  A 4096-token
+// prompt takes 219 us, 0.79 PFLOP/s: matrix cores busy in 36 % of the cycles,
+// vector instructions in 41 %, waves waiting in 25 % of theirs, no bank
+// conflicts.  Neither unit is full: two waves per SIMD are not enough to overlap
+// the two.  Six chunks also write and merge 82 MB of partial results.  Overlapping them within a wave, the next half block's keys
+// beside this half's exponentials, needs more registers than two waves leave
+// each (242 us with 247, 558 with spills, against 231 at the time).
 constexpr float kLag = 8.f;
 constexpr int kTileRows = 128;
 constexpr int kTileKeys = 64;

@@ -13,8 +13,13 @@
 //           token in it.
 // Which tokens stay comes down to one value: all above it and the first
 // `ties` that equal it, by index.  Everything that decides is exact or in 64
-// bits and summed in a fixed order: with 32-bit sums over 151936 tokens one
-// row in twenty of a flat distribution takes a neighbour of its token.
+// bits and summed in a fixed order: over 151936 normal logits a 32-bit
+// sum in blocks of 512 changes the token of one to three rows in a hundred, a
+// running one of a quarter to a third (numpy, 400 rows each, deviations 0.1 to 3).
+// 64 rows of 151936 fp16 logits (19 MB): tally 26 us (51 vector
+// instructions per token counted, some 19 of them 64-bit; the vector units issue
+// in 39 % of the cycles and waves wait in 43 %, so neither alone is the bound),
+// gather 15, pick 26.  One row takes 7, 9 and 16 us.
 #include "ondeviceinfer_sample.h"
 #include "wq_common.h"
 #include "wq_status.h"

@@ -43,7 +43,8 @@ extern "C" {
  *   cos/sin      rotation tables [table_positions, 128] fp16
  *   positions    [tokens] int32 row of the tables for each token (drafted
  *                tokens of a tree), NULL: the token's index in its sequence
- *   q_out        [tokens, q_heads, 128] the normalized, rotated queries
+ *   q_out        [tokens, q_heads, 128] the normalized, rotated queries; must
+ *                not overlap qkv
  * y = u * cos + rotate_half(u) * sin with u = x * rsqrt(mean(x^2) + eps) * w,
  * in fp32 and rounded to fp16 once.  A token whose index has no page (a
  * negative index, one past the table's width, a page number outside the pool)

@@ -128,6 +128,10 @@ extern "C" int wq_paged_append(const uint16_t* qkv, int64_t tokens, int64_t q_he
              WQ_ERR_INVALID_ARGUMENT, "qkv, weights, tables, pages and q_out must be 16-byte aligned");
   WQ_REQUIRE(((uintptr_t)positions | (uintptr_t)page_table | (uintptr_t)query_starts | (uintptr_t)seq_lens) % 4 == 0,
              WQ_ERR_INVALID_ARGUMENT, "integer operands must be 4-byte aligned");
+  // A workgroup writes its token's queries while others still read the projection.
+  const uintptr_t in0 = (uintptr_t)qkv, in1 = in0 + (size_t)tokens * (q_heads + 2 * kv_heads) * kPagedDim * 2;
+  const uintptr_t out0 = (uintptr_t)q_out, out1 = out0 + (size_t)tokens * q_heads * kPagedDim * 2;
+  WQ_REQUIRE(out1 <= in0 || in1 <= out0, WQ_ERR_INVALID_ARGUMENT, "q_out must not overlap qkv");
   AppendArgs a{};
   a.qkv = reinterpret_cast<const half_t*>(qkv);
   a.qn_w = reinterpret_cast<const half_t*>(q_norm_weight);

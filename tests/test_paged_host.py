@@ -190,6 +190,15 @@ def test_append_refuses_before_any_launch(change, code):
     assert status('wq_paged_append', *append_args(**change)) == code
 
 
+@pytest.mark.parametrize('out,code', [
+    (1 << 20, _native.WQ_ERR_INVALID_ARGUMENT),                           # the projection itself
+    ((1 << 20) + 3 * 8 * 256 - 16, _native.WQ_ERR_INVALID_ARGUMENT),      # its last 16 bytes
+    ((1 << 20) - 3 * 4 * 256 + 16, _native.WQ_ERR_INVALID_ARGUMENT)])     # its first 16 bytes
+def test_append_refuses_queries_over_the_projection(out, code):
+    """A token's queries would land on rows that another token's workgroup has not read."""
+    assert status('wq_paged_append', *append_args(qkv=1 << 20, tokens=3, out=out)) == code
+
+
 def sample_args(**change):
     a = dict(logits=16, kind=0, rows=2, vocab=100, stride=100, u=16, t=None, ta=1.0, k=None, ka=0, p=None, pa=1.0,
              m=None, ma=0.0, out=16, ws=16, wsb=1 << 30, stream=None)

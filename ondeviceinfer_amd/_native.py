@@ -986,6 +986,13 @@ def _page_stride(t: torch.Tensor, name: str) -> int:
     return stride[0] if t.shape[0] > 1 else heads * rows * dim
 
 
+def _scratch(workspace: torch.Tensor) -> tuple[int, int]:
+    """(pointer, bytes) of a caller's workspace; an expanded tensor would count bytes it does not have."""
+    if not workspace.is_contiguous():
+        raise ValueError(f'workspace must be contiguous, got strides {workspace.stride()}')
+    return workspace.data_ptr(), workspace.numel() * workspace.element_size()
+
+
 def _check_batch(page_table: torch.Tensor, query_starts: torch.Tensor, seq_lens: torch.Tensor) -> tuple[int, int]:
     """(sequences, table width) of a batch's device tensors."""
     if page_table.dim() != 2:
@@ -1078,7 +1085,7 @@ def paged_attention(query: torch.Tensor, key_pages: torch.Tensor, value_pages: t
             workspace = query.new_empty(ws_bytes, dtype=torch.uint8)
             ws_ptr = workspace.data_ptr()
     else:
-        ws_ptr, ws_bytes = workspace.data_ptr(), workspace.numel() * workspace.element_size()
+        ws_ptr, ws_bytes = _scratch(workspace)
     _call_on(device, 'wq_paged_attention', _ptr(query), tokens, q_heads, kv_heads, head_dim, _ptr(key_pages), k_stride,
              _ptr(value_pages), v_stride, pages, page_size, _ptr(page_table), width, _ptr(query_starts),
              _ptr(seq_lens), sequences, _ptr(tree_mask), float(scale), _ptr(out), ws_ptr, ws_bytes, _stream(device))
@@ -1138,9 +1145,10 @@ def sample(logits: torch.Tensor, uniform: torch.Tensor, temperature=1.0, top_k=0
         _check(out, torch.int64, (rows,), 'out')
     if workspace is None:   # sums of the row's parts (no counters): any scratch of this call's own
         workspace = uniform.new_empty(sample_workspace_size(rows, vocab), dtype=torch.uint8)
+    ws_ptr, ws_bytes = _scratch(workspace)
     _call_on(device, 'wq_sample', _ptr(logits), kind, rows, vocab, max(stride, vocab), _ptr(uniform), t_ptr,
-             float(t_all), k_ptr, k_all, p_ptr, float(p_all), m_ptr, float(m_all), _ptr(out), _ptr(workspace),
-             workspace.numel() * workspace.element_size(), _stream(device))
+             float(t_all), k_ptr, k_all, p_ptr, float(p_all), m_ptr, float(m_all), _ptr(out), ws_ptr, ws_bytes,
+             _stream(device))
     return out
 
 

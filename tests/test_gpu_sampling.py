@@ -203,6 +203,23 @@ def test_captured_replays_follow_their_inputs(gpu):
         compare(got, new, numbers, asks)
 
 
+@pytest.mark.parametrize('kind', ['none', 'top_k', 'top_p', 'min_p', 'both'])
+def test_cuts_in_more_tokens_than_a_list_holds(gpu, kind):
+    """260 rows share 64 MiB of lists: 32263 tokens each, of 40000 that all lie within a step or two."""
+    print(kind, flush=True)
+    gen = torch.Generator().manual_seed(260)
+    logits = (torch.randn(260, 40000, generator=gen) * 0.01).half()
+    u = torch.rand(260, generator=gen)
+    asks = settings(260, kind, np.random.default_rng(260))
+    compare(run(gpu, logits.to(gpu), u, asks), logits, u, asks)
+
+
+def test_a_workspace_without_memory_of_its_own_is_refused(gpu):
+    with pytest.raises(ValueError, match='contiguous'):
+        sample_tokens(torch.zeros(4, 10, device=gpu), torch.zeros(4, device=gpu),
+                      workspace=torch.empty(1, dtype=torch.uint8, device=gpu).expand(1 << 20))
+
+
 def test_refusals(gpu):
     logits, u = torch.zeros(4, 10, device=gpu), torch.zeros(4, device=gpu)
     with pytest.raises(TypeError):

@@ -216,6 +216,14 @@ def test_sampling_refuses_before_any_launch(change, code):
     assert status('wq_sample', *sample_args(**change)) == code
 
 
+def test_a_workspace_counts_the_memory_it_spans():
+    """An expanded tensor has elements without memory of their own."""
+    assert _native._scratch(torch.empty(6, 4, dtype=torch.float32))[1] == 96
+    for bad in (torch.empty(1, dtype=torch.uint8).expand(1 << 20), torch.empty(64, dtype=torch.uint8)[::2]):
+        with pytest.raises(ValueError, match='contiguous'):
+            _native._scratch(bad)
+
+
 def test_cpu_tensors_are_refused():
     c = cache(dim=128)
     seq = c.add()

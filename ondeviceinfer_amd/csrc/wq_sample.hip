@@ -19,7 +19,10 @@
 // 64 rows of 151936 fp16 logits (19 MB): tally 26 us (51 vector
 // instructions per token counted, some 19 of them 64-bit; the vector units issue
 // in 39 % of the cycles and waves wait in 43 %, so neither alone is the bound),
-// gather 15, pick 26.  One row takes 7, 9 and 16 us.
+// gather 15, pick 25 in nine draws of twelve.  The pick's time is its slowest
+// row's: 78 to 81 us where top-p ends among 44 thousand tokens of one bin (the
+// weights of them all, by one workgroup), 140 where top-k of a peaked row ends
+// among nearly the whole vocabulary.  One row takes 7, 9 and 16 us.
 #include "ondeviceinfer_sample.h"
 #include "wq_common.h"
 #include "wq_status.h"
@@ -39,6 +42,7 @@ constexpr int kBins = 16;
 constexpr int kMaxParts = 64;
 constexpr int kPickThreads = 1024;
 constexpr int kSub = 256;              // steps of a bin, or of a byte of the key
+constexpr int kBounded = 16384;        // longer lists are searched between bounds (Span)
 constexpr int kMostSorted = 512;       // tokens of one step put in order at once
 
 struct SampleArgs {
@@ -512,15 +516,15 @@ struct Key<float> {
   }
 };
 
-// The smallest value whose bin is at most `bin` (bins fall as values rise),
-// found by the wave 64 keys at a time.
-template <typename T>
-__device__ __forceinline__ float lowest_of(const Scale& s, int bin, int lane) {
+// The smallest value for which `holds` (which stays true as values rise), found
+// by the wave 64 keys at a time.
+template <typename T, typename F>
+__device__ __forceinline__ float lowest_where(int lane, F holds) {
   uint32_t lo = Key<T>::kLowest, n = Key<T>::kHighest - Key<T>::kLowest + 1;   // the key lies in lo .. lo + n - 1
   while (n > 1) {
     const uint32_t step = (n + 63) / 64;
     const uint32_t k = min(lo + lane * step, Key<T>::kHighest);
-    const uint64_t in = __builtin_amdgcn_ballot_w64(bin_at(s.below(s.y(Key<T>::value(k)))) <= bin);
+    const uint64_t in = __builtin_amdgcn_ballot_w64(holds(Key<T>::value(k)));
     // The first probe that is in, or the stretch behind the last one.
     const int first = in ? __builtin_ctzll(in) : 64;
     if (first == 0) return Key<T>::value(lo);
@@ -530,6 +534,12 @@ __device__ __forceinline__ float lowest_of(const Scale& s, int bin, int lane) {
     lo = next;
   }
   return Key<T>::value(lo);
+}
+
+// The smallest value whose bin is at most `bin` (bins fall as values rise).
+template <typename T>
+__device__ __forceinline__ float lowest_of(const Scale& s, int bin, int lane) {
+  return lowest_where<T>(lane, [&](float v) { return bin_at(s.below(s.y(v))) <= bin; });
 }
 
 // Where the parts' tokens of the bins lo .. hi lie in the list, part `lane`'s.
@@ -617,6 +627,18 @@ struct Cut {
   double kept;      // mass of this bin's tokens that stay
 };
 
+// The values of a bin or of a step of it.  The position of a token, its bin and
+// its step rise and fall with the value, so a token that lies outside is told
+// by two comparisons in place of its position in 64 bits, which costs every pass
+// about 650 cycles per 1024 tokens.  The bounds cost some 8 us to find, so only
+// lists longer than kBounded are searched between them: 64 rows of which one
+// lists all 151936 tokens take 198 us instead of 238 (180 with bins of few
+// tokens sorted at once), ordinary ones 75 with bounds always and 66 without.
+struct Span {
+  float least, above;   // above NaN: no bound
+  __device__ __forceinline__ bool has(float v) const { return (v >= least) & !(v >= above); }
+};
+
 struct PickShared {
   Exp2Table table;
   RowTally tally;
@@ -690,8 +712,8 @@ struct Picker {
     const double per = bin < 8 ? kSub : bin < kBins - 1 ? kSub / 4 : 8;
     return (int)fmin((s.base + 1.0 - bin_depth(bin) - y) * per, (double)(kSub - 1));
   }
-  __device__ __forceinline__ void walk(int bin, bool by_mass, double before, double goal, int byte, int sub,
-                                       uint32_t prefix) {
+  __device__ __forceinline__ void walk(int bin, bool by_mass, double before, double goal, int byte, bool bounded,
+                                       Span span, int sub, uint32_t prefix) {
     const int bits = a.mass_bits + bin_depth(bin) - 1;
     const double unit = ldexp(1.0, bits), per_unit = ldexp(1.0, -bits);
     for (int i = tid; i < kSub; i += kPickThreads) {
@@ -700,8 +722,9 @@ struct Picker {
     }
     __syncthreads();
     each([&](float v, int) {
+      if (!span.has(v)) return;
       const double y = s.y(v);
-      if (bin_at(s.below(y)) != bin) return;
+      if (!bounded && bin_at(s.below(y)) != bin) return;
       int d = sub_of(bin, y);
       if (byte < Key<T>::kBytes) {
         const uint32_t k = Key<T>::of(v);
@@ -776,7 +799,7 @@ struct Picker {
   template <typename F>
   __device__ __forceinline__ int sort(F take, int most) {
     each([&](float v, int index) {
-      if (!take(v, s.y(v))) return;
+      if (!take(v)) return;
       const int to = atomicAdd(&sh.taken, 1);
       if (to < kMostSorted) sh.order[to] = order_of(v, index);
     });
@@ -841,21 +864,42 @@ struct Picker {
   }
 
   // Where the count `want`, or the mass `goal` of which `before` lies in front
-  // of the bin, is reached among the tokens of bin `bin`.
-  __device__ __forceinline__ Cut find_cut(int bin, bool by_mass, uint32_t want, double before, double goal) {
+  // of the bin, is reached among the `tokens` tokens of bin `bin`.
+  __device__ __forceinline__ Cut find_cut(int bin, uint32_t tokens, bool by_mass, uint32_t want, double before, double goal) {
     if (tid == 0) {
       sh.left = want;
       sh.above = 0.0;     // mass of the bin in front of the steps found so far
       sh.ties = 0;
     }
     // The step of the bin; where many of tokens share it, most of them equal, the bytes of the key.
-    int sub = 0;
+    const int lane = tid & 63;
+    const bool bounded = listed > kBounded;
+    Span span{-INFINITY, NAN};
+    if (bounded && bin < kBins - 1) span.least = lowest_of<T>(s, bin, lane);
+    if (bounded && bin > 0) span.above = lowest_of<T>(s, bin - 1, lane);
+    int sub = -1;
     uint32_t prefix = 0;
+    if (tokens <= kMostSorted) {   // the whole bin is put in order
+      __syncthreads();
+      const int n = sort([&](float v) { return bounded ? span.has(v) : bin_at(s.below(s.y(v))) == bin; }, (int)tokens);
+      return end_in(bin, by_mass, before, goal, 0, n, (int)want, 0.0);
+    }
     bool few = false;
     for (int byte = Key<T>::kBytes; byte >= 0; --byte) {
-      walk(bin, by_mass, before, goal, byte, sub, prefix);
+      walk(bin, by_mass, before, goal, byte, bounded, span, sub, prefix);
       if (byte == Key<T>::kBytes) {
         sub = sh.step;
+        // Tokens of lower bins, of this one's first `upto` steps.
+        auto above = [&](float v, int upto) {
+          const double y = s.y(v);
+          const int b = bin_at(s.below(y));
+          return b < bin || (b == bin && sub_of(bin, y) < upto);
+        };
+        if (bounded && (sub < kSub - 1 || bin < kBins - 1)) {   // the last step of the last bin has no end
+          const float least = lowest_where<T>(lane, [&](float v) { return above(v, sub + 1); });
+          span.least = fmaxf(span.least, least);
+        }
+        if (bounded && sub > 0) span.above = lowest_where<T>(lane, [&](float v) { return above(v, sub); });
         few = sh.n <= kMostSorted;
         if (few) break;
       } else {
@@ -865,7 +909,11 @@ struct Picker {
     }
     Cut cut{bin, 0, 0, 0.0};
     if (few) {
-      const int n = sort([&](float v, double y) { return bin_at(s.below(y)) == bin && sub_of(bin, y) == sub; }, sh.n);
+      const int n = sort([&](float v) {
+        if (bounded) return span.has(v);
+        const double y = s.y(v);
+        return bin_at(s.below(y)) == bin && sub_of(bin, y) == sub;
+      }, sh.n);
       return end_in(bin, by_mass, before, goal, 0, n, (int)sh.left, sh.above);
     }
     cut.key = prefix;
@@ -914,7 +962,7 @@ __global__ __launch_bounds__(kPickThreads) void sample_pick_kernel(SampleArgs a)
   const bool cuts = g.by_k < kBins || q.top_p < 1.0;
   const bool ordered = cuts && g.listed <= (uint32_t)min(a.list_cap, kMostSorted);
   int sorted = 0;
-  if (ordered) sorted = pick.sort([](float, double) { return true; }, (int)g.listed);
+  if (ordered) sorted = pick.sort([](float) { return true; }, (int)g.listed);
   for (int stage = 0; stage < 2; ++stage) {
     const bool by_mass = stage == 1;
     if (by_mass ? q.top_p == 1.0 : g.by_k == kBins) continue;
@@ -928,7 +976,7 @@ __global__ __launch_bounds__(kPickThreads) void sample_pick_kernel(SampleArgs a)
       const int n = min((int)bins.tokens_of(bin), sorted - from);
       end = pick.end_in(bin, by_mass, before, goal, max(min(from, sorted - 1), 0), n, (int)g.want, 0.0);
     } else {
-      end = pick.find_cut(bin, by_mass, g.want, before, goal);
+      end = pick.find_cut(bin, bins.tokens_of(bin), by_mass, g.want, before, goal);
     }
     if (!by_mass) whole = before + end.kept;
     // Both may end at one value: the fewer ties.  Otherwise top-p's is the higher one, but for roundings.
@@ -955,6 +1003,7 @@ __global__ __launch_bounds__(kPickThreads) void sample_pick_kernel(SampleArgs a)
     unsigned long long m = 0;
     uint32_t ties = 0;
     auto add = [&](float v) {
+      if (!(v >= last_value)) return;
       const double y = s.y(v);
       if (bin_at(s.below(y)) != edge) return;
       const int st = stays(v, y);

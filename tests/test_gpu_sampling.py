@@ -214,6 +214,23 @@ def test_cuts_in_more_tokens_than_a_list_holds(gpu, kind):
     compare(run(gpu, logits.to(gpu), u, asks), logits, u, asks)
 
 
+@pytest.mark.parametrize('dtype', [torch.float16, torch.float32])
+@pytest.mark.parametrize('rows,vocab', [(8, 16000), (8, 40000), (70, 151936)])
+def test_top_k_far_below_a_peak(gpu, rows, vocab, dtype):
+    """One token 3 to 60 logits above the others: top-k ends in a bin of most of the vocabulary, top-p in one of few."""
+    print(rows, vocab, dtype, flush=True)
+    gen = torch.Generator().manual_seed(rows + vocab)
+    logits = torch.randn(rows, vocab, generator=gen) * 2.0
+    lift = torch.tensor([3.0, 12.0, 30.0, 60.0])[torch.arange(rows) % 4]
+    logits[torch.arange(rows), torch.randint(vocab, (rows,), generator=gen)] = logits.amax(dim=1) + lift
+    logits = logits.to(dtype)
+    u = torch.rand(rows, generator=gen)
+    u[::3] = 1.0 - 2.0 ** -24   # the last of what stays
+    asks = [((0.5, 1.0, 2.0)[r % 3], (94, 700, 5000)[r % 3], (1.0, 0.729, 0.9999)[r // 2 % 3], (0.0, 1e-9)[r % 2])
+            for r in range(rows)]
+    compare(run(gpu, logits.to(gpu), u, asks), logits, u, asks)
+
+
 def test_a_workspace_without_memory_of_its_own_is_refused(gpu):
     with pytest.raises(ValueError, match='contiguous'):
         sample_tokens(torch.zeros(4, 10, device=gpu), torch.zeros(4, device=gpu),

@@ -16,7 +16,6 @@ and the framework's kernels.
 """
 from __future__ import annotations
 
-import functools
 import math
 import random
 
@@ -223,26 +222,21 @@ def prepare(case: dict, seed: int) -> dict:
 
 # ----------------------------------------------------------------------------- the framework's operators
 
-@functools.lru_cache(maxsize=1)
-def _framework():
-    from ondeviceinfer_amd import paged, sampling
-    return paged, sampling
-
-
 def _own(state: dict):
-    paged, sampling = _framework()
+    from ondeviceinfer_amd.paged import PagedBatch, paged_append, paged_attention
+    from ondeviceinfer_amd.sampling import sample_tokens
     case = state['case']
     if case['kind'] == 'sample':
-        return sampling.sample_tokens(state['logits'], state['uniform'], temperature=state['temperature'],
-                                      top_k=state['top_k'], top_p=state['top_p'], min_p=state['min_p'])
-    batch = paged.PagedBatch(state['page_table'], state['query_starts'], state['seq_lens'])
+        return sample_tokens(state['logits'], state['uniform'], temperature=state['temperature'],
+                             top_k=state['top_k'], top_p=state['top_p'], min_p=state['min_p'])
+    batch = PagedBatch(state['page_table'], state['query_starts'], state['seq_lens'])
     if case['kind'] == 'append':
-        q = paged.paged_append(state['qkv'], state['key_pages'], state['value_pages'], batch, q_heads=case['q_heads'],
-                               q_norm=state['q_norm'], k_norm=state['k_norm'], eps=EPS, cos_table=state['cos'],
-                               sin_table=state['sin'], out=state['out'])
+        q = paged_append(state['qkv'], state['key_pages'], state['value_pages'], batch, q_heads=case['q_heads'],
+                         q_norm=state['q_norm'], k_norm=state['k_norm'], eps=EPS, cos_table=state['cos'],
+                         sin_table=state['sin'], out=state['out'])
         return q, state['key_pages'], state['value_pages']
-    return paged.paged_attention(state['query'], state['key_pages'], state['value_pages'], batch, scale=state['scale'],
-                                 tree_mask=state.get('tree_mask'), out=state['out'])
+    return paged_attention(state['query'], state['key_pages'], state['value_pages'], batch, scale=state['scale'],
+                           tree_mask=state.get('tree_mask'), out=state['out'])
 
 
 # ----------------------------------------------------------------------------- the plain forms

@@ -173,13 +173,15 @@ __device__ __forceinline__ int bin_depth(int bin) { return bin < 8 ? bin : 8 + 4
 // 2^(y - base), `below` whole octaves of it split off already: the fraction of
 // y is (k + t) / 256, 2^(k/256) comes from a table, 2^(t/256) = e^(t ln 2 /
 // 256) is its series to the fourth power (the next term is below 2e-15 of the
-// sum).
+// sum).  Of a y in (-2^-54, 0) the fraction y + 1 rounds to 1, k is 256 and the
+// table's last entry, 2, makes up for the octave that floor took off.
 struct Exp2Table {
-  double v[256];
+  double v[257];
 };
 
 __device__ __forceinline__ void fill_exp2(Exp2Table& t, int tid) {
   if (tid < 256) t.v[tid] = exp2((double)tid / 256.0);
+  if (tid == 0) t.v[256] = 2.0;
 }
 
 __device__ __forceinline__ double exp2_64(double y, int below, const Exp2Table& table) {

@@ -118,6 +118,26 @@ def test_flat_and_peaked_rows(gpu):
             compare(run(gpu, half.to(gpu), u, asks), half, u, asks)
 
 
+@pytest.mark.parametrize('kind', ['none', 'top_k', 'top_p', 'min_p', 'both'])
+def test_logits_just_below_zero(gpu, kind):
+    """Scaled logits y in (-2^-54, 0): y + 1 rounds to 1, so the fraction above floor(y) = -1 is a whole octave.  Tiny
+    values and subnormals beside ordinary ones, among themselves, and ordinary ones at a temperature of 1e20."""
+    print(kind, flush=True)
+    gen = torch.Generator().manual_seed(21)
+    tiny = torch.tensor([-1e-20, -3e-17, -1e-45, -1e-39, 0.0, 1e-45, 1e-20, -1e-30])
+    logits = tiny[torch.randint(8, (12, 6000), generator=gen)]
+    logits[:4, ::3] = torch.randn(4, 2000, generator=gen) * 2.0
+    logits[4:8] = torch.randn(4, 6000, generator=gen)
+    u = torch.rand(12, generator=gen)
+    asks = settings(12, kind, np.random.default_rng(21))
+    asks[4:8] = [(1e20, k, p, m) for _, k, p, m in asks[4:8]]
+    compare(run(gpu, logits.to(gpu), u, asks), logits, u, asks)
+    one = logits[8:]     # few rows: four waves per part
+    for r in range(4):
+        compare(run(gpu, one[r:r + 1].to(gpu), u[8 + r:9 + r], asks[8 + r:9 + r]), one[r:r + 1], u[8 + r:9 + r],
+                asks[8 + r:9 + r])
+
+
 def test_masked_and_infinite_logits(gpu):
     inf = float('inf')
     logits = torch.randn(8, 5000, generator=torch.Generator().manual_seed(5))

@@ -868,6 +868,7 @@ struct Picker {
   // Where the count `want`, or the mass `goal` of which `before` lies in front
   // of the bin, is reached among the `tokens` tokens of bin `bin`.
   __device__ __forceinline__ Cut find_cut(int bin, uint32_t tokens, bool by_mass, uint32_t want, double before, double goal) {
+    __syncthreads();   // top-p's search follows top-k's, whose end the other waves may still be reading
     if (tid == 0) {
       sh.left = want;
       sh.above = 0.0;     // mass of the bin in front of the steps found so far
@@ -927,7 +928,6 @@ struct Picker {
       cut.ties = min(sh.left, (uint32_t)sh.n);
     }
     cut.kept = sh.above + cut.ties * w;
-    __syncthreads();
     return cut;
   }
 };

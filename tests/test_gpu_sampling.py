@@ -251,6 +251,21 @@ def test_top_k_far_below_a_peak(gpu, rows, vocab, dtype):
     compare(run(gpu, logits.to(gpu), u, asks), logits, u, asks)
 
 
+@pytest.mark.parametrize('dtype', [torch.float16, torch.float32])
+@pytest.mark.parametrize('vocab', [9000, 30000])
+def test_top_p_behind_a_top_k_that_ends_in_a_full_bin(gpu, vocab, dtype):
+    """Flat rows: top-k ends in a bin of more tokens than are put in order at once, whose step it is found in, and the
+    search for top-p's end follows in the same row, in the same bin or another."""
+    print(vocab, dtype, flush=True)
+    gen = torch.Generator().manual_seed(vocab)
+    rows = 96
+    logits = torch.randn(rows, vocab, generator=gen).to(dtype)
+    u = torch.rand(rows, generator=gen)
+    asks = [((0.5, 1.0, 3.0, 20.0)[r % 4], (700, 2500, 6000)[r // 4 % 3], (0.5, 0.9, 0.999)[r // 12 % 3], 0.0)
+            for r in range(rows)]
+    compare(run(gpu, logits.to(gpu), u, asks), logits, u, asks)
+
+
 def test_a_workspace_without_memory_of_its_own_is_refused(gpu):
     with pytest.raises(ValueError, match='contiguous'):
         sample_tokens(torch.zeros(4, 10, device=gpu), torch.zeros(4, device=gpu),

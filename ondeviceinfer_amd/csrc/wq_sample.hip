@@ -1135,60 +1135,66 @@ __global__ __launch_bounds__(kPickThreads) void sample_pick_kernel(SampleArgs a)
   }
   if (lane == 63) sh.wave_d[wave] = x;
   __syncthreads();
-  double sum = 0.0;
-  for (int w = 0; w < wave; ++w) sum += sh.wave_d[w];
-  sum += x - m;
-  // The first token at which the running weight exceeds the target: in the one thread's run where it does, a token per
-  // lane of that thread's wave.  Failing that (roundings) the last that stays.
-  int hit = INT_MAX;
-  const uint64_t mine = __builtin_amdgcn_ballot_w64(sum <= target && sum + m > target);
-  if (mine != 0) {
-    const int l = __builtin_ctzll(mine);
-    const int f0 = __builtin_amdgcn_readlane(t0, l), f1 = __builtin_amdgcn_readlane(t1, l);
-    double before = __shfl(sum, l);
-    uint32_t ties = (uint32_t)__builtin_amdgcn_readlane((int)ties0, l);
-    hit = __builtin_amdgcn_readlane(last, l);
-    const int j1 = min(r.index(f1), r.vocab);
-    for (int j0 = max(r.index(f0), 0); j0 < j1; j0 += 64) {
-      const int j = j0 + lane;
-      const float v = j < j1 ? (float)r.base[j] + 0.f : 0.f;
-      const double y = s.y(v);
-      const int st = j < j1 ? stays(v, y) : 0;
-      const uint64_t tied = __builtin_amdgcn_ballot_w64(st == 2);
-      const uint32_t in_front = ties + (uint32_t)__popcll(tied & ((1ull << lane) - 1));
-      const double w = (st == 1) | ((st == 2) & (in_front < cut.ties)) ? weight(y) : 0.0;
-      double upto = w;
-#pragma unroll
-      for (int o = 1; o < 64; o <<= 1) {
-        const double u = __shfl_up(upto, o);
-        if (lane >= o) upto += u;
-      }
-      const uint64_t past = __builtin_amdgcn_ballot_w64((w > 0.0) & (before + upto > target));
-      if (past) {
-        hit = j0 + __builtin_ctzll(past);
-        break;
-      }
-      before += __shfl(upto, 63);
-      ties += (uint32_t)__popcll(tied);
-    }
-  }
-#pragma unroll
-  for (int o = 32; o > 0; o >>= 1) {
-    hit = min(hit, __shfl_xor(hit, o));
-    last = max(last, __shfl_xor(last, o));
-  }
+  double upto = 0.0;   // the mass of the threads up to this one
+  for (int w = 0; w < wave; ++w) upto += sh.wave_d[w];
+  upto += x;
+  // The first thread at which the running weight exceeds the target, as for the parts: decided by one set of sums, so
+  // that a target on the border of two runs falls into one of them.  Failing that (roundings) the last with any weight.
+  const uint64_t some = __builtin_amdgcn_ballot_w64(m > 0.0);
+  const uint64_t past = __builtin_amdgcn_ballot_w64((m > 0.0) & (upto > target));
   if (lane == 0) {
-    sh.wave_i[wave] = hit;
-    sh.wave_n[wave] = (uint32_t)last;
+    sh.wave_i[wave] = past ? __builtin_ctzll(past) : INT_MAX;
+    sh.wave_n[wave] = some ? 64u - (uint32_t)__builtin_clzll(some) : 0u;   // 0: none
   }
   __syncthreads();
-  if (tid == 0) {
-    for (int w = 1; w < 16; ++w) {
-      hit = min(hit, sh.wave_i[w]);
-      last = max(last, (int)sh.wave_n[w]);
+  int owner = 0, l = -1;
+  for (int w = 0; w < 16; ++w) {
+    if (l < 0 && sh.wave_i[w] != INT_MAX) {
+      owner = w;
+      l = sh.wave_i[w];
     }
-    a.tokens[row] = hit != INT_MAX ? hit : last;
   }
+  if (l < 0) {
+    for (int w = 0; w < 16; ++w) {
+      if (sh.wave_n[w] != 0) {
+        owner = w;
+        l = (int)sh.wave_n[w] - 1;
+      }
+    }
+  }
+  // A part is drawn only with weight in it, weighed by the tally and in whole numbers: should nothing here come to more
+  // than 0, the first thread's `last` is -1.
+  if (wave != owner) return;
+  l = __builtin_amdgcn_readfirstlane(max(l, 0));
+  // That thread's run, a token per lane of its wave: the first one past the target, or (roundings) the last that stays.
+  const int f0 = __builtin_amdgcn_readlane(t0, l), f1 = __builtin_amdgcn_readlane(t1, l);
+  double before = __shfl(upto - m, l);
+  uint32_t ties = (uint32_t)__builtin_amdgcn_readlane((int)ties0, l);
+  int hit = __builtin_amdgcn_readlane(last, l);
+  const int j1 = min(r.index(f1), r.vocab);
+  for (int j0 = max(r.index(f0), 0); j0 < j1; j0 += 64) {
+    const int j = j0 + lane;
+    const float v = j < j1 ? (float)r.base[j] + 0.f : 0.f;
+    const double y = s.y(v);
+    const int st = j < j1 ? stays(v, y) : 0;
+    const uint64_t tied = __builtin_amdgcn_ballot_w64(st == 2);
+    const uint32_t in_front = ties + (uint32_t)__popcll(tied & ((1ull << lane) - 1));
+    const double w = (st == 1) | ((st == 2) & (in_front < cut.ties)) ? weight(y) : 0.0;
+    double run_upto = w;
+#pragma unroll
+    for (int o = 1; o < 64; o <<= 1) {
+      const double u = __shfl_up(run_upto, o);
+      if (lane >= o) run_upto += u;
+    }
+    const uint64_t hits = __builtin_amdgcn_ballot_w64((w > 0.0) & (before + run_upto > target));
+    if (hits) {
+      hit = j0 + __builtin_ctzll(hits);
+      break;
+    }
+    before += __shfl(run_upto, 63);
+    ties += (uint32_t)__popcll(tied);
+  }
+  if (lane == 0) a.tokens[row] = hit;
 }
 
 // Parts of a row, a wave each: sixteen waves per compute unit over all rows,

@@ -105,6 +105,23 @@ def test_equal_values_are_cut_exactly(gpu):
     assert got.tolist() == [0, 4, 7, 3]
 
 
+@pytest.mark.parametrize('value', [0.75, 1.0, 3.0, -4.0, 0.1])
+@pytest.mark.parametrize('vocab', [4096, 16384])
+def test_draws_on_the_border_between_equal_tokens(gpu, vocab, value):
+    """vocab equal weights w, u = k / vocab: token k.  The sums of the weights are rounded, at most vocab 2^-53 of the
+    whole and so far below one w each way: the target may fall on the other side of token k's border, but no further."""
+    print(vocab, value, flush=True)
+    k = torch.arange(0, vocab, 8 if vocab == 4096 else 32)
+    k = torch.cat((k, k + 1, torch.arange(1023, vocab, 1024)))
+    u = k.float() / vocab
+    for dtype in (torch.float16, torch.float32):
+        logits = torch.full((1, vocab), value, dtype=dtype, device=gpu)
+        many = sample_tokens(logits.expand(k.numel(), vocab).contiguous(), u.to(gpu)).cpu()   # a wave per part
+        assert ((many - k).abs() <= 1).all(), (k[(many - k).abs() > 1][:5], many[(many - k).abs() > 1][:5])
+        few = torch.cat([sample_tokens(logits, u[i:i + 1].to(gpu)) for i in range(0, k.numel(), 7)]).cpu()
+        assert ((few - k[::7]).abs() <= 1).all(), (k[::7][(few - k[::7]).abs() > 1][:5], few[(few - k[::7]).abs() > 1][:5])
+
+
 def test_flat_and_peaked_rows(gpu):
     """Large and small temperatures: nearly all tokens in one octave of weights, or one token with all of it."""
     gen = torch.Generator().manual_seed(4)

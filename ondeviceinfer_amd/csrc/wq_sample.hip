@@ -1,8 +1,9 @@
 // Sampling one token per row of logits: temperature, top-k, top-p, min-p and
 // the draw from a given uniform number.
 //
-// With y = logit log2(e) / T a token weighs 2^y.  Three launches, the row cut
-// into parts of whole 16-byte chunks:
+// With y = logit log2(e) / T a token weighs 2^(y - the largest y): exactly 1 for
+// the largest, so that equal ones are drawn and cut exactly.  Three launches,
+// the row cut into parts of whole 16-byte chunks:
 //   tally   counts every part's tokens and adds their weights in 16 bins of
 //           octaves of weight, from the part's largest down;
 //   gather  from the row's bins follow the ones in which top-k, top-p and
@@ -57,7 +58,7 @@ struct SampleArgs {
   int32_t top_k_all;
   int64_t* tokens;
   float2_t* peak;     // [rows][parts] (largest logit, bits of its first index); NaN: the part holds one
-  double* mass;       // [rows][parts][kBins], in units of 2^base of the part
+  double* mass;       // [rows][parts][kBins], the part's largest weighs 1
   uint32_t* count;    // [rows][parts][kBins]
   float2_t* list;     // [rows][list_cap] (logit, bits of its index)
 };
@@ -140,24 +141,27 @@ __device__ __forceinline__ Ask read_ask(const SampleArgs& a, int row) {
   return q;
 }
 
-// Weights against a base, the octave of the largest rounded up to one of
+// Positions against a base, the octave of the largest rounded up to one of
 // 4 n + 3: the bins of a part and of the row then start whole multiples of
-// four octaves apart.  Infinite logits: where the largest is +inf only its
-// equals weigh anything, and a part that holds nothing above -inf weighs
-// nothing.
+// four octaves apart.  Weights against the largest itself.  Infinite logits:
+// where the largest is +inf only its equals weigh anything, and a part that
+// holds nothing above -inf weighs nothing.
 struct Scale {
-  double to_octaves, base;
+  double to_octaves, base, zero;
   float top;
   bool infinite;
 
   __device__ __forceinline__ Scale(double per_logit, float largest)
       : to_octaves(per_logit), top(largest), infinite(isinf(largest)) {
     base = infinite ? 3.0 : 4.0 * floor(0.25 * floor((double)largest * per_logit)) + 3.0;
+    zero = infinite ? 0.0 : (double)largest;
   }
-  __device__ __forceinline__ double y(float v) const {
-    const float u = infinite ? (((v == top) & (top > 0.f)) ? 0.f : -INFINITY) : v;
-    return (double)u * to_octaves;
+  __device__ __forceinline__ double finite(float v) const {
+    return (double)(infinite ? (((v == top) & (top > 0.f)) ? 0.f : -INFINITY) : v);
   }
+  __device__ __forceinline__ double y(float v) const { return finite(v) * to_octaves; }
+  // log2 of its weight: 0 for the largest.  The difference of two logits is exact, or as good as.
+  __device__ __forceinline__ double fall(float v) const { return (finite(v) - zero) * to_octaves; }
   // Whole octaves below the base, 1100 for as many or more (2^-1100 is nothing).
   __device__ __forceinline__ int below(double y) const { return (int)fmin(base - floor(y), 1100.0); }
 };
@@ -170,11 +174,11 @@ __device__ __forceinline__ int bin_at(int depth) {
 }
 __device__ __forceinline__ int bin_depth(int bin) { return bin < 8 ? bin : 8 + 4 * (bin - 8); }   // its first octave
 
-// 2^(y - base), `below` whole octaves of it split off already: the fraction of
-// y is (k + t) / 256, 2^(k/256) comes from a table, 2^(t/256) = e^(t ln 2 /
-// 256) is its series to the fourth power (the next term is below 2e-15 of the
-// sum).  Of a y in (-2^-54, 0) the fraction y + 1 rounds to 1, k is 256 and the
-// table's last entry, 2, makes up for the octave that floor took off.
+// 2^d for d <= 0: its whole octaves split off, the fraction is (k + t) / 256,
+// 2^(k/256) comes from a table, 2^(t/256) = e^(t ln 2 / 256) is its series to
+// the fourth power (the next term is below 2e-15 of the sum).  Of a d in
+// (-2^-54, 0) the fraction d + 1 rounds to 1, k is 256 and the table's last
+// entry, 2, makes up for the octave that floor took off.
 struct Exp2Table {
   double v[257];
 };
@@ -184,16 +188,17 @@ __device__ __forceinline__ void fill_exp2(Exp2Table& t, int tid) {
   if (tid == 0) t.v[256] = 2.0;
 }
 
-__device__ __forceinline__ double exp2_64(double y, int below, const Exp2Table& table) {
+__device__ __forceinline__ double exp2_64(double d, const Exp2Table& table) {
   constexpr double c = 0.69314718055994530942 / 256.0;
-  const double f = 256.0 * fmax(y - floor(y), 0.0);   // 0 for -inf, whose difference is NaN
+  const double whole = floor(d);
+  const double f = 256.0 * fmax(d - whole, 0.0);   // 0 for -inf, whose difference is NaN
   const int k = (int)f;
   const double t = f - (double)k;
   double s = __builtin_fma(t, c * c * c * c / 24.0, c * c * c / 6.0);
   s = __builtin_fma(s, t, c * c / 2.0);
   s = __builtin_fma(s, t, c);
   s = __builtin_fma(s, t, 1.0);
-  return ldexp(s * table.v[k], -below);
+  return ldexp(s * table.v[k], (int)fmax(whole, -1100.0));
 }
 
 // (best, at) the better of two of a row's largest: NaN first, then the larger, then the lower index.
@@ -280,9 +285,8 @@ __global__ __launch_bounds__(256) void sample_tally_kernel(SampleArgs a) {
     const uint32_t in = r.load(c, v);
 #pragma unroll
     for (int e = 0; e < E; ++e) {
-      const double y = s.y(v[e]);
-      const int below = s.below(y), b = bin_at(below);
-      const double w = exp2_64(y, below, table);
+      const int b = bin_at(s.below(s.y(v[e])));
+      const double w = exp2_64(s.fall(v[e]), table);
       const uint32_t one = (in >> e) & 1;   // 0: not of the row
       add_lds(&mass[b][tid], one ? w : 0.0);
       add_lds(&count[b][tid], one);
@@ -330,10 +334,10 @@ struct RowTally {
   uint32_t count[kBins];
   double part_mass[kMaxParts][kBins];
   uint32_t part_count[kMaxParts][kBins];
-  double raw_mass[kMaxParts][kBins];        // against the part's base
+  double raw_mass[kMaxParts][kBins];        // against the part's largest
   uint32_t raw_count[kMaxParts][kBins];
   int shift[kMaxParts];       // octaves from the row's base down to the part's (64: as many or more)
-  double scale[kMaxParts];    // 2^-octaves
+  double scale[kMaxParts];    // what the part's largest weighs
 };
 
 // A thread's share of the row's tallies, requested before the row's settings are known.
@@ -365,7 +369,7 @@ __device__ __forceinline__ void read_tally(const SampleArgs& a, const Scale& s, 
     const double down = isinf(s.top) || isinf(top) ? (top == s.top ? 0.0 : INFINITY)
                                                    : s.base - Scale(s.to_octaves, top).base;
     t.shift[tid] = (int)fmin(down, 64.0);
-    t.scale[tid] = down < 1074.0 ? ldexp(1.0, -(int)down) : 0.0;
+    t.scale[tid] = exp2(s.fall(top));
   }
 #pragma unroll
   for (int i = 0; i < TallyShare<THREADS>::N; ++i) {   // past the last part: repeats, never read
@@ -695,9 +699,12 @@ struct Picker {
     }
   }
 
-  __device__ __forceinline__ double weight_of(float v) const {
-    const double y = s.y(v);
-    return exp2_64(y, s.below(y), sh.table);
+  __device__ __forceinline__ double weight_of(float v) const { return exp2_64(s.fall(v), sh.table); }
+
+  // Fraction bits of masses of bin `bin` as whole numbers: the largest position lies 0 to 3 octaves below the base, and
+  // a weight of the bin is at most 2^(1 - those of the bin's first octave beyond them), or 1.
+  __device__ __forceinline__ int bits_of(int bin) const {
+    return a.mass_bits + max(bin_depth(bin) - 1 - s.below(s.y(s.top)), 0);
   }
 
   __device__ __forceinline__ uint64_t order_of(float v, int index) const {
@@ -707,16 +714,16 @@ struct Picker {
   // One step of 256 down a bin (`byte` = kBytes), or down the values of its
   // step `sub` that share the leading bytes of the key: which step holds the
   // end, what lies above it.  The last bin, which has no end, goes in eighths
-  // of an octave.  Masses are whole numbers of 2^-mass_bits of the power of two
-  // next above the bin's weights, so that their sum does not depend on the
-  // order.
+  // of an octave.  Masses are whole numbers of 2^-mass_bits of a power of two
+  // that the bin's weights do not exceed, so that their sum does not depend on
+  // the order.
   __device__ __forceinline__ int sub_of(int bin, double y) const {
     const double per = bin < 8 ? kSub : bin < kBins - 1 ? kSub / 4 : 8;
     return (int)fmin((s.base + 1.0 - bin_depth(bin) - y) * per, (double)(kSub - 1));
   }
   __device__ __forceinline__ void walk(int bin, bool by_mass, double before, double goal, int byte, bool bounded,
                                        Span span, int sub, uint32_t prefix) {
-    const int bits = a.mass_bits + bin_depth(bin) - 1;
+    const int bits = bits_of(bin);
     const double unit = ldexp(1.0, bits), per_unit = ldexp(1.0, -bits);
     for (int i = tid; i < kSub; i += kPickThreads) {
       sh.step_count[i] = 0;
@@ -734,7 +741,7 @@ struct Picker {
         d = 255 - (int)((k >> (8 * byte)) & 255);
       }
       atomicAdd(&sh.step_count[d], 1u);
-      atomicAdd(&sh.step_mass[d], (unsigned long long)rint(exp2_64(y, s.below(y), sh.table) * unit));
+      atomicAdd(&sh.step_mass[d], (unsigned long long)rint(weight_of(v) * unit));
     });
     __syncthreads();
     if (tid < 64) {   // four steps per lane
@@ -990,11 +997,10 @@ __global__ __launch_bounds__(kPickThreads) void sample_pick_kernel(SampleArgs a)
   const float last_value = cut.bin < kBins ? Key<T>::value(cut.key) : -INFINITY;
   const double min_y = g.min_y;
   auto stays = [&](float v, double y) -> int { return y >= min_y ? (int)(v > last_value) + 2 * (int)(v == last_value) : 0; };
-  auto weight = [&](double y) { return exp2_64(y, s.below(y), sh.table); };
 
   // What stays of every part: the bins in front of the edge, and its own tokens of the edge, sixteen lanes per part.
   static_assert(kPickThreads == 16 * kMaxParts, "sixteen lanes per part");
-  const int bits = a.mass_bits + bin_depth(edge) - 1;
+  const int bits = pick.bits_of(edge);
   const double unit = ldexp(1.0, bits), per_unit = ldexp(1.0, -bits);
   {
     uint32_t from, to;
@@ -1009,7 +1015,7 @@ __global__ __launch_bounds__(kPickThreads) void sample_pick_kernel(SampleArgs a)
       const double y = s.y(v);
       if (bin_at(s.below(y)) != edge) return;
       const int st = stays(v, y);
-      if (st == 1) m += (unsigned long long)rint(weight(y) * unit);
+      if (st == 1) m += (unsigned long long)rint(pick.weight_of(v) * unit);
       ties += st == 2;
     };
     if (p < a.parts && edge < kBins && sh.tally.part_count[p][edge] != 0) {
@@ -1059,7 +1065,7 @@ __global__ __launch_bounds__(kPickThreads) void sample_pick_kernel(SampleArgs a)
     // Signed on purpose: of the unsigned form, ties < cut.ties ? min(n, cut.ties - ties) : 0, hipcc 7.2 keeps a plain
     // subtraction and drops the comparison.
     const int kept = max(min((int)n, (int)cut.ties - (int)ties), 0);
-    if (kept > 0) m += kept * weight(s.y(Key<T>::value(cut.key)));
+    if (kept > 0) m += kept * pick.weight_of(Key<T>::value(cut.key));
     double upto = m;
 #pragma unroll
     for (int o = 1; o < 64; o <<= 1) {
@@ -1067,7 +1073,7 @@ __global__ __launch_bounds__(kPickThreads) void sample_pick_kernel(SampleArgs a)
       if (lane >= o) upto += u;
     }
     const double target = (double)a.uniform[row] * __shfl(upto, 63);
-    const uint64_t some = __builtin_amdgcn_ballot_w64(m > 0.0);   // never none: the largest weighs at least 1
+    const uint64_t some = __builtin_amdgcn_ballot_w64(m > 0.0);   // never none: the largest weighs 1
     const uint64_t past = __builtin_amdgcn_ballot_w64(m > 0.0 && upto > target);
     const int part = past ? __builtin_ctzll(past) : 63 - __builtin_clzll(some);
     if (lane == part) {
@@ -1115,13 +1121,12 @@ __global__ __launch_bounds__(kPickThreads) void sample_pick_kernel(SampleArgs a)
       const uint32_t in = r.load(c, v);
 #pragma unroll
       for (int e = 0; e < E; ++e) {
-        const double y = s.y(v[e]);
-        const int st = (in >> e) & 1 ? stays(v[e], y) : 0;
+        const int st = (in >> e) & 1 ? stays(v[e], s.y(v[e])) : 0;
         const bool tie = st == 2;
         const bool in_draw = (st == 1) | (tie & (ties < cut.ties));
         ties += tie;
         if (__builtin_amdgcn_ballot_w64(in_draw) == 0) continue;   // of a filtered row most waves have nothing here
-        const double w = in_draw ? weight(y) : 0.0;
+        const double w = in_draw ? pick.weight_of(v[e]) : 0.0;
         m += w;
         last = w > 0.0 ? r.index(c) + e : last;
       }
@@ -1162,8 +1167,6 @@ __global__ __launch_bounds__(kPickThreads) void sample_pick_kernel(SampleArgs a)
       }
     }
   }
-  // A part is drawn only with weight in it, weighed by the tally and in whole numbers: should nothing here come to more
-  // than 0, the first thread's `last` is -1.
   if (wave != owner) return;
   l = __builtin_amdgcn_readfirstlane(max(l, 0));
   // That thread's run, a token per lane of its wave: the first one past the target, or (roundings) the last that stays.
@@ -1175,11 +1178,10 @@ __global__ __launch_bounds__(kPickThreads) void sample_pick_kernel(SampleArgs a)
   for (int j0 = max(r.index(f0), 0); j0 < j1; j0 += 64) {
     const int j = j0 + lane;
     const float v = j < j1 ? (float)r.base[j] + 0.f : 0.f;
-    const double y = s.y(v);
-    const int st = j < j1 ? stays(v, y) : 0;
+    const int st = j < j1 ? stays(v, s.y(v)) : 0;
     const uint64_t tied = __builtin_amdgcn_ballot_w64(st == 2);
     const uint32_t in_front = ties + (uint32_t)__popcll(tied & ((1ull << lane) - 1));
-    const double w = (st == 1) | ((st == 2) & (in_front < cut.ties)) ? weight(y) : 0.0;
+    const double w = (st == 1) | ((st == 2) & (in_front < cut.ties)) ? pick.weight_of(v) : 0.0;
     double run_upto = w;
 #pragma unroll
     for (int o = 1; o < 64; o <<= 1) {
@@ -1194,7 +1196,8 @@ __global__ __launch_bounds__(kPickThreads) void sample_pick_kernel(SampleArgs a)
     before += __shfl(run_upto, 63);
     ties += (uint32_t)__popcll(tied);
   }
-  if (lane == 0) a.tokens[row] = hit;
+  // The tally found weight in this part; should none be left of it here (at 2^-1074), the largest is the answer.
+  if (lane == 0) a.tokens[row] = hit >= 0 ? hit : first;
 }
 
 // Parts of a row, a wave each: sixteen waves per compute unit over all rows,

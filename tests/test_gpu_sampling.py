@@ -122,6 +122,30 @@ def test_draws_on_the_border_between_equal_tokens(gpu, vocab, value):
         assert ((few - k[::7]).abs() <= 1).all(), (k[::7][(few - k[::7]).abs() > 1][:5], few[(few - k[::7]).abs() > 1][:5])
 
 
+@pytest.mark.parametrize('value', [0.75, 1.0, 3.0, -4.0, 0.1, -0.3, 700.0])
+@pytest.mark.parametrize('temperature', [1.0, 0.7, 50.0])
+def test_equal_logits_are_drawn_and_cut_exactly(gpu, temperature, value):
+    """The largest weighs exactly 1, so rows of equal logits of any value have exact sums: u = k / 8192 draws token k,
+    top_p = 1/2 keeps 4096 of them, top_p = 3/4 of 4096 kept by top-k 3072; behind far smaller ones too."""
+    print(value, temperature, flush=True)
+    n = 8192
+    k = torch.cat((torch.arange(0, n, 64), torch.arange(1023, n, 1024)))
+    u = (k.float() / n).to(gpu)
+    rows = k.numel()
+    for dtype in (torch.float16, torch.float32):
+        logits = torch.full((rows, n), value, dtype=dtype, device=gpu)
+        one = logits[:1]
+        assert torch.equal(sample_tokens(logits, u, temperature=temperature).cpu(), k)
+        assert torch.equal(sample_tokens(logits, u, temperature=temperature, top_p=0.5).cpu(), k // 2)
+        assert torch.equal(sample_tokens(logits, u, temperature=temperature, top_p=0.75, top_k=4096).cpu(), 3 * k // 8)
+        few = torch.cat([sample_tokens(one, u[i:i + 1], temperature=temperature, top_p=0.5) for i in range(0, rows, 9)])
+        assert torch.equal(few.cpu(), k[::9] // 2)
+        wide = torch.full((rows, 4 * n), -60000.0, dtype=dtype, device=gpu)
+        wide[:, 2::4] = value
+        assert torch.equal(sample_tokens(wide, u, temperature=temperature).cpu(), 4 * k + 2)
+        assert torch.equal(sample_tokens(wide, u, temperature=temperature, top_p=0.5).cpu(), 4 * (k // 2) + 2)
+
+
 def test_flat_and_peaked_rows(gpu):
     """Large and small temperatures: nearly all tokens in one octave of weights, or one token with all of it."""
     gen = torch.Generator().manual_seed(4)

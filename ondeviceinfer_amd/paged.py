@@ -146,8 +146,8 @@ class PagedKVCache:
 
     def extend(self, sequences: Sequence[int], counts: Sequence[int]) -> PagedBatch:
         """Room for ``counts[i]`` new tokens of ``sequences[i]``, and the batch
-        that a step over them takes.  Raises before anything changes when the
-        pool has too few pages."""
+        that a step over them takes.  Nothing has changed if it raises (too few
+        pages in the pool, no memory for the batch)."""
         if len(sequences) != len(counts) or len(set(sequences)) != len(sequences):
             raise ValueError('a step takes each of its sequences once, with a count each')
         if any(n < 0 for n in counts):
@@ -156,16 +156,20 @@ class PagedKVCache:
         want = [-(-n // self.page_size) - len(self._pages[s]) for s, n in zip(sequences, lens)]
         if sum(want) > len(self._free):
             raise ValueError(f'KV cache capacity exceeded: {sum(want)} more pages needed, {len(self._free)} free')
-        for s, n, more in zip(sequences, lens, want):
-            self._pages[s].extend(self._free.pop() for _ in range(more))
-            self._lengths[s] = n
-        width = max([1, *(len(self._pages[s]) for s in sequences)])
-        rows = [self._pages[s] + [-1] * (width - len(self._pages[s])) for s in sequences]
+        spare = reversed(self._free)
+        more = [[next(spare) for _ in range(n)] for n in want]
+        rows = [self._pages[s] + pages for s, pages in zip(sequences, more)]
+        width = max([1, *map(len, rows)])
+        rows = [row + [-1] * (width - len(row)) for row in rows]
         starts = [0]
         for n in counts:
             starts.append(starts[-1] + n)
         # One copy to the device for all three.
         flat = torch.tensor([x for row in rows for x in row] + starts + lens, dtype=torch.int32).to(self.device)
+        for s, pages, n in zip(sequences, more, lens):
+            self._pages[s].extend(pages)
+            self._lengths[s] = n
+        del self._free[len(self._free) - sum(want):]
         table = len(rows) * width
         return PagedBatch(flat[:table].view(len(rows), width), flat[table:table + len(starts)],
                           flat[table + len(starts):])

@@ -44,6 +44,20 @@ def test_a_step_that_does_not_fit_changes_nothing():
         c.extend([a], [-1])
 
 
+def test_a_step_whose_batch_cannot_be_made_changes_nothing():
+    c = cache(pages=6)
+    a, b = c.add(), c.add()
+    first = c.extend([a], [20]).page_table.tolist()
+    c.device = 'nowhere'
+    with pytest.raises(RuntimeError):
+        c.extend([a, b], [20, 5])
+    assert c.free_pages == 4 and c.length(a) == 20 and c.length(b) == 0
+    c.device = torch.device('cpu')
+    batch = c.extend([b, a], [5, 20])
+    assert batch.page_table[1, :2].tolist() == first[0]
+    assert len(set(batch.page_table[batch.page_table >= 0].tolist())) == 4 and c.free_pages == 2
+
+
 def test_pages_come_back():
     c = cache(pages=6)
     a = c.add()

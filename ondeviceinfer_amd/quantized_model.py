@@ -714,16 +714,15 @@ class QuantizedQwen3ForCausalLM:
         try:
             hidden_states = self._paged_layers(input_ids, PagedStep(
                 cache, batch, *self._rope_tables(max(n + c for n, c in zip(past, counts))),
-                1.0 / float(cfg.head_dim) ** 0.5, positions, tree_mask))
+                1.0 / float(cfg.head_dim) ** 0.5, positions, tree_mask))[0]
+            if not all_logits and len(counts) < hidden_states.shape[0]:
+                hidden_states = hidden_states[batch.query_starts[1:].long() - 1]
+            hidden_states = rms_norm(hidden_states.contiguous(), self.final_norm, cfg.rms_norm_eps)
+            return CausalLMOutput(logits=self._logits(hidden_states), cache=cache)
         except BaseException:
-            for seq, n in zip(sequences, past):   # the step's positions hold nothing
+            for seq, n in zip(sequences, past):   # a step that failed has not happened
                 cache.truncate(seq, n)
             raise
-        hidden_states = hidden_states[0]
-        if not all_logits and len(counts) < hidden_states.shape[0]:
-            hidden_states = hidden_states[batch.query_starts[1:].long() - 1]
-        hidden_states = rms_norm(hidden_states.contiguous(), self.final_norm, cfg.rms_norm_eps)
-        return CausalLMOutput(logits=self._logits(hidden_states), cache=cache)
 
     def _paged_layers(self, input_ids: Tensor, step: PagedStep) -> Tensor:
         """The decoder layers over a step's tokens, ``[1, tokens, hidden]``."""

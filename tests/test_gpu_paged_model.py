@@ -109,6 +109,30 @@ def test_a_step_without_room_leaves_the_sequences_as_they_were(tiny):
     assert cache.length(seq) == 20 and cache.free_pages == 1
 
 
+def test_a_step_that_fails_at_the_lm_head_has_not_happened(tiny, monkeypatch):
+    _, model = tiny
+    cache = model.make_paged_cache(num_pages=8)
+    seqs = [cache.add(), cache.add()]
+    tokens = torch.arange(40)
+    model.forward_paged(tokens[:25], cache, seqs, [20, 5])
+    free = cache.free_pages
+
+    def no_memory(hidden_states):
+        raise torch.OutOfMemoryError('no memory for the logits')
+
+    with monkeypatch.context() as patch:
+        patch.setattr(model, '_logits', no_memory)
+        for kw in (dict(), dict(all_logits=True)):
+            with pytest.raises(torch.OutOfMemoryError):
+                model.forward_paged(tokens[25:40], cache, seqs, [13, 2], **kw)
+            assert [cache.length(s) for s in seqs] == [20, 5] and cache.free_pages == free
+    got = model.forward_paged(tokens[25:40], cache, seqs, [13, 2]).logits
+    other = model.make_paged_cache(num_pages=8)
+    again = [other.add(), other.add()]
+    model.forward_paged(tokens[:25], other, again, [20, 5])
+    assert torch.equal(got, model.forward_paged(tokens[25:40], other, again, [13, 2]).logits)
+
+
 def test_sampled_generation(tiny):
     np_model, model = tiny
     rng = np.random.default_rng(3)

@@ -182,6 +182,32 @@ def test_tree_attention(gpu, name):
     check(got, want, tol)
 
 
+LONG = {
+    # name: (new, past, hq, hkv, page, tree): what of the kernels' loops it reaches that shorter sequences do not
+    'more-chunks-than-lanes': ([1], [9000], 2, 1, 16, False),             # small tiles: 71 chunks, 64 of them at once
+    'more-chunks-than-half-a-wave': ([64], [9001], 1, 1, 32, True),       # large tiles: 36 chunks, 32 at once
+    'many-chunks-of-a-prompt': ([300, 70], [8700, 8300], 1, 1, 16, False),
+    'unsplit-tokens': ([1] * 1100, [4600 if b in (3, 600) else b % 37 for b in range(1100)], 3, 3, 16, False),
+    'unsplit-chunks': ([129] * 8, [1300 if b == 5 else 3 * b for b in range(8)], 64, 64, 16, False),
+}
+
+
+@pytest.mark.parametrize('name', list(LONG))
+def test_long_sequences(gpu, name):
+    """Merges of more chunks than a wave or half of one holds, and the page numbers of a wave's or a tile's keys looked
+    up a second time (more than 1024 keys in one chunk: where the call's tiles fill the machine nothing is split)."""
+    new, past, hq, hkv, page, tree = LONG[name]
+    print(name, flush=True)
+    pool = Pool(new, past, hq=hq, hkv=hkv, page=page, seed=len(name))
+    masks = tree_masks(new, random.Random(17)) if tree else None
+    query = pool.rand(pool.tokens, hq, D, scale=1.5)
+    scale = 1.0 / math.sqrt(D)
+    want, tol = expected_attention(pool, query, scale, masks)
+    k, v, batch = pool.to(gpu)
+    mask = None if masks is None else torch.tensor([signed(m) for m in masks], dtype=torch.int64, device=gpu)
+    check(paged_attention(query.to(gpu), k, v, batch, scale=scale, tree_mask=mask), want, tol)
+
+
 def test_rows_that_attend_nothing_are_zero(gpu):
     """An empty mask in front of an empty cache, and lengths shorter than the new tokens."""
     pool = Pool([3, 2], [0, 40], hq=4, hkv=2, page=16, seed=1)

@@ -292,6 +292,37 @@ def test_large_tiles_with_bad_pages_and_empty_rows(gpu):
     check(got[150:], want[150:], tol[150:])
 
 
+@pytest.mark.parametrize('past', [37, 2500])            # one chunk, several
+@pytest.mark.parametrize('count', [1, 40])             # small tiles, large tiles
+def test_large_scores(gpu, count, past):
+    """Keys c u and queries a u of one direction u of +-1, a and c of eleven bits: scores up to 2^36 whose
+    products with the scale are rounded by many octaves, keys that are alike having the same score.  A row's largest
+    key is ahead of the next by far, so it has all the weight, or half of it where two are alike.  The result is that
+    key's value, or the mean of two, with one rounding."""
+    pool = Pool([count], [past], hq=4, hkv=2, page=16, seed=count)
+    gen, length = pool.gen, count + past
+    u = torch.randint(2, (D,), generator=gen).float() * 2 - 1
+    odd = lambda *shape: 1 + torch.randint(1024, shape, generator=gen).float() / 1024  # noqa: E731
+    size = odd(length) * 2.0 ** torch.randint(0, 11, (length,), generator=gen).float()
+    for i, top in ((3, 12), (past // 2, 13), (past // 2 + 1, 13), (past - 1, 14)):
+        size[i] = 1397 / 1024 * 2.0 ** top
+    for i in range(length):
+        slot = pool.table[0, i // 16].item()
+        pool.k[slot, :, i % 16] = (size[i] * u).half()
+    query = (u * odd(count, 4, 1) * 2.0 ** torch.randint(8, 15, (count, 4, 1), generator=gen).float()).half()
+    k, v, batch = pool.to(gpu)
+    values = pool.rows(0, pool.v).double()
+    for scale in (1.0 / math.sqrt(D), 1.0, 100.0, 2.0 ** -18, 2.0 ** -20):
+        want = values[past - 1].repeat_interleave(2, dim=0)
+        got = paged_attention(query.to(gpu), k, v, batch, scale=scale).double().cpu()
+        assert torch.equal(got, want.expand(count, 4, D))
+        # One position less than cached: the last token sees the two that are alike at the most.
+        near = batch._replace(seq_lens=batch.seq_lens - count - 1)
+        got = paged_attention(query.to(gpu), k, v, near, scale=scale)[-1].double().cpu()
+        want = ((values[past // 2] + values[past // 2 + 1]) / 2).repeat_interleave(2, dim=0)
+        assert ((got - want).abs() <= want.abs() * HALF_ULP + TINY).all()
+
+
 @pytest.mark.parametrize('count', [1, 40])
 def test_pages_beyond_32_bit_offsets(gpu, count):
     """Pages 2^30 elements apart: the last one starts 6 GiB into the pool."""

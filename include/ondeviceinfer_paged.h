@@ -78,7 +78,8 @@ int wq_paged_attention_workspace_size(int64_t tokens, int64_t sequences, int64_t
  *                bit is set in its mask (bit j: the j-th, its own bit
  *                included); at most 64 new tokens per sequence.
  * out = softmax(scale * q . k) . v in fp32, the probabilities rounded to fp16
- * for the product with v.  What a token does not attend has no influence on
+ * for the product with v and their sum: by 2^-11 of each, or by 2^-36 of the
+ * largest of its chunk of keys where that is more.  What a token does not attend has no influence on
  * it, infinite or NaN as it may be; one that attends an infinite or NaN value
  * is no number there, and may be NaN in its other elements too.  A token that
  * attends nothing gets zeros, one that

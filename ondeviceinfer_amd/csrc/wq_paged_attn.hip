@@ -19,6 +19,13 @@ constexpr int kKeys = 32;          // keys per step of a wave
 constexpr int kWaves = 4;          // waves per workgroup
 constexpr int kMaxPagedGroup = 16; // q heads per kv head
 
+// Probabilities are rounded to fp16 for the product with the values, 2^kLift
+// times as large as they are (so are their sums, and the quotient is not): the
+// largest is 2^14, and what lies up to 28 octaves below it keeps its eleven
+// bits, where fractions of 1 would fade from 14 octaves on and be 0 from 25.
+// The sums are of the rounded ones, so that the values' weights add up to one.
+constexpr float kLift = 14.f;
+
 struct PagedArgs {
   const half_t *q, *kp, *vp;
   const int32_t *table, *starts, *lens;
@@ -338,11 +345,11 @@ __global__ __launch_bounds__(256, 2) void paged_attention_rows_kernel(PagedArgs 
 #pragma unroll
       for (int h = 0; h < 2; ++h)
 #pragma unroll
-        for (int v = 0; v < 4; ++v) {
-          const float pv = exp2_hw((sc[h][v] - m_use) * a.scale_log2);
-          ls += pv;
-          pb[4 * h + v] = (half_t)pv;
-        }
+        for (int v = 0; v < 4; ++v)
+          pb[4 * h + v] = (half_t)exp2_hw(__builtin_fmaf(sc[h][v] - m_use, a.scale_log2, kLift));
+#pragma unroll
+      for (int e = 0; e < 8; e += 2)
+        ls = __builtin_amdgcn_fdot2(half2_t{pb[e], pb[e + 1]}, half2_t{(half_t)1.f, (half_t)1.f}, ls, false);
       l_run = l_run * alpha + ls;
       if (__builtin_amdgcn_ballot_w64(alpha != 1.f) != 0) {
 #pragma unroll
@@ -429,7 +436,8 @@ __global__ __launch_bounds__(256, 2) void paged_attention_rows_kernel(PagedArgs 
 // the two.  Six chunks also write and merge 82 MB of partial results.  Overlapping them within a wave, the next half block's keys
 // beside this half's exponentials, needs more registers than two waves leave
 // each (242 us with 247, 558 with spills, against 231 at the time).
-constexpr float kLag = 8.f;
+constexpr float kLag = 4.f;
+constexpr float kTileLift = kLift - kLag + 1.f;   // of the probabilities: up to 2^(kTileLift + kLag) = 2^15
 constexpr float kLarge = 4096.f;   // octaves
 constexpr int kTileRows = 128;
 constexpr int kTileKeys = 64;
@@ -622,8 +630,8 @@ __global__ __launch_bounds__(256, 2) void paged_attention_tile_kernel(PagedArgs 
       const float mb = max_halves(fmaxf(m2[0], m2[1]));
       // The reference of the exponents follows the largest score only once that
       // is kLag octaves ahead in some row (of 32 rows nearly every block would
-      // move one): the probabilities, at most 2^kLag, are as exact in fp16 and
-      // the sums in fp32 have room.
+      // move one): the probabilities, so much larger than those of the
+      // reference, are as exact in fp16 and the sums in fp32 have room.
       const float m_new = fmaxf(m_run, mb);   // of the raw scores, as in the kernel for small tiles
       if (__builtin_amdgcn_ballot_w64((m_new - m_run) * a.scale_log2 > kLag) != 0) {   // NaN while both are -inf
         const float alpha = exp2_hw((m_run - (m_new == -INFINITY ? 0.f : m_new)) * a.scale_log2);
@@ -638,10 +646,10 @@ __global__ __launch_bounds__(256, 2) void paged_attention_tile_kernel(PagedArgs 
       // less than the scores are, and it needs no instruction of its own (subtracting always: 219 us in place of 214 for
       // a 4096-token prompt).
       const float m_use = m_run == -INFINITY ? 0.f : m_run;
-      float m_scaled = m_use * a.scale_log2;
+      float m_scaled = __builtin_fmaf(m_use, a.scale_log2, -kTileLift);
       const bool large = !(fabsf(m_scaled) < kLarge);
       if (__builtin_amdgcn_ballot_w64(large) != 0) {
-        m_scaled = large ? 0.f : m_scaled;
+        m_scaled = large ? -kTileLift : m_scaled;
 #pragma unroll
         for (int kt = 0; kt < 2; ++kt)
 #pragma unroll

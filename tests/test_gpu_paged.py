@@ -323,6 +323,28 @@ def test_large_scores(gpu, count, past):
         assert ((got - want).abs() <= want.abs() * HALF_ULP + TINY).all()
 
 
+@pytest.mark.parametrize('octaves', [20, 24.5, 26.3, 28])
+@pytest.mark.parametrize('count', [1, 64])             # small tiles, large tiles
+def test_many_small_probabilities_beside_a_large_one(gpu, count, octaves):
+    """One key draws a query, 9000 others lie 20 to 28 octaves below: nothing each, and below fp16's subnormals as
+    fractions of the largest, but all there is of the result where the one key's value is 0."""
+    pool = Pool([count], [9000], hq=2, hkv=1, page=16, seed=count)
+    u = torch.randint(2, (D,), generator=pool.gen).float() * 2 - 1
+    scale = 1.0 / math.sqrt(D)
+    sink = (u * (octaves * math.log(2.0) / (D * scale))).half()
+    for i in range(9000 + count):
+        slot = pool.table[0, i // 16].item()
+        pool.k[slot, 0, i % 16] = sink if i == 4321 else 0.0
+        pool.v[slot, 0, i % 16] = 0.0 if i == 4321 else 1000.0 + 100.0 * pool.v[slot, 0, i % 16]
+    query = u.half().expand(count, 2, D).contiguous()
+    want, _ = expected_attention(pool, query, scale)
+    # The weights and their sum are of probabilities rounded by 2^-11 of each, or by 2^-36 of the largest, which is
+    # nearly all of the sum; the result is rounded once.  All terms are positive.
+    tol = want * 3 * HALF_ULP + TINY + 9100 * 2.0 ** -36 * 1500.0
+    k, v, batch = pool.to(gpu)
+    check(paged_attention(query.to(gpu), k, v, batch, scale=scale), want, tol)
+
+
 @pytest.mark.parametrize('count', [1, 40])
 def test_pages_beyond_32_bit_offsets(gpu, count):
     """Pages 2^30 elements apart: the last one starts 6 GiB into the pool."""

@@ -70,7 +70,8 @@ int wq_paged_attention_workspace_size(int64_t tokens, int64_t sequences, int64_t
 
 /* Grouped-query attention of the new tokens over their sequences' pages
  * (which hold the new tokens' keys and values already).
- *   q, out       [tokens, q_heads, 128] fp16, token-major
+ *   q, out       [tokens, q_heads, 128] fp16, token-major; out may be q itself
+ *                and must not overlap it otherwise
  *   tree_mask    NULL: token i of a sequence attends its positions up to its
  *                own.  Otherwise [tokens] int64: the new tokens are drafted
  *                ones that form a tree, every one attends all positions

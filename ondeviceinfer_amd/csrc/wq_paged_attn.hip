@@ -911,6 +911,10 @@ extern "C" int wq_paged_attention(const uint16_t* q, int64_t tokens, int64_t q_h
   WQ_REQUIRE(((uintptr_t)page_table | (uintptr_t)query_starts | (uintptr_t)seq_lens) % 4 == 0 &&
                  (uintptr_t)tree_mask % 8 == 0,
              WQ_ERR_INVALID_ARGUMENT, "integer operands must be aligned to their size");
+  // A workgroup reads its rows' queries before it writes the same rows; others may not have.
+  const uintptr_t in0 = (uintptr_t)q, out0 = (uintptr_t)out, bytes = (uintptr_t)(tokens * q_heads * kPagedDim * 2);
+  WQ_REQUIRE(out0 == in0 || out0 + bytes <= in0 || in0 + bytes <= out0, WQ_ERR_INVALID_ARGUMENT,
+             "out must be q itself or not overlap it");
   const PagedPlan plan = paged_plan(tokens, sequences, q_heads / kv_heads, kv_heads, table_width, page_size);
   WQ_REQUIRE(plan.bytes == 0 || (workspace && workspace_bytes >= plan.bytes && (uintptr_t)workspace % 16 == 0),
              WQ_ERR_WORKSPACE, "paged attention needs a 16-byte aligned workspace of %zu bytes (got %zu)", plan.bytes,

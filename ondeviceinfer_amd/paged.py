@@ -65,7 +65,8 @@ def paged_attention(query: Tensor, key_pages: Tensor, value_pages: Tensor, batch
     drafted ones: each attends everything before them, and of them those whose
     bit is set in its mask (its own bit included).  A token that attends
     nothing gets zeros, one that attends a position without a page NaN; rows
-    behind the last sequence keep what ``out`` held."""
+    behind the last sequence keep what ``out`` held.  ``out`` may be ``query``
+    itself and must not overlap it otherwise."""
     return _native.paged_attention(query, key_pages, value_pages, batch.page_table, batch.query_starts, batch.seq_lens,
                                    scale, tree_mask, out, workspace)
 

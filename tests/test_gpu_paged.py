@@ -182,6 +182,17 @@ def test_tree_attention(gpu, name):
     check(got, want, tol)
 
 
+@pytest.mark.parametrize('name', ['decode', 'decode-long', 'chunk-wide'])
+def test_queries_may_be_overwritten(gpu, name):
+    new, past, hq, hkv, page = BATCHES[name]
+    pool = Pool(new, past, hq=hq, hkv=hkv, page=page, seed=4)
+    k, v, batch = pool.to(gpu)
+    query = pool.rand(pool.tokens, hq, D).to(gpu)
+    want = paged_attention(query, k, v, batch, scale=0.1)
+    assert paged_attention(query, k, v, batch, scale=0.1, out=query) is query
+    assert torch.equal(query, want)
+
+
 LONG = {
     # name: (new, past, hq, hkv, page, tree): what of the kernels' loops it reaches that shorter sequences do not
     'more-chunks-than-lanes': ([1], [9000], 2, 1, 16, False),             # small tiles: 71 chunks, 64 of them at once

@@ -213,6 +213,15 @@ def test_append_refuses_queries_over_the_projection(out, code):
     assert status('wq_paged_append', *append_args(qkv=1 << 20, tokens=3, out=out)) == code
 
 
+@pytest.mark.parametrize('out,code', [
+    ((1 << 20) + 256, _native.WQ_ERR_INVALID_ARGUMENT),                  # a head further
+    ((1 << 20) - 3 * 4 * 256 + 16, _native.WQ_ERR_INVALID_ARGUMENT),     # its first 16 bytes
+    ((1 << 20) + 3 * 4 * 256, _native.WQ_ERR_WORKSPACE),                 # behind it: refused for the missing workspace
+    (1 << 20, _native.WQ_ERR_WORKSPACE)])                                # the queries themselves
+def test_attention_refuses_outputs_over_other_queries(out, code):
+    assert status('wq_paged_attention', *attention_args(q=1 << 20, tokens=3, out=out, width=200)) == code
+
+
 def sample_args(**change):
     a = dict(logits=16, kind=0, rows=2, vocab=100, stride=100, u=16, t=None, ta=1.0, k=None, ka=0, p=None, pa=1.0,
              m=None, ma=0.0, out=16, ws=16, wsb=1 << 30, stream=None)

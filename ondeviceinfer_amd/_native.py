@@ -1094,6 +1094,7 @@ def paged_attention(query: torch.Tensor, key_pages: torch.Tensor, value_pages: t
 
 # ----------------------------------------------------------------------------- sampling
 
+_FLOAT_MAX = torch.finfo(torch.float32).max
 _LOGITS = {torch.float16: 0, torch.float32: 1}
 
 
@@ -1133,7 +1134,7 @@ def sample(logits: torch.Tensor, uniform: torch.Tensor, temperature=1.0, top_k=0
     k_ptr, k_all = _setting(top_k, torch.int32, rows, 'top_k')
     p_ptr, p_all = _setting(top_p, torch.float32, rows, 'top_p')
     m_ptr, m_all = _setting(min_p, torch.float32, rows, 'min_p')
-    if t_ptr is None and not 0.0 <= t_all < float('inf'):
+    if t_ptr is None and not 0.0 <= t_all <= _FLOAT_MAX:   # it travels as fp32
         raise ValueError(f'temperature must be finite and not negative, got {t_all}')
     if (p_ptr is None and p_all != p_all) or (m_ptr is None and m_all != m_all):
         raise ValueError('top_p and min_p must be numbers')

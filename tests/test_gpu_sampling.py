@@ -307,6 +307,13 @@ def test_top_p_behind_a_top_k_that_ends_in_a_full_bin(gpu, vocab, dtype):
     compare(run(gpu, logits.to(gpu), u, asks), logits, u, asks)
 
 
+def test_a_temperature_beyond_fp32_is_refused(gpu):
+    logits, u = torch.tensor([[0.0, 1.0]], device=gpu), torch.zeros(1, device=gpu)
+    with pytest.raises(ValueError, match='temperature'):
+        sample_tokens(logits, u, temperature=1e39)
+    assert sample_tokens(logits, u, temperature=3e38).tolist() == [0]      # both weigh 1
+
+
 def test_a_workspace_without_memory_of_its_own_is_refused(gpu):
     with pytest.raises(ValueError, match='contiguous'):
         sample_tokens(torch.zeros(4, 10, device=gpu), torch.zeros(4, device=gpu),

@@ -201,6 +201,17 @@ def _check(t: torch.Tensor, dtype: torch.dtype, shape: tuple, name: str) -> None
         raise ValueError(f'{name}: must be contiguous')
 
 
+def _scratch(workspace: torch.Tensor) -> tuple[int, int]:
+    """(pointer, bytes) of a caller's workspace; an expanded tensor would count bytes it does not have."""
+    if not workspace.is_contiguous():
+        raise ValueError(f'workspace must be contiguous, got strides {workspace.stride()}')
+    return workspace.data_ptr(), workspace.numel() * workspace.element_size()
+
+
+def _ws_args(workspace: torch.Tensor | None) -> tuple[int | None, int]:
+    return (None, 0) if workspace is None else _scratch(workspace)
+
+
 def _aligned(t: torch.Tensor) -> torch.Tensor:
     return t if t.data_ptr() % 16 == 0 else t.clone()
 
@@ -388,7 +399,7 @@ def shared_workspace(device: torch.device, nbytes: int, layout: tuple, zeroed: i
 def w4a16_linear(x: torch.Tensor, tiles: torch.Tensor, meta: torch.Tensor, n: int, group_size: int,
                  out: torch.Tensor | None = None, workspace: torch.Tensor | None = None) -> torch.Tensor:
     """``y[m, n] = x[m, k] . dequant(W)^T`` on the repacked weight."""
-    device = _require_gpu(x, tiles, meta, out)
+    device = _require_gpu(x, tiles, meta, out, workspace)
     if x.dtype != torch.float16 or x.dim() != 2:
         raise TypeError(f'x must be a 2-D float16 tensor, got {x.dtype} {tuple(x.shape)}')
     m, k = x.shape
@@ -408,9 +419,7 @@ def w4a16_linear(x: torch.Tensor, tiles: torch.Tensor, meta: torch.Tensor, n: in
             # M > 4: the counters sit in a fixed region at the front and are
             # zero after every call, so all such shapes share one buffer.
             workspace = shared_workspace(device, nbytes, ('w4a16', m, n, k, group_size) if m <= 4 else ('w4a16-split',), zeroed)
-    ws_ptr, ws_bytes = None, 0
-    if workspace is not None:
-        ws_ptr, ws_bytes = workspace.data_ptr(), workspace.numel() * workspace.element_size()
+    ws_ptr, ws_bytes = _ws_args(workspace)
     _call('wq_w4a16_linear', _ptr(x), m, k, _ptr(tiles), _ptr(meta), n, group_size, _ptr(out), ws_ptr, ws_bytes,
           _stream(device))
     return out
@@ -528,12 +537,6 @@ def _decode_fused_args(x, n, x_mode, norm_weight, sumsq_in, residual, sumsq_out,
     elif out.dtype != torch.float16 or out.numel() != n or not out.is_contiguous():
         raise ValueError(f'out must be contiguous float16 with {n} elements')
     return k, out
-
-
-def _ws_args(workspace):
-    if workspace is None:
-        return None, 0
-    return workspace.data_ptr(), workspace.numel() * workspace.element_size()
 
 
 def w4a16_decode_fused(x: torch.Tensor, tiles: torch.Tensor, meta: torch.Tensor, n: int, group_size: int, *,
@@ -662,7 +665,7 @@ def w8a16_linear(x: torch.Tensor, qweight, scale: torch.Tensor, bias: torch.Tens
     """``y = x . (q * scale)^T (+ bias)`` straight from the INT8 weight:
     row-major [n, k] (``wq_w8a16_linear``) or ``W8Tiles`` (``wq_w8a16_linear_tiled``)."""
     n, k, q, tiled = _w8_weight(qweight)
-    device = _require_gpu(x, q, scale, bias, out)
+    device = _require_gpu(x, q, scale, bias, out, workspace)
     if x.dtype != torch.float16 or x.dim() != 2:
         raise TypeError(f'x must be a 2-D float16 tensor, got {x.dtype} {tuple(x.shape)}')
     if x.shape[1] != k:
@@ -682,9 +685,7 @@ def w8a16_linear(x: torch.Tensor, qweight, scale: torch.Tensor, bias: torch.Tens
             workspace = shared_workspace(device, nbytes, ('w8a16', m, n, k))
         else:   # split partials only (no counters): any scratch of this call's own
             workspace = x.new_empty(nbytes, dtype=torch.uint8)
-    ws_ptr, ws_bytes = None, 0
-    if workspace is not None:
-        ws_ptr, ws_bytes = workspace.data_ptr(), workspace.numel() * workspace.element_size()
+    ws_ptr, ws_bytes = _ws_args(workspace)
     _call('wq_w8a16_linear_tiled' if tiled else 'wq_w8a16_linear', _ptr(x), m, k, _ptr(q), _ptr(scale.contiguous()), n,
           _ptr(None if bias is None else bias.contiguous()), _ptr(out), ws_ptr, ws_bytes, _stream(device))
     return out
@@ -830,8 +831,7 @@ def decode_attention(qkv: torch.Tensor, q_heads: int, kv_heads: int, q_norm: tor
     need = decode_attention_workspace_size(q_heads, kv_heads, head_dim, max_seq)
     if workspace is None and need:
         workspace = shared_workspace(device, need, ('attention', q_heads, kv_heads, max_seq))
-    ws_ptr, ws_bytes = (None, 0) if workspace is None else (workspace.data_ptr(),
-                                                             workspace.numel() * workspace.element_size())
+    ws_ptr, ws_bytes = _ws_args(workspace)
     _call('wq_decode_attention', _ptr(qkv), q_heads, kv_heads, head_dim, _ptr(q_norm), _ptr(k_norm), float(eps),
           _ptr(cos_table), _ptr(sin_table), _ptr(position), _ptr(key_cache), _ptr(value_cache), max_seq,
           float(scale), _ptr(out), ws_ptr, ws_bytes, _stream(device))
@@ -932,8 +932,7 @@ def lm_head(x: torch.Tensor, weight: torch.Tensor, *, logits: torch.Tensor | Non
         raise ValueError('token must be one contiguous int64')
     if workspace is None and token is not None:
         workspace = shared_workspace(device, lm_head_workspace_size(k, vocab), ('lm_head', k, vocab))
-    ws_ptr, ws_bytes = (None, 0) if workspace is None else (workspace.data_ptr(),
-                                                             workspace.numel() * workspace.element_size())
+    ws_ptr, ws_bytes = _ws_args(workspace)
     if norm_weight is None:
         _call('wq_lm_head', _ptr(_aligned(x)), k, _ptr(weight), vocab, _ptr(logits), _ptr(token), ws_ptr, ws_bytes,
               _stream(device))
@@ -968,8 +967,7 @@ def argmax_f16(x: torch.Tensor, *, out: torch.Tensor | None = None,
         raise ValueError('out must be one contiguous int64')
     if workspace is None:
         workspace = shared_workspace(device, argmax_f16_workspace_size(n), ('argmax_f16', n))
-    _call('wq_argmax_f16', _ptr(_aligned(x)), n, _ptr(out), workspace.data_ptr(),
-          workspace.numel() * workspace.element_size(), _stream(device))
+    _call('wq_argmax_f16', _ptr(_aligned(x)), n, _ptr(out), *_scratch(workspace), _stream(device))
     return out
 
 
@@ -984,13 +982,6 @@ def _page_stride(t: torch.Tensor, name: str) -> int:
     if stride[1:] != (rows * dim, dim, 1) and not t[:1].is_contiguous():
         raise ValueError(f'{name}: a page [{heads}, {rows}, {dim}] must be contiguous')
     return stride[0] if t.shape[0] > 1 else heads * rows * dim
-
-
-def _scratch(workspace: torch.Tensor) -> tuple[int, int]:
-    """(pointer, bytes) of a caller's workspace; an expanded tensor would count bytes it does not have."""
-    if not workspace.is_contiguous():
-        raise ValueError(f'workspace must be contiguous, got strides {workspace.stride()}')
-    return workspace.data_ptr(), workspace.numel() * workspace.element_size()
 
 
 def _check_batch(page_table: torch.Tensor, query_starts: torch.Tensor, seq_lens: torch.Tensor) -> tuple[int, int]:

@@ -182,6 +182,54 @@ def test_tree_attention(gpu, name):
     check(got, want, tol)
 
 
+def test_as_many_sequences_as_a_call_takes(gpu):
+    """65536 sequences of one new token each over one shared page, 1 to 16 positions; then an append
+    whose last 16 tokens are one sequence's, the others alone in theirs."""
+    n = 65536
+    gen = torch.Generator().manual_seed(31)
+    k, v = torch.randn(2, 1, 1, 16, D, generator=gen).half().unbind(0)
+    query = torch.randn(n, 1, D, generator=gen).half()
+    length = torch.arange(n) % 16 + 1
+    batch = PagedBatch(*(t.to(torch.int32).to(gpu) for t in (torch.zeros(n, 1), torch.arange(n + 1), length)))
+    got = paged_attention(query.to(gpu), k.to(gpu), v.to(gpu), batch, scale=0.1)
+    scores = query[:, 0].double() @ k[0, 0].double().t() * 0.1
+    p = torch.softmax(scores.masked_fill(torch.arange(16) >= length[:, None], float('-inf')), dim=1)
+    want = p @ v[0, 0].double()
+    # As for the other tests: the probabilities' rounding, their sum's and the result's, 16 scores of a size below 16.
+    tol = (p @ v[0, 0].double().abs()) * (HALF_ULP + 2 * 130 * 2.0 ** -24 * 16) + 2 * want.abs() * HALF_ULP + TINY
+    check(got[:, 0], want, tol)
+    cos, sin = tables(16)
+    qkv = torch.randn(n, 3 * D, generator=gen).half().to(gpu)
+    starts = torch.full((n + 1,), n, dtype=torch.int32, device=gpu)     # n - 15 and on: no tokens
+    starts[:n - 15] = torch.arange(n - 15, device=gpu)
+    lens = torch.full((n,), 1, dtype=torch.int32, device=gpu)
+    lens[n - 16] = 16
+    pages = torch.zeros(2, 1, 1, 16, D, dtype=torch.float16, device=gpu)
+    paged_append(qkv, pages[0], pages[1], PagedBatch(batch.page_table, starts, lens), q_heads=1, q_norm=None, k_norm=None,
+                 eps=1e-6, cos_table=cos.to(gpu), sin_table=sin.to(gpu))
+    assert torch.equal(pages[1, 0, 0, 1:], qkv[n - 15:, 2 * D:])
+
+
+WIDE = {
+    'page-1024': ([1, 3, 70], [1500, 1021, 1000], 4, 2, 1024),
+    'page-4112': ([1, 2], [4111, 10], 4, 2, 4112),
+    'group-16-large-tiles': ([37, 1, 20], [60, 300, 0], 16, 1, 16),
+    'group-7': ([60, 9], [45, 333], 14, 2, 16),
+}
+
+
+@pytest.mark.parametrize('name', list(WIDE))
+def test_long_pages_and_wide_groups(gpu, name):
+    new, past, hq, hkv, page = WIDE[name]
+    print(name, flush=True)
+    pool = Pool(new, past, hq=hq, hkv=hkv, page=page, seed=len(name))
+    query = pool.rand(pool.tokens, hq, D, scale=1.5)
+    scale = 1.0 / math.sqrt(D)
+    want, tol = expected_attention(pool, query, scale)
+    k, v, batch = pool.to(gpu)
+    check(paged_attention(query.to(gpu), k, v, batch, scale=scale), want, tol)
+
+
 @pytest.mark.parametrize('name', ['decode', 'decode-long', 'chunk-wide'])
 def test_queries_may_be_overwritten(gpu, name):
     new, past, hq, hkv, page = BATCHES[name]

@@ -307,6 +307,28 @@ def test_top_p_behind_a_top_k_that_ends_in_a_full_bin(gpu, vocab, dtype):
     compare(run(gpu, logits.to(gpu), u, asks), logits, u, asks)
 
 
+def test_as_many_tokens_as_a_row_may_have(gpu):
+    """2^30 equal logits: every sum is exact, u = j / 2^24 draws token 64 j."""
+    j = torch.tensor([0, 1, 16383, 8388608, 16777215])
+    logits = torch.full((1, 1 << 30), 0.5, dtype=torch.float16, device=gpu)
+    u = (j.float() / 2 ** 24).to(gpu)
+    got = torch.cat([sample_tokens(logits, u[i:i + 1]) for i in range(len(j))])
+    assert torch.equal(got.cpu(), 64 * j)
+    row = logits[:, :1 << 24]
+    got = torch.cat([sample_tokens(row, u[i:i + 1], min_p=0.5) for i in range(len(j))])
+    assert torch.equal(got.cpu(), j)
+
+
+def test_as_many_rows_as_a_call_takes(gpu):
+    rows = 65535
+    u = torch.rand(rows, generator=torch.Generator().manual_seed(22)).to(gpu)
+    logits = torch.zeros(rows, 17, device=gpu)
+    logits[:, 16] = -float('inf')
+    assert torch.equal(sample_tokens(logits, u), (u * 16).long())
+    assert torch.equal(sample_tokens(logits, u, top_k=8), (u * 8).long())
+    assert torch.equal(sample_tokens(logits, u, top_p=0.25), (u * 4).long())
+
+
 def test_a_temperature_beyond_fp32_is_refused(gpu):
     logits, u = torch.tensor([[0.0, 1.0]], device=gpu), torch.zeros(1, device=gpu)
     with pytest.raises(ValueError, match='temperature'):

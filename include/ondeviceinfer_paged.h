@@ -49,8 +49,8 @@ extern "C" {
  * in fp32 and rounded to fp16 once.  A token whose index has no page (a
  * negative index, one past the table's width, a page number outside the pool)
  * or whose position is outside the tables gets NaN in q_out and writes
- * nothing to the pages.  Two tokens that name the same page row leave one of
- * the two there.
+ * nothing to the pages.  Of two tokens that name the same page row either's
+ * elements are left there, eight at a time.
  * Replaces, for a batch: q/k rms_norm + apply_rotary_pos_emb + cache.update
  * (quantized_model.py:177-195, layers.py:64-80, cache.py:60-80). */
 int wq_paged_append(const uint16_t* qkv, int64_t tokens, int64_t q_heads, int64_t kv_heads, int64_t head_dim,

@@ -21,7 +21,10 @@ extern "C" {
 #define WQ_LOGITS_F32 1
 
 /* Workspace bytes for wq_sample (no initialization needed; calls that may
- * overlap need separate workspaces). */
+ * overlap need separate workspaces).  Nearly all of it is a list per row, 8
+ * bytes per token of the vocabulary while that comes to at most 64 MiB for all
+ * rows, and at least 4096 tokens a row: 64 rows of 151936 take 64 MiB, 65535
+ * rows 2 GiB. */
 int wq_sample_workspace_size(int64_t rows, int64_t vocab, size_t* bytes);
 
 /* tokens[r] = one token drawn from row r of logits [rows, vocab] (row_stride
@@ -35,7 +38,10 @@ int wq_sample_workspace_size(int64_t rows, int64_t vocab, size_t* bytes);
  *   the first token of the order always stays.
  * The token is the first of the remaining ones, by index, at which their
  * running weight exceeds uniform[r] times their whole weight.  Weights and
- * sums are 64-bit.  temperature 0 takes the first token of the order.
+ * sums are 64-bit; those of the tokens within a few octaves of a cut are added
+ * as whole numbers of 2^-b of a power of two next to the largest of them, b =
+ * 63 - log2(vocab) rounded up and 50 at the most (45 for 151936 tokens).
+ * temperature 0 takes the first token of the order.
  * The settings are per-row device arrays; NULL takes the scalar for all rows.
  * A row has no distribution, and its token is -1, when it holds NaN or nothing
  * above -inf, or when its uniform, temperature (negative or not finite), top_p

@@ -216,8 +216,8 @@ __device__ __forceinline__ uint4_t stream_load(const half_t* p) {
 // The next step's keys are requested as soon as the scores have consumed the
 // present ones, the values likewise, so that both are in flight during the
 // softmax of the other.  Bound by the cache's bytes: 2.27 GB of 64 sequences in
-// 375 us, 6.1 TB/s with 160 registers and three workgroups per compute unit;
-// one sequence of 4101 positions (16.8 MB) by latency, 9 us and 6 more for the
+// 374 us, 6.1 TB/s with 158 registers and three workgroups per compute unit;
+// one sequence of 4101 positions (16.8 MB) by latency, 9 to 10 us and 6 for the
 // merge: the starts, the page numbers, the keys, the values one after another.
 template <bool ONCE>
 __global__ __launch_bounds__(256, 2) void paged_attention_rows_kernel(PagedArgs a) {
@@ -430,12 +430,13 @@ __global__ __launch_bounds__(256, 2) void paged_attention_rows_kernel(PagedArgs 
 // of row ql, and the probabilities, rounded to fp16, are the B operand of O^T
 // = V^T . P^T once V^T's key slots follow the same order: slot 8 h + 4 j + e
 // of a 16-key step holds key 8 j + 4 h + e.  A 4096-token
-// prompt takes 219 us, 0.79 PFLOP/s: matrix cores busy in 36 % of the cycles,
-// vector instructions in 41 %, waves waiting in 25 % of theirs, no bank
-// conflicts.  Neither unit is full: two waves per SIMD are not enough to overlap
-// the two.  Six chunks also write and merge 82 MB of partial results.  Overlapping them within a wave, the next half block's keys
-// beside this half's exponentials, needs more registers than two waves leave
-// each (242 us with 247, 558 with spills, against 231 at the time).
+// prompt takes 214 to 224 us from card to card, 0.77 to 0.80 PFLOP/s: matrix
+// cores busy in 35 % of the cycles, vector instructions in 41 %, waves waiting
+// in 26 % of theirs, no bank conflicts.  Neither unit is full: two waves per SIMD are not enough to overlap
+// the two.  Overlapping them within a wave, the next half block's keys beside
+// this half's exponentials, needs more registers than two waves leave each (242
+// us with 247, 558 with spills, against 231 at the time).  Six chunks also write
+// and merge 82 MB of partial results.
 constexpr float kLag = 4.f;
 constexpr float kTileLift = kLift - kLag + 1.f;   // of the probabilities: up to 2^(kTileLift + kLag) = 2^15
 constexpr float kLarge = 4096.f;   // octaves
@@ -839,9 +840,10 @@ struct PagedPlan {
 
 PagedPlan paged_plan(int64_t tokens, int64_t sequences, int64_t G, int64_t KV, int64_t width, int64_t page_size) {
   PagedPlan p{};
-  // On average more than 48 rows per sequence take the large tiles, with the merge 16 us and up: 7 tokens of 40 / 8
-  // heads behind 4000 take 15.9 us in small tiles and 18.5 in large ones, 10 take 22.3 and 19.8 (batch 8: 10 tokens
-  // 39.0 and 38.1, 16 tokens 50.0 and 45.3).
+  // On average more than 48 rows per sequence take the large tiles.  40 / 8 heads behind 4000 positions, us in small and
+  // in large tiles: one sequence of 6 tokens 14.9 and 16.2, 10 tokens 18.5 and 18.4, 20 tokens 21.6 and 23.7; eight
+  // sequences of 3 tokens 37.1 and 36.2, 7 tokens 51 and 42, 20 tokens 88 and 55.  One line for both costs the single
+  // sequence up to 2 us above it and a batch up to 10 below.
   p.rows = tokens * G > 48 * sequences ? kTileRows : 16;
   // sum_b ceil(count_b G / R) <= ceil(tokens G / R) + sequences, and no more tiles than rows.
   p.tiles = (tokens * G + p.rows - 1) / p.rows + sequences;
@@ -947,8 +949,8 @@ extern "C" int wq_paged_attention(const uint16_t* q, int64_t tokens, int64_t q_h
   a.spare = (int)plan.spare;
   a.min_blocks = plan.min_blocks;
   const dim3 grid((unsigned)(plan.slots * kv_heads));
-  // One tile per sequence on average: single tokens.  64 long sequences 424 us, with non-temporal loads 397; seven
-  // drafted tokens, three tiles that share their keys through the L2, 17.5 and 18.6.
+  // One tile per sequence on average: single tokens.  64 long sequences 424 us, with non-temporal loads 397 (380 with
+  // more chunks too); seven drafted tokens, three tiles that share their keys through the L2, 17.5 and 18.6.
   if (plan.rows == 16 && tokens * a.G <= 16 * sequences)
     hipLaunchKernelGGL(paged_attention_rows_kernel<true>, grid, dim3(256), 0, as_stream(stream), a);
   else if (plan.rows == 16)

@@ -17,13 +17,13 @@
 // bits and summed in a fixed order: over 151936 normal logits a 32-bit
 // sum in blocks of 512 changes the token of one to three rows in a hundred, a
 // running one of a quarter to a third (numpy, 400 rows each, deviations 0.1 to 3).
-// 64 rows of 151936 fp16 logits (19 MB): tally 26 us (51 vector
-// instructions per token counted, some 19 of them 64-bit; the vector units issue
-// in 39 % of the cycles and waves wait in 43 %, so neither alone is the bound),
-// gather 15, pick 25 in nine draws of twelve.  The pick's time is its slowest
-// row's: 78 to 81 us where top-p ends among 44 thousand tokens of one bin (the
-// weights of them all, by one workgroup), 140 where top-k of a peaked row ends
-// among nearly the whole vocabulary.  One row takes 7, 9 and 16 us.
+// 64 rows of 151936 fp16 logits (19 MB): tally 26 to 27 us (55 vector
+// instructions per token counted, 24 of them 64-bit; the vector units issue in
+// 41 % of the cycles and waves wait in 41 %, so neither alone is the bound),
+// gather 15, pick 24 to 29 in nine draws of twelve.  The pick's time is its
+// slowest row's: 80 to 84 us where top-p ends among 44 thousand tokens of one
+// bin (the weights of them all, by one workgroup), 141 where top-k of a peaked
+// row ends among nearly the whole vocabulary.  One row takes 7, 9 and 17 us.
 #include "ondeviceinfer_sample.h"
 #include "wq_common.h"
 #include "wq_status.h"
@@ -638,8 +638,9 @@ struct Cut {
 // by two comparisons in place of its position in 64 bits, which costs every pass
 // about 650 cycles per 1024 tokens.  The bounds cost some 8 us to find, so only
 // lists longer than kBounded are searched between them: 64 rows of which one
-// lists all 151936 tokens take 198 us instead of 238 (180 with bins of few
-// tokens sorted at once), ordinary ones 75 with bounds always and 66 without.
+// lists all 151936 tokens took 198 us instead of 238 (183 now that bins of few
+// tokens are sorted at once), ordinary ones 75 with bounds always and 66 without
+// (now 67 to 72).
 struct Span {
   float least, above;   // above NaN: no bound
   __device__ __forceinline__ bool has(float v) const { return (v >= least) & !(v >= above); }

@@ -104,8 +104,10 @@ def sample_generate(model, prompts, *, max_new_tokens: int, cache, temperature=1
     or a device tensor with one entry per prompt); ``generator`` (of the model's
     device) makes a run repeatable.  A sequence ends at ``max_new_tokens`` or
     with ``eos_token_id``, which is kept, or before a token that its row of
-    logits does not allow (-1).  Its pages go back to the cache when it ends;
-    without an ``eos_token_id`` the host waits only once, at the end."""
+    logits does not allow (-1).  Its pages go back to the cache when it ends.
+    The tokens are read after every step with an ``eos_token_id`` and once, at
+    the end, without; every step's page numbers go to the device in a copy that
+    waits for the step before it in either case."""
     prompts = [torch.as_tensor(p, dtype=torch.long).reshape(-1) for p in prompts]
     if not prompts or any(p.numel() == 0 for p in prompts):
         raise ValueError('every prompt needs at least one token')

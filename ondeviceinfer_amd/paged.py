@@ -47,6 +47,7 @@ def paged_append(qkv: Tensor, key_pages: Tensor, value_pages: Tensor, batch: Pag
     ``q_norm`` / ``k_norm`` may be None (no norm).  A token is rotated by row
     ``positions[token]`` of the tables, its index in the sequence by default.
     A token without a page or a table row gets NaN queries and writes nothing;
+    of two that name the same row of a page the elements of either are left;
     rows behind the last sequence keep what ``out`` held.  ``out`` must not
     overlap ``qkv``."""
     return _native.paged_append(qkv, q_heads, q_norm, k_norm, eps, cos_table, sin_table, key_pages, value_pages,

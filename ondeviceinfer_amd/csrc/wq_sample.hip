@@ -523,14 +523,15 @@ struct Key<float> {
 };
 
 // The smallest value for which `holds` (which stays true as values rise), found
-// by the wave 64 keys at a time.
+// by the wave 64 keys at a time; NaN, the key next above +inf, if there is none
+// (the bins above that of a row's infinite logits hold nothing).
 template <typename T, typename F>
 __device__ __forceinline__ float lowest_where(int lane, F holds) {
-  uint32_t lo = Key<T>::kLowest, n = Key<T>::kHighest - Key<T>::kLowest + 1;   // the key lies in lo .. lo + n - 1
-  while (n > 1) {
+  uint32_t lo = Key<T>::kLowest, n = Key<T>::kHighest - Key<T>::kLowest + 2;   // the key lies in lo .. lo + n - 1
+  while (n > 1) {   // n falls to a 64th, never below 1: the last key is taken to hold, whatever it and those beyond say
     const uint32_t step = (n + 63) / 64;
-    const uint32_t k = min(lo + lane * step, Key<T>::kHighest);
-    const uint64_t in = __builtin_amdgcn_ballot_w64(holds(Key<T>::value(k)));
+    const uint32_t k = lane * step;
+    const uint64_t in = __builtin_amdgcn_ballot_w64((k >= n - 1) | holds(Key<T>::value(lo + min(k, n - 1))));
     // The first probe that is in, or the stretch behind the last one.
     const int first = in ? __builtin_ctzll(in) : 64;
     if (first == 0) return Key<T>::value(lo);
@@ -542,7 +543,7 @@ __device__ __forceinline__ float lowest_where(int lane, F holds) {
   return Key<T>::value(lo);
 }
 
-// The smallest value whose bin is at most `bin` (bins fall as values rise).
+// The smallest value whose bin is at most `bin` (bins fall as values rise), NaN if there is none.
 template <typename T>
 __device__ __forceinline__ float lowest_of(const Scale& s, int bin, int lane) {
   return lowest_where<T>(lane, [&](float v) { return bin_at(s.below(s.y(v))) <= bin; });

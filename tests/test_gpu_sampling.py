@@ -197,6 +197,25 @@ def test_masked_and_infinite_logits(gpu):
         assert got[1] == -1 and got[2] == -1 and got[4] == 77 and got[6] == 0
 
 
+@pytest.mark.parametrize('kind', ['none', 'top_k', 'top_p', 'min_p', 'both', 'all'])
+@pytest.mark.parametrize('dtype', [torch.float16, torch.float32])
+@pytest.mark.parametrize('rows,vocab,share', [(2, 60, 0.1), (3, 5000, 0.0), (40, 5000, 0.01), (200, 30000, 0.9)])
+def test_infinite_logits_with_every_filter(gpu, rows, vocab, share, dtype, kind):
+    """+inf in one token (share 0) up to most of a row: the bins above theirs hold no value at all.  fp16 logits overflow to
+    it."""
+    print(rows, vocab, share, dtype, kind, flush=True)
+    gen = torch.Generator().manual_seed(rows + vocab)
+    logits = torch.randn(rows, vocab, generator=gen) * 3.0
+    logits[torch.rand(rows, vocab, generator=gen) < share] = float('inf')
+    logits[torch.arange(rows), torch.randint(vocab, (rows,), generator=gen)] = 1e6 if dtype == torch.float16 else float('inf')
+    logits[:, ::7] = -float('inf')
+    logits[:, -1] = float('inf')
+    logits = logits.to(dtype)
+    u = torch.rand(rows, generator=gen)
+    asks = settings(rows, kind, np.random.default_rng(rows))
+    compare(run(gpu, logits.to(gpu), u, asks), logits, u, asks)
+
+
 def test_settings_without_a_meaning_give_minus_one(gpu):
     nan, inf = float('nan'), float('inf')
     logits = torch.randn(8, 300, generator=torch.Generator().manual_seed(6)).to(gpu)

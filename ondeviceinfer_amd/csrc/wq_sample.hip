@@ -1017,7 +1017,10 @@ __global__ __launch_bounds__(kPickThreads) void sample_pick_kernel(SampleArgs a)
       const double y = s.y(v);
       if (bin_at(s.below(y)) != edge) return;
       const int st = stays(v, y);
-      if (st == 1) m += (unsigned long long)rint(pick.weight_of(v) * unit);
+      if (st == 1) {   // what weighs anything counts for something: the last bin has no end
+        const double w = pick.weight_of(v);
+        m += w > 0.0 ? (unsigned long long)fmax(rint(w * unit), 1.0) : 0ull;
+      }
       ties += st == 2;
     };
     if (p < a.parts && edge < kBins && sh.tally.part_count[p][edge] != 0) {

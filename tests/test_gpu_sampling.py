@@ -216,6 +216,19 @@ def test_infinite_logits_with_every_filter(gpu, rows, vocab, share, dtype, kind)
     compare(run(gpu, logits.to(gpu), u, asks), logits, u, asks)
 
 
+@pytest.mark.parametrize('dtype', [torch.float16, torch.float32])
+@pytest.mark.parametrize('rows,vocab', [(2, 3000), (24, 3000), (6, 60000)])
+def test_zero_draws_the_first_token_that_stays(gpu, rows, vocab, dtype):
+    """u = 0: the first kept token with any weight in 64 bits, were it 2^-1000 beside the largest."""
+    print(rows, vocab, dtype, flush=True)
+    gen = torch.Generator().manual_seed(vocab)
+    logits = (torch.randn(rows, vocab, generator=gen) * torch.linspace(2.0, 60.0, rows)[:, None]).to(dtype)
+    u = torch.zeros(rows)
+    for top_k in (0, 10, 300, 2000):
+        asks = [((1.0, 0.4)[r % 2], top_k, 1.0, 0.0) for r in range(rows)]
+        compare(run(gpu, logits.to(gpu), u, asks), logits, u, asks)
+
+
 def test_settings_without_a_meaning_give_minus_one(gpu):
     nan, inf = float('nan'), float('inf')
     logits = torch.randn(8, 300, generator=torch.Generator().manual_seed(6)).to(gpu)
